@@ -47,7 +47,9 @@ def _flags():
     # extra preprocessor defines for same-box A/B builds of a variant copy (e.g.
     # PGDIST_DEFINES="NAME=VALUE ..."); empty for the in-tree build
     common += ["-D" + d for d in os.environ.get("PGDIST_DEFINES", "").split()]
-    hip = common + [f"--offload-arch={ARCH}", "-x", "hip", "-munsafe-fp-atomics"]
+    # no packed fp32 arithmetic (v_pk_{add,mul,fma}_f32): some of its forms have returned wrong results
+    hip = common + [f"--offload-arch={ARCH}", "-x", "hip", "-munsafe-fp-atomics",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     # host translation units (bindings, runtime) contain no kernels; target gfx950 only as well
     host = common + [f"--offload-arch={ARCH}", "-fvisibility=hidden"] + ["-I" + p for p in _pybind_includes()]
     return hip, host

@@ -108,6 +108,18 @@ void wgrad_reduce_flush(hipStream_t st);
 long long bn_part_floats(int, int);
 void register_side_stream(hipStream_t);
 void launch_reduce_metrics(const float *, const float *, int, double *, hipStream_t);
+// ---- group norm, 8-bit activation checkpoints (groupnorm.hip, mx8.hip) ----
+long long gn_workspace_floats(int, long long, long long, int, int, int);
+void launch_gn_fwd(int, const void *, const float *, const float *, void *, float *, float *, uint8_t *, uint8_t *,
+                   float *, long long, long long, int, int, float, int, hipStream_t);
+void launch_gn_bwd(int, const void *, const void *, const uint8_t *, const uint8_t *, const float *, const float *,
+                   const float *, const float *, void *, float *, float *, long long, long long, int, int, int,
+                   hipStream_t);
+void launch_mx8_pack(int, const void *, uint8_t *, uint8_t *, long long, int, hipStream_t);
+void launch_mx8_unpack(int, const uint8_t *, const uint8_t *, void *, long long, int, hipStream_t);
+long long mx8_wgrad_workspace_floats(int, int, int);
+void launch_mx8_wgrad(int, const void *, const uint8_t *, const uint8_t *, float *, float *, float *, int, int, int,
+                      hipStream_t);
 // ---- dense convolutions (ResNet-50), kernels/conv.hip ----
 int conv_fwd_num_partials(int, int, int, int, int, int);
 int conv_dgrad_num_partials(int, int, int, int, int, int, int, int);
@@ -160,6 +172,12 @@ static std::string last_error() {
   return e == hipSuccess ? std::string() : std::string(hipGetErrorString(e));
 }
 
+// a launch the runtime refused raises in the caller
+static void launched(const char *what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": launch failed: " + hipGetErrorString(e));
+}
+
 PYBIND11_MODULE(_pgdist_C, m) {
   m.doc() = "pgdist native library: gfx950 HIP kernels + C++ runtime";
   m.attr("arch") = "gfx950";
@@ -190,6 +208,45 @@ PYBIND11_MODULE(_pgdist_C, m) {
     pgdist_rt::run_op([=] {
       launch_bn_apply(ptr<bf16_t>(y), ptr<bf16_t>(res), ptr<float>(scale), ptr<float>(shift),
                       ptr<bf16_t>(out), M, C, relu6, S(s));
+    });
+  });
+  // ---- group norm, 8-bit activation checkpoints ----
+  m.def("gn_workspace_floats", &gn_workspace_floats);
+  m.def("gn_fwd", [](int dt, P x, P gamma, P beta, P y, P mean, P rstd, P q, P qs, P ws, long long B, long long S_,
+                     int C, int G, float eps, int act, P s) {
+    pgdist_rt::run_op([=] {
+      launch_gn_fwd(dt, ptr<void>(x), ptr<float>(gamma), ptr<float>(beta), ptr<void>(y), ptr<float>(mean),
+                    ptr<float>(rstd), ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<float>(ws), B, S_, C, G, eps, act, S(s));
+      launched("gn_fwd");
+    });
+  });
+  m.def("gn_bwd", [](int dt, P dy, P x, P q, P qs, P gamma, P beta, P mean, P rstd, P dx, P dgb, P ws, long long B,
+                     long long S_, int C, int G, int act, P s) {
+    pgdist_rt::run_op([=] {
+      launch_gn_bwd(dt, ptr<void>(dy), ptr<void>(x), ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<float>(gamma),
+                    ptr<float>(beta), ptr<float>(mean), ptr<float>(rstd), ptr<void>(dx), ptr<float>(dgb),
+                    ptr<float>(ws), B, S_, C, G, act, S(s));
+      launched("gn_bwd");
+    });
+  });
+  m.def("mx8_pack", [](int dt, P x, P q, P qs, long long M, int C, P s) {
+    pgdist_rt::run_op([=] {
+      launch_mx8_pack(dt, ptr<void>(x), ptr<uint8_t>(q), ptr<uint8_t>(qs), M, C, S(s));
+      launched("mx8_pack");
+    });
+  });
+  m.def("mx8_unpack", [](int dt, P q, P qs, P x, long long M, int C, P s) {
+    pgdist_rt::run_op([=] {
+      launch_mx8_unpack(dt, ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<void>(x), M, C, S(s));
+      launched("mx8_unpack");
+    });
+  });
+  m.def("mx8_wgrad_workspace_floats", &mx8_wgrad_workspace_floats);
+  m.def("mx8_wgrad", [](int dt, P dy, P q, P qs, P dw, P db, P ws, int M, int N, int K, P s) {
+    pgdist_rt::run_op([=] {
+      launch_mx8_wgrad(dt, ptr<void>(dy), ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<float>(dw), ptr<float>(db),
+                       ptr<float>(ws), M, N, K, S(s));
+      launched("mx8_wgrad");
     });
   });
   // ---- optimizer ----

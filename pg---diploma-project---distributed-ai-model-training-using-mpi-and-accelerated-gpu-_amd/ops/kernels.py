@@ -1034,6 +1034,203 @@ def conv_wgrad_s2d(G, Y, ga, gb, gc, x2, ws, grad, B, H2, N=64):
     lib().conv_wgrad_s2d(_p(G), _p(Y), _p(ga), _p(gb), _p(gc), _p(x2), _p(ws), _p(grad), B, H2, N, _s())
 
 
+# --------------------------------------------------------------------------- group norm, 8-bit checkpoints
+GN_NONE, GN_RELU, GN_RELU6, GN_SILU = 0, 1, 2, 3
+MX8_BLOCK = 32
+_DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_I31 = (1 << 31) - 1
+
+
+def _operand(t, nm, dtype, numel):
+    """Address of an operand of the group-norm / checkpoint kernels (64-bit offsets: any size)."""
+    if t is None:
+        return 0
+    if t.dtype != dtype:
+        raise TypeError(f"{nm}: expected {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{nm}: must be contiguous")
+    if t.numel() != numel:
+        raise ValueError(f"{nm}: has {t.numel()} elements, expected {numel}")
+    p = t.data_ptr()
+    if p & 15:
+        raise ValueError(f"{nm}: must be 16-byte aligned")
+    return p
+
+
+def _device_of(what, *ts):
+    """The current device's index; every operand has to be on it (the launch goes to its current stream)."""
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise ValueError(f"{what}: expected a device tensor, got one on {t.device}")
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: operand on {t.device}, the current device is cuda:{dev}")
+    return dev
+
+
+def _apart(what, outs, ins):
+    """No output may share memory with an operand or another output: (name, address, bytes) each."""
+    for i, (na, a, la) in enumerate(outs):
+        if a and la:
+            for nb_, b, lb in outs[i + 1:] + ins:
+                if b and a < b + lb and b < a + la:
+                    raise ValueError(f"{what}: {na} overlaps {nb_}")
+
+
+def _workspace(what, ws, need, dev):
+    """The caller's workspace, checked, or one from the allocator for this call alone."""
+    if ws is None:
+        if not need:
+            return None
+        if plan_recording():
+            raise ValueError(f"{what}: pass ws while a launch plan is recorded (its replays use the same memory)")
+        return torch.empty(need, dtype=F32, device=torch.device("cuda", dev))
+    if ws.dtype != F32 or not ws.is_contiguous() or ws.numel() < need or ws.data_ptr() & 15:
+        raise ValueError(f"{what}: ws must be {need} contiguous, 16-byte aligned floats")
+    _device_of(what, ws)
+    return ws
+
+
+def mx8_blocks(C):
+    """Scales of a checkpoint row of C channels."""
+    return -(-C // MX8_BLOCK)
+
+
+def _gn_check(what, t, B, S, C, G, act):
+    if t.dtype not in _DT:
+        raise TypeError(f"{what}: bf16, fp16 or fp32 activations, got {t.dtype}")
+    if B < 0 or S < 0 or C < 1 or G < 1 or C % G:
+        raise ValueError(f"{what}: B={B} S={S} C={C} G={G}: G must divide C, B and S be 0 at least")
+    if act not in (GN_NONE, GN_RELU, GN_RELU6, GN_SILU):
+        raise ValueError(f"{what}: unknown activation {act}")
+
+
+def gn_workspace(B, S, C, G, dtype, bwd=False):
+    """Floats of workspace that gn_fwd / gn_bwd of these sizes take as ``ws``."""
+    return int(lib().gn_workspace_floats(_DT[dtype], B, S, C, G, int(bwd)))
+
+
+def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=None, qs=None, ws=None):
+    """Group norm + activation of a channels-last [B, S, C] tensor (bf16, fp16 or fp32):
+    y = act((x - mean) * rstd * gamma + beta), mean / rstd over the S * C/G values of each (image,
+    group) and written as well (fp32 [B, G]; :func:`gn_bwd` reads them).  gamma / beta: fp32 [C] or
+    None.  With q, qs the 8-bit checkpoint of x (:func:`mx8_pack` of [B*S, C]) is also written.
+    ``ws``: :func:`gn_workspace` floats for this call alone; None takes them from the allocator.
+    No output may overlap another operand.  S = 0 gives mean 0, rstd 1/sqrt(eps)."""
+    _gn_check("gn_fwd", x, B, S, C, G, act)
+    if not eps > 0:
+        raise ValueError(f"gn_fwd: eps={eps} must be positive")
+    if (q is None) != (qs is None):
+        raise ValueError("gn_fwd: q and qs both or neither")
+    n, ns, e = B * S * C, B * S * mx8_blocks(C), x.element_size()
+    px, py = _operand(x, "x", x.dtype, n), _operand(y, "y", x.dtype, n)
+    pg, pb = _operand(gamma, "gamma", F32, C), _operand(beta, "beta", F32, C)
+    pm, pr = _operand(mean, "mean", F32, B * G), _operand(rstd, "rstd", F32, B * G)
+    pq, ps = _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
+    _apart("gn_fwd", [("y", py, n * e), ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G), ("q", pq, n), ("qs", ps, ns)],
+           [("x", px, n * e), ("gamma", pg, 4 * C), ("beta", pb, 4 * C)])
+    dev = _device_of("gn_fwd", x, y, gamma, beta, mean, rstd, q, qs)
+    if n == 0:
+        mean.zero_()
+        rstd.fill_(eps ** -0.5)
+        return
+    ws = _workspace("gn_fwd", ws, gn_workspace(B, S, C, G, x.dtype), dev)
+    lib().gn_fwd(_DT[x.dtype], px, pg, pb, py, pm, pr, pq, ps, 0 if ws is None else ws.data_ptr(), B, S, C, G,
+                 float(eps), act, _s())
+
+
+def gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=GN_NONE, q=None, qs=None, ws=None):
+    """Backward of :func:`gn_fwd` from dy and either x or (x None) its 8-bit checkpoint q, qs, whose
+    decoded values then stand for x; mean / rstd as gn_fwd wrote them.  dx [B, S, C] in dy's type,
+    dgb fp32 [2, C] = (dgamma, dbeta), overwritten, or None where neither is wanted.  Sums are in
+    fp32 in a fixed order.  On which side of relu's or relu6's borders a value lies is decided from
+    the operands in 64 bits where fp32 could tell it wrongly.  ``ws``: as gn_fwd (bwd=True)."""
+    _gn_check("gn_bwd", dy, B, S, C, G, act)
+    if (q is None) != (qs is None) or (x is None) == (q is None):
+        raise ValueError("gn_bwd: either x, or both q and qs")
+    n, ns, e = B * S * C, B * S * mx8_blocks(C), dy.element_size()
+    pd, px, po = _operand(dy, "dy", dy.dtype, n), _operand(x, "x", dy.dtype, n), _operand(dx, "dx", dy.dtype, n)
+    pg, pb = _operand(gamma, "gamma", F32, C), _operand(beta, "beta", F32, C)
+    pm, pr = _operand(mean, "mean", F32, B * G), _operand(rstd, "rstd", F32, B * G)
+    pq, ps = _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
+    pw = _operand(dgb, "dgb", F32, 2 * C)
+    _apart("gn_bwd", [("dx", po, n * e), ("dgb", pw, 8 * C)],
+           [("dy", pd, n * e), ("x", px, n * e), ("q", pq, n), ("qs", ps, ns), ("gamma", pg, 4 * C), ("beta", pb, 4 * C),
+            ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G)])
+    dev = _device_of("gn_bwd", dy, x, gamma, beta, mean, rstd, dx, dgb, q, qs)
+    if n == 0:
+        if dgb is not None:
+            dgb.zero_()
+        return
+    ws = _workspace("gn_bwd", ws, gn_workspace(B, S, C, G, dy.dtype, True), dev)
+    lib().gn_bwd(_DT[dy.dtype], pd, px, pq, ps, pg, pb, pm, pr, po, pw, 0 if ws is None else ws.data_ptr(), B, S, C, G,
+                 act, _s())
+
+
+def _mx8_check(what, t, M, C):
+    if t.dtype not in _DT:
+        raise TypeError(f"{what}: bf16, fp16 or fp32 values, got {t.dtype}")
+    if M < 0 or not 1 <= C <= _I31:
+        raise ValueError(f"{what}: M={M} C={C}: C must be positive, M 0 at least")
+
+
+def mx8_pack(x, q, qs, M, C):
+    """8-bit checkpoint of a [M, C] activation (bf16, fp16 or fp32): q uint8 [M, C] e4m3 codes, qs
+    uint8 [M, mx8_blocks(C)] the biased exponents (e + 127) of one power-of-two scale per 32
+    channels of a row; x ~ code * 2^e.  e is the least exponent at which the block's largest finite
+    magnitude is at most 448 * 2^e (within [-117, 120]), so nothing saturates; codes round to
+    nearest even; NaN and infinities become NaN."""
+    _mx8_check("mx8_pack", x, M, C)
+    n, ns = M * C, M * mx8_blocks(C)
+    px, pq, ps = _operand(x, "x", x.dtype, n), _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
+    _apart("mx8_pack", [("q", pq, n), ("qs", ps, ns)], [("x", px, n * x.element_size())])
+    _device_of("mx8_pack", x, q, qs)
+    if n:
+        lib().mx8_pack(_DT[x.dtype], px, pq, ps, M, C, _s())
+
+
+def mx8_unpack(q, qs, x, M, C):
+    """x [M, C] (bf16, fp16 or fp32) = the values a checkpoint stands for: exact in bf16 and fp32;
+    in fp16 rounded to nearest even and held within +-65504."""
+    _mx8_check("mx8_unpack", x, M, C)
+    n, ns = M * C, M * mx8_blocks(C)
+    px, pq, ps = _operand(x, "x", x.dtype, n), _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
+    _apart("mx8_unpack", [("x", px, n * x.element_size())], [("q", pq, n), ("qs", ps, ns)])
+    _device_of("mx8_unpack", x, q, qs)
+    if n:
+        lib().mx8_unpack(_DT[x.dtype], pq, ps, px, M, C, _s())
+
+
+def mx8_wgrad_workspace(M, N, K):
+    """Floats of workspace that mx8_wgrad of these sizes takes as ``ws``."""
+    return int(lib().mx8_wgrad_workspace_floats(M, N, K))
+
+
+def mx8_wgrad(dy, q, qs, grad, M, N, K, db=None, ws=None):
+    """Weight gradient of y = x W^T (+ b), a linear layer or 1x1 convolution, whose input was kept as
+    the checkpoint q, qs of [M, K]: grad [N, K] (fp32, overwritten) = dy^T x~, and db [N] (fp32) =
+    the column sums of dy.  dy [M, N] bf16 or fp16; x~ is decoded inside the product (exact in
+    bf16; in fp16 as :func:`mx8_unpack`).  fp32 accumulation in a fixed order.  ``ws``:
+    :func:`mx8_wgrad_workspace` floats for this call alone; None takes them from the allocator."""
+    if dy.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"mx8_wgrad: dy bf16 or fp16, got {dy.dtype}")
+    if not 0 <= M <= _I31 or not 1 <= N <= _I31 or not 1 <= K <= _I31:
+        raise ValueError(f"mx8_wgrad: M={M} N={N} K={K}: N and K must be positive, M 0 at least, each below 2^31")
+    nq, ns = M * K, M * mx8_blocks(K)
+    pd, pq, ps = _operand(dy, "dy", dy.dtype, M * N), _operand(q, "q", torch.uint8, nq), _operand(qs, "qs", torch.uint8, ns)
+    pw, pb = _operand(grad, "grad", F32, N * K), _operand(db, "db", F32, N)
+    _apart("mx8_wgrad", [("grad", pw, 4 * N * K), ("db", pb, 4 * N)], [("dy", pd, 2 * M * N), ("q", pq, nq), ("qs", ps, ns)])
+    dev = _device_of("mx8_wgrad", dy, q, qs, grad, db)
+    if M == 0:
+        grad.zero_()
+        if db is not None:
+            db.zero_()
+        return
+    ws = _workspace("mx8_wgrad", ws, mx8_wgrad_workspace(M, N, K), dev)
+    lib().mx8_wgrad(_DT[dy.dtype], pd, pq, ps, pw, pb, 0 if ws is None else ws.data_ptr(), M, N, K, _s())
+
+
 # --------------------------------------------------------------------------- launch plans
 def stream_wait(waiter, signaler):
     """``waiter`` waits for the work enqueued so far on ``signaler`` (torch streams); unlike
@@ -1149,5 +1346,6 @@ for _name in ("bn_fwd_finalize", "bn_bwd_finalize", "bn_apply", "bn_finalize_bat
               "step_begin", "reduce_metrics", "dw_fwd", "dw_dgrad", "dw_wgrad", "pw_gemm", "pw_gemm_f8", "w8_quant",
               "wt_transpose", "pw_bwd", "wgrad_reduce", "wgrad_reduce_flush", "pw_wgrad", "stem_fwd", "stem_wgrad",
               "head", "augment", "conv_fwd", "conv_dgrad", "conv_wgrad", "bn_mat", "conv_wt", "res_out", "maxpool_fwd",
-              "maxpool_bwd", "avgpool", "head_bwd", "softmax_ce", "fc_gemm", "col_sum", "image_prep", "memset"):
+              "maxpool_bwd", "avgpool", "head_bwd", "softmax_ce", "fc_gemm", "col_sum", "image_prep", "memset", "gn_fwd",
+              "gn_bwd", "mx8_pack", "mx8_unpack", "mx8_wgrad"):
     globals()[_name] = _logged(globals()[_name])

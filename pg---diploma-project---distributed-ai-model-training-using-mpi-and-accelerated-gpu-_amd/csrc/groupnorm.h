@@ -1,0 +1,685 @@
+// Group norm with an activation over channels-last [B][S][C] tensors, forward and backward, with
+// the 8-bit checkpoint of the input (mx8.h) written by the forward and read by the backward.
+//
+//   y = act(z), z = (x - mean) rstd gamma + beta, statistics over the S * C/G values of (b, g)
+//   dz = dy act'(z), xh = (x - mean) rstd:  dgamma = sum dz xh, dbeta = sum dz,
+//   dx = rstd (dz gamma - (s1 + xh s2) / m), s1 = sum_g dz gamma, s2 = sum_g dz gamma xh
+//
+// Both are bound by memory: what matters is to read every value once.  A workgroup therefore keeps
+// its rows x channels tile in registers between the statistics and the use of them:
+//   solo     the tile is all S rows of a slab of whole groups: one launch, nothing exchanged
+//   cluster  the S rows are split over k workgroups; each publishes its tile's sums, waits for the
+//            other k - 1 and goes on with the tile it still holds.  Also one read.
+//   split    k is larger than what is sure to be resident together: sums and use are two launches
+//            and the tile is read twice.
+//   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
+//            one workgroup per (image, group), then one value a thread.
+// A thread owns one vector of V channels (16 bytes where C allows) and every R-th row of the tile.
+// Sums are taken in a fixed order in all three, so results do not vary from run to run.
+#pragma once
+#include "mx8.h"
+#include "reduce.h"
+
+#include <type_traits>
+
+namespace gn {
+enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_RELU6 = 2, GN_SILU = 3 };
+enum GnMode : int { SOLO = 0, CLUSTER = 1, SUMS = 2, APPLY = 3, WIDE = 4 };
+
+// ---- vectors of V channels -------------------------------------------------------------------
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { typedef uint4 type; };
+template <> struct RawOf<8> { typedef uint2 type; };
+template <> struct RawOf<4> { typedef uint32_t type; };
+template <> struct RawOf<2> { typedef uint16_t type; };
+template <> struct RawOf<1> { typedef uint8_t type; };
+
+template <class T, int V> struct Vec {
+  typedef typename RawOf<V * (int)sizeof(T)>::type raw;
+  struct alignas(sizeof(raw)) arr { T v[V]; };
+  static PG_DEVICE void unpack(const raw &r, float (&f)[V]) {
+    const arr a = __builtin_bit_cast(arr, r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = tof(a.v[j]);
+  }
+  static PG_DEVICE raw pack(const float (&f)[V]) {
+    if constexpr (sizeof(T) == 2 && V >= 2 && __is_same(T, bf16_t)) {
+      struct alignas(sizeof(raw)) { uint32_t w[V / 2]; } a;
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) a.w[j] = pack2(f[2 * j], f[2 * j + 1]);
+      return __builtin_bit_cast(raw, a);
+    } else {
+      arr a;
+#pragma unroll
+      for (int j = 0; j < V; ++j) a.v[j] = fromf<T>(f[j]);
+      return __builtin_bit_cast(raw, a);
+    }
+  }
+};
+
+// V codes
+template <int V> struct Codes {
+  typedef typename RawOf<V>::type raw;
+  static PG_DEVICE raw encode(const float (&f)[V], float inv) {
+    if constexpr (V == 8)
+      return make_uint2(mx8_enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                        mx8_enc4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+    else if constexpr (V == 4) return mx8_enc4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
+    else if constexpr (V == 2) return (uint16_t)mx8_enc2<false>(f[0] * inv, f[1] * inv, 0);
+    else return mx8_enc1(f[0] * inv);
+  }
+  static PG_DEVICE void decode(const raw &r, float sc, float (&f)[V]) {
+    if constexpr (V == 8) {
+      mx8_dec4(r.x, sc, f[0], f[1], f[2], f[3]);
+      mx8_dec4(r.y, sc, f[4], f[5], f[6], f[7]);
+    } else if constexpr (V == 4) mx8_dec4(r, sc, f[0], f[1], f[2], f[3]);
+    else if constexpr (V == 2) mx8_dec2<false>(r, sc, f[0], f[1]);
+    else f[0] = mx8_dec1(r) * sc;
+  }
+};
+
+// ---- tile geometry ---------------------------------------------------------------------------
+struct Geo {
+  long long B, S;
+  int C, G, cg;
+  int cs;       // channels of a slab (whole groups; the last slab may be narrower)
+  int nslab;
+  int CVp;      // vector columns of a tile row (padded to whole 32-channel blocks for checkpoints)
+  int R;        // tile rows per sweep: blockDim / CVp
+  int k;        // tiles per (image, slab)
+  int gs;       // groups of a full slab
+  int wait;     // polls before a workgroup computes the others' sums itself
+};
+
+// this workgroup's place
+struct Place {
+  long long b, bs;   // image; image * nslab + slab
+  int chunk, c0, csl, ng, g0;
+  int col, row, c;
+  bool on;           // this thread has a column
+};
+template <int V> PG_DEVICE Place place(const Geo &g) {
+  Place p;
+  const int id = blockIdx.x;
+  p.chunk = id % g.k;
+  p.bs = id / g.k;
+  const int slab = (int)(p.bs % g.nslab);
+  p.b = p.bs / g.nslab;
+  p.c0 = slab * g.cs;
+  p.csl = min(g.cs, g.C - p.c0);
+  p.ng = p.csl / g.cg;
+  p.g0 = p.c0 / g.cg;
+  p.col = threadIdx.x % g.CVp;
+  p.row = threadIdx.x / g.CVp;
+  p.on = p.col < p.csl / V && p.row < g.R;
+  p.c = p.on ? p.c0 + p.col * V : p.c0;
+  return p;
+}
+
+// element at a byte offset from a base that is the same for the whole workgroup (a tile spans less
+// than 2^31 bytes): one scalar base and one 32-bit offset register a load
+template <class R> PG_DEVICE const R &at(const void *base, uint32_t off) {
+  return *reinterpret_cast<const R *>(static_cast<const char *>(base) + off);
+}
+template <class R> PG_DEVICE R &at(void *base, uint32_t off) {
+  return *reinterpret_cast<R *>(static_cast<char *>(base) + off);
+}
+
+PG_DEVICE float seg_sum(float v, int W) {   // sum over aligned segments of W lanes
+  for (int o = W >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+PG_DEVICE int seg_width(int n) {   // lanes that share n terms: a power of two up to 64
+  int W = 64;
+  while (W > 1 && (W >> 1) >= n) W >>= 1;
+  return W;
+}
+
+// out[g] = sum over the tile of the values of group g; acc: this thread's column sums.
+// FOLD: C/G is a multiple of V, so the thread's channels are one group's.
+template <int V, bool FOLD>
+PG_DEVICE void group_sums(const Geo &g, const Place &p, const float (&acc)[V], float *red, float *out) {
+  const int t = threadIdx.x;
+  if (p.on) {
+    if constexpr (FOLD) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += acc[j];
+      red[p.row * g.CVp + p.col] = s;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) red[(p.row * g.CVp + p.col) * V + j] = acc[j];
+    }
+  }
+  __syncthreads();
+  const int width = FOLD ? g.cg / V : g.cg, pitch = FOLD ? g.CVp : g.CVp * V;
+  const int E = g.R * width, W = seg_width(E), per = 64 / W;
+  const int lane = t & 63, l = lane & (W - 1);
+  for (int gi = (t >> 6) * per + lane / W; gi - lane / W < p.ng; gi += (blockDim.x >> 6) * per) {
+    float s = 0.f;
+    if (gi < p.ng)
+      for (int e = l; e < E; e += W) s += red[e / width * pitch + gi * width + e % width];
+    s = seg_sum(s, W);
+    if (l == 0 && gi < p.ng) out[gi] = s;
+  }
+  __syncthreads();
+}
+
+// One arrival of this workgroup, then the wait for all k.  Published values were stored with st_sc1.
+// True: all have arrived.  False (uniformly): not within `polls`, the caller does the work itself.
+PG_DEVICE bool arrive_and_wait(int *ctr, int k, int polls, int *flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+    for (int i = 0; n < k && i < polls; ++i) {
+      __builtin_amdgcn_s_sleep(1);
+      n = __hip_atomic_load(ctr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    *flag = n >= k;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// ---- forward ---------------------------------------------------------------------------------
+struct FwdArgs {
+  Geo g;
+  const void *x;
+  const float *gamma, *beta;
+  void *y;
+  float *mean, *rstd;
+  uint8_t *q, *qs;
+  int *ctr;      // [B * nslab] arrivals (cluster)
+  float *part;   // [B * nslab][k][gs][2]: mean and sum of squares about it of every tile and group
+  float eps;
+  int act;
+};
+
+// NaN passes through every activation
+template <int ACT> PG_DEVICE float gn_act(float z) {
+  if constexpr (ACT == GN_RELU) return z < 0.f ? 0.f : z;
+  else if constexpr (ACT == GN_RELU6) return z < 0.f ? 0.f : z > 6.f ? 6.f : z;
+  else if constexpr (ACT == GN_SILU) return z / (1.f + __expf(-z));
+  else return z;
+}
+
+template <class T, int V, int NV, int MODE, bool CK, bool FOLD>
+__global__ __launch_bounds__(1024) void gn_fwd_kernel(const FwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  const Geo &g = a.g;
+  const Place p = place<V>(g);
+  float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
+  __shared__ int flag;
+  const int tile = g.R * NV;
+  constexpr int VG = FOLD ? 1 : V;
+  int gi[VG];   // slab group of each channel (FOLD: of all)
+#pragma unroll
+  for (int j = 0; j < VG; ++j) gi[j] = (p.c - p.c0 + j) / g.cg;
+
+  typename X::raw d[NV];
+  int nr = 0;
+  // rows past the end (and threads without a column) read a row that exists and are masked
+  auto load = [&](int chunk) {
+    const long long s0 = (long long)chunk * tile;
+    nr = (int)min((long long)tile, g.S - s0);
+    const T *src = static_cast<const T *>(a.x) + (p.b * g.S + s0) * g.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t r = min(p.row + i * g.R, nr - 1);
+      d[i] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
+    }
+  };
+  // mean and sum of squares about it of the tile's groups -> gm, gr
+  auto sums = [&]() {
+    float acc[V], mu[VG];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (p.row + i * g.R < nr) {
+        float f[V];
+        X::unpack(d[i], f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += f[j];
+      }
+    group_sums<V, FOLD>(g, p, acc, red, gm);
+    const float rn = 1.f / ((float)nr * (float)g.cg);
+#pragma unroll
+    for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]] * rn;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (p.row + i * g.R < nr) {
+        float f[V];
+        X::unpack(d[i], f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float df = f[j] - mu[FOLD ? 0 : j];
+          acc[j] = fmaf(df, df, acc[j]);
+        }
+      }
+    __syncthreads();   // gm and red have been read
+    if (threadIdx.x < p.ng) gm[threadIdx.x] *= rn;
+    for (int i = threadIdx.x + blockDim.x; i < p.ng; i += blockDim.x) gm[i] *= rn;
+    group_sums<V, FOLD>(g, p, acc, red, gr);
+  };
+  auto publish = [&](int chunk) {
+    float *dst = a.part + ((p.bs * g.k + chunk) * g.gs) * 2;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
+      st_sc1(dst + 2 * i, gm[i]);
+      st_sc1(dst + 2 * i + 1, gr[i]);
+    }
+  };
+
+  if constexpr (MODE == CLUSTER) {
+    // The first round is this workgroup's own tile.  Where a peer does not come in time the others
+    // follow, computed here to the same bits as theirs, its own again at the end.
+    for (int i = 0, ch = p.chunk;;) {
+      load(ch);
+      __syncthreads();
+      sums();
+      publish(ch);
+      if (i == 0 ? arrive_and_wait(a.ctr + p.bs, g.k, g.wait, &flag) : i == g.k) break;
+      ++i;
+      ch = p.chunk + i < g.k ? p.chunk + i : p.chunk + i - g.k;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  } else {
+    load(p.chunk);
+    if constexpr (MODE != APPLY) sums();
+    if constexpr (MODE == SUMS) {
+      publish(p.chunk);
+      return;
+    }
+  }
+  const float n = (float)g.S * (float)g.cg;
+  if constexpr (MODE == SOLO) {
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
+  } else {   // join the tiles: W lanes a group
+    const float *src = a.part + p.bs * g.k * g.gs * 2;
+    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+    auto count = [&](int ch) { return (float)min((long long)tile, g.S - (long long)ch * tile) * (float)g.cg; };
+    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+      float m = 0.f, v = 0.f;
+      if (i < p.ng)
+        for (int ch = l; ch < g.k; ch += W) m += count(ch) * ld_sc1(src + (ch * g.gs + i) * 2);
+      m = seg_sum(m, W) / n;
+      if (i < p.ng)
+        for (int ch = l; ch < g.k; ch += W) {
+          const float dm = ld_sc1(src + (ch * g.gs + i) * 2) - m;
+          v += ld_sc1(src + (ch * g.gs + i) * 2 + 1) + count(ch) * dm * dm;
+        }
+      v = seg_sum(v, W);
+      if (l == 0 && i < p.ng) {
+        gm[i] = m;
+        gr[i] = 1.f / sqrtf(v / n + a.eps);
+      }
+    }
+  }
+  __syncthreads();
+  if (p.chunk == 0)
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
+      a.mean[p.b * g.G + p.g0 + i] = gm[i];
+      a.rstd[p.b * g.G + p.g0 + i] = gr[i];
+    }
+  if constexpr (CK) {
+    // the checkpoint: 32 channels are 32 / V neighbouring lanes (CVp is a multiple of that).
+    const long long r0 = p.b * g.S + (long long)p.chunk * tile;
+    const int nb = (g.C + kMxBlock - 1) / kMxBlock;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float f[V], m = 0.f;
+      X::unpack(d[i], f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(f[j]));
+      m = p.on ? m : 0.f;
+#pragma unroll
+      for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+      const int r = p.row + i * g.R, e = mx8_exp(m);
+      if (p.on && r < nr) {
+        at<typename Codes<V>::raw>(a.q + r0 * g.C, (uint32_t)r * g.C + p.c) = Codes<V>::encode(f, mx8_inv_scale(e));
+        if (p.c % kMxBlock == 0) at<uint8_t>(a.qs + r0 * nb, (uint32_t)r * nb + p.c / kMxBlock) = (uint8_t)e;
+      }
+    }
+  }
+  if (!p.on) return;
+  float mu[VG], sc[V], be[V];
+#pragma unroll
+  for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    sc[j] = gr[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
+    be[j] = a.beta ? a.beta[p.c + j] : 0.f;
+  }
+  T *dst = static_cast<T *>(a.y) + (p.b * g.S + (long long)p.chunk * tile) * g.C;
+  auto apply = [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int r = p.row + i * g.R;
+      if (r < nr) {
+        float f[V];
+        X::unpack(d[i], f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = gn_act<decltype(act)::value>(fmaf(f[j] - mu[FOLD ? 0 : j], sc[j], be[j]));
+        at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = X::pack(f);
+      }
+    }
+  };
+  if (a.act == GN_RELU6) apply(std::integral_constant<int, GN_RELU6>());
+  else if (a.act == GN_RELU) apply(std::integral_constant<int, GN_RELU>());
+  else if (a.act == GN_SILU) apply(std::integral_constant<int, GN_SILU>());
+  else apply(std::integral_constant<int, GN_NONE>());
+}
+
+// ---- backward --------------------------------------------------------------------------------
+struct BwdArgs {
+  Geo g;
+  const void *dy, *x;
+  const uint8_t *q, *qs;
+  const float *gamma, *beta, *mean, *rstd;
+  void *dx;
+  int *ctr;       // [B * nslab]
+  float *part;    // [B * nslab][k][gs][2]: s1, s2 of every tile and group
+  float *dpart;   // [B * k][2][C]: dgamma, dbeta of every tile, or null
+  int silu;
+  float lo, hi;   // the other activations' borders
+};
+
+// act'(z) dy of V channels (df = x - mean).  SILU, or dy where lo < z < hi and 0 elsewhere: none is
+// (-inf, inf), relu (0, inf), relu6 (0, 6).  Which side of a border z lies on is decided from the
+// operands as they are: within fp32's rounding of a border (z takes four roundings of terms no
+// larger than |z| + |beta|) z is formed again in 64 bits, once in some 10^5 vectors.
+template <bool SILU, int V, int VG>
+PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al)[V], const float (&be)[V],
+                     float (&dy)[V], const BwdArgs &a, const float *mean, const float *rstd, const int (&gi)[VG],
+                     int c) {
+  if constexpr (SILU) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = fmaf(df[j], al[j], be[j]);
+      const float s = 1.f / (1.f + __expf(-z));
+      dy[j] *= s * fmaf(z, 1.f - s, 1.f);
+    }
+  } else {
+    bool near = false, out[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = fmaf(df[j], al[j], be[j]);
+      out[j] = z <= a.lo || z >= a.hi;
+      const float tol = 1e-6f * fabsf(be[j]);
+      near |= fabsf(z - a.lo) <= tol || fabsf(z - a.hi) <= tol + 8e-6f;
+    }
+    if (near) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        // One value at a time, its operands read again and made opaque: together, or hoisted out
+        // of the row loop, their 64-bit copies would cost the whole kernel its registers.
+        int k = gi[VG == 1 ? 0 : j], cj = c + j;
+        float b = be[j], v = x[j];
+        asm volatile("" : "+v"(k), "+v"(cj), "+v"(b), "+v"(v));
+        const float tol = 1e-6f * fabsf(b), z = fmaf(df[j], al[j], b);
+        if (fabsf(z - a.lo) <= tol || fabsf(z - a.hi) <= tol + 8e-6f) {
+          const double w = ((double)v - (double)mean[k]) * (double)rstd[k] * (a.gamma ? (double)a.gamma[cj] : 1.0) +
+                           (double)b;
+          out[j] = w <= (double)a.lo || w >= (double)a.hi;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) dy[j] = out[j] ? 0.f : dy[j];
+  }
+}
+
+template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU>
+__global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  const Geo &g = a.g;
+  const Place p = place<V>(g);
+  // sums of the slab's groups, its channels' sums, the reduction's rows
+  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
+  __shared__ int flag;
+  const int tile = g.R * NV, nb = (g.C + kMxBlock - 1) / kMxBlock;
+  const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
+  constexpr int VG = FOLD ? 1 : V;
+  int gi[VG];
+  float mu[VG], al[V], be[V];
+#pragma unroll
+  for (int j = 0; j < VG; ++j) {
+    gi[j] = (p.c - p.c0 + j) / g.cg;
+    mu[j] = mean[gi[j]];
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    al[j] = rstd[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
+    be[j] = a.beta ? a.beta[p.c + j] : 0.f;
+  }
+  typename X::raw dy[NV];
+  typename X::raw xr[CK ? 1 : NV];
+  typename Codes<V>::raw qr[CK ? NV : 1];
+  float sc[CK ? NV : 1];
+  int nr = 0;
+  auto load = [&](int chunk) {
+    const long long s0 = (long long)chunk * tile, r0 = p.b * g.S + s0;
+    nr = (int)min((long long)tile, g.S - s0);
+    const T *src = static_cast<const T *>(a.dy) + r0 * g.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint32_t r = min(p.row + i * g.R, nr - 1), o = r * g.C + p.c;
+      dy[i] = at<typename X::raw>(src, o * (uint32_t)sizeof(T));
+      if constexpr (CK) {
+        qr[i] = at<typename Codes<V>::raw>(a.q + r0 * g.C, o);
+        sc[i] = mx8_scale(at<uint8_t>(a.qs + r0 * nb, r * nb + p.c / kMxBlock));
+      } else {
+        xr[i] = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * g.C, o * (uint32_t)sizeof(T));
+      }
+    }
+  };
+  auto input = [&](int i, float (&f)[V]) {
+    if constexpr (CK) Codes<V>::decode(qr[i], sc[i], f);
+    else X::unpack(xr[i], f);
+  };
+  // tot[c] = dgamma, tot[cs + c] = dbeta of the tile; g1, g2 = s1, s2 of its groups
+  auto sums = [&]() {
+    float s0[V], s1[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (p.row + i * g.R < nr) {
+        float f[V], df[V], dz[V];
+        input(i, f);
+        X::unpack(dy[i], dz);
+#pragma unroll
+        for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
+        gn_dz<SILU, V, VG>(df, f, al, be, dz, a, mean, rstd, gi, p.c);
+        // dz is dy or 0 (all but silu): it takes dy's place for the second use
+        if constexpr (!SILU) dy[i] = X::pack(dz);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          s1[j] = fmaf(dz[j], df[j], s1[j]);
+          s0[j] += dz[j];
+        }
+      }
+    const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (p.on) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
+      }
+      __syncthreads();
+      if (nt <= 1) {
+        for (int o = t; o < n; o += blockDim.x) {
+          float s = 0.f;
+          for (int r = 0; r < g.R; ++r) s += red[r * ld + o];
+          tot[h * g.cs + o] = h ? s : s * rstd[o / g.cg];
+        }
+      } else {   // nt stripes of rows a channel
+        const int o = t % n, st = t / n;
+        if (st < nt) {
+          float s = 0.f;
+          for (int r = st; r < g.R; r += nt) s += red[r * ld + o];
+          red2[st * n + o] = s;
+        }
+        __syncthreads();
+        if (t < n) {
+          float s = 0.f;
+          for (int i = 0; i < nt; ++i) s += red2[i * n + t];
+          tot[h * g.cs + t] = h ? s : s * rstd[t / g.cg];
+        }
+      }
+      __syncthreads();
+    }
+    const int W = seg_width(g.cg), per = 64 / W, lane = t & 63, l = lane & (W - 1);
+    for (int i = (t >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+      float u = 0.f, v = 0.f;
+      if (i < p.ng)
+        for (int c = i * g.cg + l; c < (i + 1) * g.cg; c += W) {
+          const float ga = a.gamma ? a.gamma[p.c0 + c] : 1.f;
+          u = fmaf(ga, tot[g.cs + c], u);
+          v = fmaf(ga, tot[c], v);
+        }
+      u = seg_sum(u, W);
+      v = seg_sum(v, W);
+      if (l == 0 && i < p.ng) {
+        g1[i] = u;
+        g2[i] = v;
+      }
+    }
+    __syncthreads();
+  };
+  auto publish = [&](int chunk) {
+    float *dst = a.part + ((p.bs * g.k + chunk) * g.gs) * 2;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
+      st_sc1(dst + 2 * i, g1[i]);
+      st_sc1(dst + 2 * i + 1, g2[i]);
+    }
+  };
+  for (int i = 0, ch = p.chunk;;) {   // more than one round only as in the forward
+    load(ch);
+    if constexpr (MODE == APPLY) break;
+    if constexpr (MODE == CLUSTER) __syncthreads();
+    sums();
+    if (i == 0 && a.dpart) {
+      float *dst = a.dpart + (p.b * g.k + ch) * 2 * g.C + p.c0;
+      for (int j = threadIdx.x; j < p.csl; j += blockDim.x) {
+        dst[j] = tot[j];
+        dst[g.C + j] = tot[g.cs + j];
+      }
+    }
+    if constexpr (MODE == SOLO) break;
+    publish(ch);
+    if constexpr (MODE == SUMS) return;
+    if (i == 0 ? arrive_and_wait(a.ctr + p.bs, g.k, g.wait, &flag) : i == g.k) break;
+    ++i;
+    ch = p.chunk + i < g.k ? p.chunk + i : p.chunk + i - g.k;
+  }
+  if constexpr (MODE == CLUSTER) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+  if constexpr (MODE != SOLO) {
+    const float *src = a.part + p.bs * g.k * g.gs * 2;
+    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+      float u = 0.f, v = 0.f;
+      if (i < p.ng)
+        for (int ch = l; ch < g.k; ch += W) {
+          u += ld_sc1(src + (ch * g.gs + i) * 2);
+          v += ld_sc1(src + (ch * g.gs + i) * 2 + 1);
+        }
+      u = seg_sum(u, W);
+      v = seg_sum(v, W);
+      if (l == 0 && i < p.ng) {
+        g1[i] = u;
+        g2[i] = v;
+      }
+    }
+    __syncthreads();
+  }
+  if (!p.on) return;
+  // dx = dz al - (k1 + (x - mean) k2)
+  const float rm = 1.f / ((float)g.S * (float)g.cg);
+  float k1[VG], k2[VG];
+#pragma unroll
+  for (int j = 0; j < VG; ++j) {
+    const float rs = rstd[gi[j]];
+    k1[j] = rs * g1[gi[j]] * rm;
+    k2[j] = rs * rs * g2[gi[j]] * rm;
+  }
+  T *dst = static_cast<T *>(a.dx) + (p.b * g.S + (long long)p.chunk * tile) * g.C;
+  constexpr bool masked = !SILU && MODE != APPLY;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int r = p.row + i * g.R;
+    if (r < nr) {
+      float f[V], df[V], dz[V];
+      input(i, f);
+      X::unpack(dy[i], dz);
+#pragma unroll
+      for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
+      if constexpr (!masked) gn_dz<SILU, V, VG>(df, f, al, be, dz, a, mean, rstd, gi, p.c);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = fmaf(dz[j], al[j], -fmaf(df[j], k2[FOLD ? 0 : j], k1[FOLD ? 0 : j]));
+      *reinterpret_cast<typename X::raw *>(dst + (size_t)(uint32_t)r * (uint32_t)g.C + p.c) = X::pack(f);
+    }
+  }
+}
+
+// ---- launch ------------------------------------------------------------------------------------
+struct Plan {
+  Geo g;
+  int V, NV, TH, mode;   // mode SUMS: SUMS, then APPLY
+  long long wgs;
+};
+
+struct Fwd {
+  typedef FwdArgs Args;
+  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto kernel() {
+    return gn_fwd_kernel<T, V, NV, MODE, CK, FOLD>;
+  }
+};
+struct Bwd {
+  typedef BwdArgs Args;
+  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto kernel() {
+    return gn_bwd_kernel<T, V, NV, MODE, CK, FOLD, SILU>;
+  }
+};
+
+template <class D, class T, int V, int NV, bool CK, bool FOLD, bool SILU>
+void launch_mode(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(p.TH), lds, st, a); };
+  if (p.mode == SOLO) go(D::template kernel<T, V, NV, SOLO, CK, FOLD, SILU>());
+  else if (p.mode == CLUSTER) go(D::template kernel<T, V, NV, CLUSTER, CK, FOLD, SILU>());
+  else {
+    go(D::template kernel<T, V, NV, SUMS, CK, FOLD, SILU>());
+    go(D::template kernel<T, V, NV, APPLY, CK, FOLD, SILU>());
+  }
+}
+// the plan gives NV 2, 4 (forward: 8) to full vectors of one group each, 2 to full vectors that
+// straddle groups (their constants take the registers), 4 to narrower ones
+template <class D, class T, int VMAX, int MOST, bool CK, bool SILU>
+void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
+  if (p.V == VMAX && p.g.cg % VMAX == 0) {
+    if (p.NV == 2) launch_mode<D, T, VMAX, 2, CK, true, SILU>(p, lds, a, st);
+    else if (MOST == 4 || p.NV == 4) launch_mode<D, T, VMAX, 4, CK, true, SILU>(p, lds, a, st);
+    else launch_mode<D, T, VMAX, MOST, CK, true, SILU>(p, lds, a, st);
+  } else if (p.V == VMAX) launch_mode<D, T, VMAX, 2, CK, false, SILU>(p, lds, a, st);
+  else if (VMAX == 8 && p.V == 4) launch_mode<D, T, 4, 4, CK, false, SILU>(p, lds, a, st);
+  else if (p.V == 2) launch_mode<D, T, 2, 4, CK, false, SILU>(p, lds, a, st);
+  else launch_mode<D, T, 1, 4, CK, false, SILU>(p, lds, a, st);
+}
+
+// one translation unit per direction and type
+void fwd_bf16(const Plan &p, size_t lds, const FwdArgs &a, hipStream_t st);
+void fwd_fp16(const Plan &p, size_t lds, const FwdArgs &a, hipStream_t st);
+void fwd_fp32(const Plan &p, size_t lds, const FwdArgs &a, hipStream_t st);
+void bwd_bf16(const Plan &p, size_t lds, const BwdArgs &a, hipStream_t st);
+void bwd_fp16(const Plan &p, size_t lds, const BwdArgs &a, hipStream_t st);
+void bwd_fp32(const Plan &p, size_t lds, const BwdArgs &a, hipStream_t st);
+}  // namespace gn

@@ -1,0 +1,12 @@
+// group norm backward, fp16 (groupnorm.h)
+#include "../groupnorm.h"
+
+void gn::bwd_fp16(const Plan &p, size_t lds, const BwdArgs &a, hipStream_t st) {
+  if (a.silu) {
+    if (a.q) launch<Bwd, _Float16, 8, 4, true, true>(p, lds, a, st);
+    else launch<Bwd, _Float16, 8, 4, false, true>(p, lds, a, st);
+  } else {
+    if (a.q) launch<Bwd, _Float16, 8, 4, true, false>(p, lds, a, st);
+    else launch<Bwd, _Float16, 8, 4, false, false>(p, lds, a, st);
+  }
+}

@@ -1,0 +1,7 @@
+// group norm forward, fp32 (groupnorm.h)
+#include "../groupnorm.h"
+
+void gn::fwd_fp32(const Plan &p, size_t lds, const FwdArgs &a, hipStream_t st) {
+  if (a.q) launch<Fwd, float, 4, 8, true, false>(p, lds, a, st);
+  else launch<Fwd, float, 4, 8, false, false>(p, lds, a, st);
+}

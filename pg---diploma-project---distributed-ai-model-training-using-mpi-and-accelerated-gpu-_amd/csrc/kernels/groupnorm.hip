@@ -1,192 +1,341 @@
-// Group norm with an activation over channels-last [B][S][C] tensors, forward and backward, with
-// the 8-bit checkpoint of the input (mx8.h) written by the forward and read by the backward.
-//
-//   y = act(z), z = (x - mean) * rstd * gamma + beta, statistics over the S * C/G values of (b, g)
-//   dz = dy act'(z), xh = (x - mean) rstd:  dgamma = sum dz xh, dbeta = sum dz,
-//   dx = rstd (dz gamma - (s1 + xh s2) / m), s1 = sum_g dz gamma, s2 = sum_g dz gamma xh
-#include "../mx8.h"
+// Group norm: geometry, workspace and launches (groupnorm.h holds the kernels), and the sums over
+// images and tiles that give dgamma and dbeta.
+#include "../groupnorm.h"
+
+#include <algorithm>
+#include <cmath>
+#include <numeric>
+#include <stdexcept>
+
+using namespace gn;
 
 namespace {
-enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_RELU6 = 2, GN_SILU = 3 };
-
-// NaN passes through every activation
-PG_DEVICE float gn_act(float z, int act) {
-  if (act == GN_RELU) return z < 0.f ? 0.f : z;
-  if (act == GN_RELU6) return z < 0.f ? 0.f : z > 6.f ? 6.f : z;
-  if (act == GN_SILU) return z / (1.f + __expf(-z));
-  return z;
+// ---- wide groups: not tuned, every access one value -----------------------------------------------
+// A plain loop over memory: C / G of thousands of channels, or over a thousand of an odd number.
+PG_DEVICE float load_one(const void *x, int dt, long long i) {
+  return dt == 0 ? bf2f(static_cast<const bf16_t *>(x)[i])
+                 : dt == 1 ? (float)static_cast<const _Float16 *>(x)[i] : static_cast<const float *>(x)[i];
 }
-
-// act'(z) dy.  Which side of a border z lies on is decided from the operands as they are: within the
-// fp32 rounding of the border (|z - border| below a bound on it) z is formed again in 64 bits.
-PG_DEVICE float gn_dz(float dy, float x, float mean, float rstd, float g, float b, int act) {
-  const float z = (x - mean) * rstd * g + b;
-  if (act == GN_NONE) return dy;
-  if (act == GN_SILU) {
-    const float s = 1.f / (1.f + __expf(-z));
-    return dy * (s * (1.f + z * (1.f - s)));
-  }
-  const float tol = 1e-6f * (fabsf(z) + 2.f * fabsf(b));
-  bool in = z > 0.f && !(act == GN_RELU6 && z >= 6.f);
-  if (fabsf(z) <= tol || (act == GN_RELU6 && fabsf(z - 6.f) <= tol)) {
-    const double w = ((double)x - (double)mean) * (double)rstd * (double)g + (double)b;
-    in = w > 0.0 && !(act == GN_RELU6 && w >= 6.0);
-  }
-  return in ? dy : 0.f;
+PG_DEVICE void store_one(void *y, int dt, long long i, float v) {
+  if (dt == 0) static_cast<bf16_t *>(y)[i] = f2bf(v);
+  else if (dt == 1) static_cast<_Float16 *>(y)[i] = (_Float16)v;
+  else static_cast<float *>(y)[i] = v;
 }
-
-template <class F> PG_DEVICE float block_sum(float v, F *sh) {
+PG_DEVICE float block_sum(float v) {   // 256 threads
+  __shared__ float sh[4];
   v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += sh[i];
-  return s;
+  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// one workgroup per (b, g): mean, then the squares about it
-template <class T>
-__global__ __launch_bounds__(256) void gn_stats_kernel(const T *__restrict__ x, float *__restrict__ mean,
-                                                       float *__restrict__ rstd, long long S, int C, int G, float eps) {
-  __shared__ float sh[4];
-  const int cg = C / G;
-  const long long b = blockIdx.x / G, n = S * cg;
-  const T *src = x + b * S * C + (long long)(blockIdx.x % G) * cg;
-  float a = 0.f;
-  for (long long i = threadIdx.x; i < n; i += 256) a += tof(src[i / cg * C + i % cg]);
-  const float mu = block_sum(a, sh) / (float)n;
-  float v = 0.f;
+__global__ __launch_bounds__(256) void gn_wide_stats_kernel(const FwdArgs a, int dt) {
+  const Geo &g = a.g;
+  const long long n = g.S * g.cg, base = blockIdx.x / g.G * g.S * g.C + (long long)(blockIdx.x % g.G) * g.cg;
+  float s = 0.f, v = 0.f;
+  for (long long i = threadIdx.x; i < n; i += 256) s += load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg);
+  const float mu = block_sum(s) / (float)n;
   for (long long i = threadIdx.x; i < n; i += 256) {
-    const float d = tof(src[i / cg * C + i % cg]) - mu;
-    v += d * d;
+    const float d = load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg) - mu;
+    v = fmaf(d, d, v);
   }
-  v = block_sum(v, sh);
+  v = block_sum(v);
   if (threadIdx.x == 0) {
-    mean[blockIdx.x] = mu;
-    rstd[blockIdx.x] = 1.f / sqrtf(v / (float)n + eps);
+    a.mean[blockIdx.x] = mu;
+    a.rstd[blockIdx.x] = 1.f / sqrtf(v / (float)n + a.eps);
   }
 }
-
-template <class T>
-__global__ __launch_bounds__(256) void gn_apply_kernel(const T *__restrict__ x, const float *__restrict__ gamma,
-                                                       const float *__restrict__ beta, const float *__restrict__ mean,
-                                                       const float *__restrict__ rstd, T *__restrict__ y, long long n,
-                                                       long long SC, int C, int G, int act) {
+__global__ __launch_bounds__(256) void gn_wide_apply_kernel(const FwdArgs a, int dt) {
+  const Geo &g = a.g;
+  const long long n = g.B * g.S * g.C;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int c = (int)(i % C);
-    const long long k = i / SC * G + c / (C / G);
-    const float z = (tof(x[i]) - mean[k]) * rstd[k] * (gamma ? gamma[c] : 1.f) + (beta ? beta[c] : 0.f);
-    y[i] = fromf<T>(gn_act(z, act));
+    const int c = (int)(i % g.C);
+    const long long k = i / (g.S * g.C) * g.G + c / g.cg;
+    const float z = fmaf(load_one(a.x, dt, i) - a.mean[k], a.rstd[k] * (a.gamma ? a.gamma[c] : 1.f),
+                         a.beta ? a.beta[c] : 0.f);
+    store_one(a.y, dt, i, a.act == GN_RELU6 ? gn_act<GN_RELU6>(z) : a.act == GN_RELU ? gn_act<GN_RELU>(z)
+                              : a.act == GN_SILU ? gn_act<GN_SILU>(z) : z);
   }
 }
 
-// one workgroup per (b, c): sum dz, sum dz xh over S
-template <class T>
-__global__ __launch_bounds__(256) void gn_bwd_sums_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                          const uint8_t *__restrict__ q,
-                                                          const uint8_t *__restrict__ qs,
-                                                          const float *__restrict__ gamma,
-                                                          const float *__restrict__ beta,
-                                                          const float *__restrict__ mean,
-                                                          const float *__restrict__ rstd, float *__restrict__ part,
-                                                          long long S, int C, int G, int act) {
-  __shared__ float sh[4];
-  const long long b = blockIdx.x / C;
-  const int c = blockIdx.x % C, nb = (C + kMxBlock - 1) / kMxBlock;
-  const float mu = mean[b * G + c / (C / G)], rs = rstd[b * G + c / (C / G)];
-  const float g = gamma ? gamma[c] : 1.f, be = beta ? beta[c] : 0.f;
-  float a0 = 0.f, a1 = 0.f;
-  for (long long s = threadIdx.x; s < S; s += 256) {
-    const long long r = b * S + s, i = r * C + c;
-    const float v = x ? tof(x[i]) : mx8_dec1(q[i]) * mx8_scale(qs[r * nb + c / kMxBlock]);
-    const float dz = gn_dz(tof(dy[i]), v, mu, rs, g, be, act);
-    a0 += dz;
-    a1 += dz * ((v - mu) * rs);
+// value i's x - mean, gamma rstd and dz
+PG_DEVICE void wide_dz(const BwdArgs &a, int dt, long long r, int c, float &df, float &al, float &dz) {
+  const Geo &g = a.g;
+  const long long i = r * g.C + c, k = r / g.S * g.G + c / g.cg;
+  const int nb = (g.C + kMxBlock - 1) / kMxBlock, gi[1] = {0};
+  const float x[1] = {a.q ? mx8_dec1(a.q[i]) * mx8_scale(a.qs[r * nb + c / kMxBlock]) : load_one(a.x, dt, i)};
+  const float d[1] = {x[0] - a.mean[k]}, s[1] = {a.rstd[k] * (a.gamma ? a.gamma[c] : 1.f)};
+  const float b[1] = {a.beta ? a.beta[c] : 0.f};
+  float v[1] = {load_one(a.dy, dt, i)};
+  if (a.silu) gn_dz<true, 1, 1>(d, x, s, b, v, a, a.mean + k, a.rstd + k, gi, c);
+  else gn_dz<false, 1, 1>(d, x, s, b, v, a, a.mean + k, a.rstd + k, gi, c);
+  df = d[0];
+  al = s[0];
+  dz = v[0];
+}
+// one workgroup per (image, channel) -> dpart [B][2][C]
+__global__ __launch_bounds__(256) void gn_wide_dsums_kernel(const BwdArgs a, int dt) {
+  const Geo &g = a.g;
+  const long long b = blockIdx.x / g.C;
+  const int c = (int)(blockIdx.x % g.C);
+  float s0 = 0.f, s1 = 0.f, df, al, dz;
+  for (long long s = threadIdx.x; s < g.S; s += 256) {
+    wide_dz(a, dt, b * g.S + s, c, df, al, dz);
+    s0 += dz;
+    s1 = fmaf(dz, df, s1);
   }
-  a0 = block_sum(a0, sh);
-  a1 = block_sum(a1, sh);
+  s0 = block_sum(s0);
+  s1 = block_sum(s1);
   if (threadIdx.x == 0) {
-    part[(b * 2) * C + c] = a1;
-    part[(b * 2 + 1) * C + c] = a0;
+    a.dpart[b * 2 * g.C + c] = s1 * a.rstd[b * g.G + c / g.cg];
+    a.dpart[(b * 2 + 1) * g.C + c] = s0;
+  }
+}
+// one workgroup per (image, group) -> part [B * G][2]
+__global__ __launch_bounds__(256) void gn_wide_gsums_kernel(const BwdArgs a) {
+  const Geo &g = a.g;
+  const long long b = blockIdx.x / g.G;
+  const int c0 = (int)(blockIdx.x % g.G) * g.cg;
+  float u = 0.f, v = 0.f;
+  for (int c = c0 + threadIdx.x; c < c0 + g.cg; c += 256) {
+    const float ga = a.gamma ? a.gamma[c] : 1.f;
+    v = fmaf(ga, a.dpart[b * 2 * g.C + c], v);
+    u = fmaf(ga, a.dpart[(b * 2 + 1) * g.C + c], u);
+  }
+  u = block_sum(u);
+  v = block_sum(v);
+  if (threadIdx.x == 0) {
+    a.part[2ll * blockIdx.x] = u;
+    a.part[2ll * blockIdx.x + 1] = v;
+  }
+}
+__global__ __launch_bounds__(256) void gn_wide_dx_kernel(const BwdArgs a, int dt) {
+  const Geo &g = a.g;
+  const long long n = g.B * g.S * g.C;
+  const float rm = 1.f / ((float)g.S * (float)g.cg);
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long r = i / g.C;
+    const int c = (int)(i % g.C);
+    float df, al, dz;
+    wide_dz(a, dt, r, c, df, al, dz);
+    const long long k = r / g.S * g.G + c / g.cg;
+    const float rs = a.rstd[k];
+    store_one(a.dx, dt, i, fmaf(dz, al, -fmaf(df, rs * rs * a.part[2 * k + 1] * rm, rs * a.part[2 * k] * rm)));
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void gn_bwd_apply_kernel(const T *__restrict__ dy, const T *__restrict__ x,
-                                                           const uint8_t *__restrict__ q,
-                                                           const uint8_t *__restrict__ qs,
-                                                           const float *__restrict__ gamma,
-                                                           const float *__restrict__ beta,
-                                                           const float *__restrict__ mean,
-                                                           const float *__restrict__ rstd,
-                                                           const float *__restrict__ part, T *__restrict__ dx,
-                                                           long long n, long long S, int C, int G, int act) {
-  const int cg = C / G, nb = (C + kMxBlock - 1) / kMxBlock;
-  const float rm = 1.f / ((float)S * (float)cg);
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int c = (int)(i % C), g0 = c / cg * cg;
-    const long long r = i / C, b = r / S, k = b * G + c / cg;
-    float s1 = 0.f, s2 = 0.f;
-    for (int j = g0; j < g0 + cg; ++j) {
-      const float g = gamma ? gamma[j] : 1.f;
-      s2 += g * part[(b * 2) * C + j];
-      s1 += g * part[(b * 2 + 1) * C + j];
+// ---- dgamma, dbeta: column sums of [rows][n] in a fixed order -----------------------------------
+// grid (columns / 64, row splits): 64 columns x 16 stripes of rows; with one split dst is the result
+__global__ __launch_bounds__(1024) void gn_dparam_kernel(const float *__restrict__ part, float *__restrict__ dst,
+                                                         long long rows, int n, int split) {
+  __shared__ float sh[16][64];
+  const int col = threadIdx.x & 63, st = threadIdx.x >> 6, j = blockIdx.x * 64 + col;
+  const long long r0 = (long long)blockIdx.y * split, r1 = min(rows, r0 + split);
+  float s = 0.f;
+  if (j < n)
+    for (long long r = r0 + st; r < r1; r += 16) s += part[r * n + j];
+  sh[st][col] = s;
+  __syncthreads();
+  if (st == 0 && j < n) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += sh[i][col];
+    dst[(size_t)blockIdx.y * n + j] = s;
+  }
+}
+
+__global__ __launch_bounds__(256) void gn_zero_kernel(int *__restrict__ p, long long n) {
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+// ---- host: geometry ----------------------------------------------------------------------------
+constexpr int kMaxCluster = 192;   // tiles that wait for one another; at least 512 are resident
+constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
+int g_wait = 1 << 20;
+
+int gcd_pow2(long long c, int most) {
+  int v = most;
+  while (c % v) v >>= 1;
+  return v;
+}
+
+// the sums and rows that a workgroup holds in shared memory
+size_t gn_lds(const Plan &p, bool bwd) {
+  const size_t red = (size_t)p.TH * p.V;
+  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 2 * (size_t)p.g.cs + p.TH : 0) + red);
+}
+
+Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {
+  Plan p{};
+  Geo &g = p.g;
+  g.B = B;
+  g.S = S;
+  g.C = C;
+  g.G = G;
+  g.cg = C / G;
+  g.wait = g_wait;
+  const int elt = dt == 2 ? 4 : 2;
+  const int V = gcd_pow2(C, 16 / elt);
+  p.V = V;
+  const int only = V * elt < 16 ? 4 : g.cg % V ? 2 : 0;   // NV of the kinds of vector that have one
+  const int Q = ck && !bwd ? kMxBlock / V : 1;   // lanes of a checkpoint block
+  // a slab is made of whole groups, vectors and (where they are written) checkpoint blocks
+  long long L = std::lcm<long long>(g.cg, V);
+  if (ck && !bwd) L = std::lcm<long long>(L, kMxBlock);
+  if (L > C) L = C;
+  auto shape = [&](long long cs) {
+    g.cs = (int)std::min<long long>(cs, C);
+    g.nslab = (C + g.cs - 1) / g.cs;
+    g.gs = g.cs / g.cg;
+    g.CVp = (g.cs / V + Q - 1) / Q * Q;
+  };
+  auto check = [&](long long k) {   // grid and in-tile offsets
+    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)g.R * p.NV * C * elt > 0x7fffffff)
+      throw std::invalid_argument("group norm: sizes past the kernels' 32-bit grid and tile offsets");
+  };
+  const int most = bwd ? 512 : 1024;
+  const int nvs[3] = {2, 4, 8};
+  const int nv_most = bwd ? 4 : 8;
+  // solo: rows of 128 bytes at least, more while the tile is small and the chip stays full
+  long long cs = (128 / elt + L - 1) / L * L;
+  while (cs < C && S * cs * elt < 16384 && B * ((C + 2 * cs - 1) / (2 * cs)) >= 1024) cs *= 2;
+  shape(cs);
+  if (g.CVp <= 1024) {
+    for (int nv : nvs) {
+      if (nv > nv_most) break;
+      if (only && nv != only) continue;
+      const long long rows = (S + nv - 1) / nv;   // sweeps of R rows each
+      const long long th = (rows * g.CVp + 63) / 64 * 64;
+      if (th <= std::max(most, (g.CVp + 63) / 64 * 64) && th * nv <= 4096 + 64 * nv) {
+        p.NV = nv;
+        p.TH = (int)th;
+        g.R = p.TH / g.CVp;
+        g.k = 1;
+        if (gn_lds(p, bwd) > 65536) break;
+        p.mode = SOLO;
+        p.wgs = B * g.nslab;
+        check(1);
+        return p;
+      }
     }
-    const float v = x ? tof(x[i]) : mx8_dec1(q[i]) * mx8_scale(qs[r * nb + c / kMxBlock]);
-    const float g = gamma ? gamma[c] : 1.f;
-    const float dz = gn_dz(tof(dy[i]), v, mean[k], rstd[k], g, beta ? beta[c] : 0.f, act);
-    dx[i] = fromf<T>(rstd[k] * (dz * g - (s1 + (v - mean[k]) * rstd[k] * s2) * rm));
   }
+  // whole rows where they fit a workgroup, the fewest slabs otherwise
+  long long slabs = 1;
+  for (;; ++slabs) {
+    cs = ((C + slabs - 1) / slabs + L - 1) / L * L;
+    shape(cs);
+    if (g.CVp <= (bwd ? 512 : 1024) || cs == L) break;
+  }
+  p.TH = std::max(512, (g.CVp + 63) / 64 * 64);
+  if (g.CVp > 1024 || gn_lds(p, bwd) > 65536) {
+    p.mode = WIDE;
+    g.k = 1;
+    g.nslab = G;   // sums per (image, group)
+    g.gs = 1;
+    p.wgs = B * G;
+    return p;
+  }
+  g.R = p.TH / g.CVp;
+  // fewer rows a tile while the tiles do not fill the chip
+  p.NV = nv_most;
+  auto tiles = [&](int nv) { return (S + (long long)g.R * nv - 1) / ((long long)g.R * nv); };
+  while (p.NV > 2 && B * g.nslab * tiles(p.NV) < 512) p.NV /= 2;
+  if (only) p.NV = only;
+  const long long k = tiles(p.NV);
+  g.k = (int)k;
+  p.mode = g.k == 1 ? SOLO : g.k <= kMaxCluster ? CLUSTER : SUMS;
+  p.wgs = B * g.nslab * k;
+  check(k);
+  return p;
 }
 
-// out[j] = sum over rows of part[row][j], rows in order
-__global__ __launch_bounds__(256) void gn_dparam_kernel(const float *__restrict__ part, float *__restrict__ out,
-                                                        long long rows, int n) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
-  float a = 0.f;
-  for (long long r = 0; r < rows; ++r) a += part[r * n + j];
-  out[j] = a;
+struct Ws {
+  long long ctr, part, dpart, lvl, total;   // offsets in floats
+};
+long long up4(long long n) { return (n + 3) / 4 * 4; }
+Ws gn_ws(const Plan &p, bool bwd) {
+  Ws w{};
+  const Geo &g = p.g;
+  if (p.mode != SOLO) {
+    w.part = up4(g.B * g.nslab);
+    w.dpart = w.part + up4(p.wgs * g.gs * 2);
+  }
+  w.lvl = w.dpart;
+  if (bwd) {
+    const long long rows = g.B * g.k;
+    w.lvl = w.dpart + rows * 2 * g.C;
+    w.total = w.lvl + (rows > 16 * kSplitRows ? (long long)kSplitRows * 2 * g.C : 0);
+  } else {
+    w.total = w.lvl;
+  }
+  return w;
 }
 
-unsigned gn_grid(long long n) { return (unsigned)(n + 255 < 256ll * 65536 ? (n + 255) / 256 : 65536); }
+void gn_zero(const Plan &p, int *ctr, hipStream_t st) {
+  if (p.mode != CLUSTER) return;
+  const long long n = p.g.B * p.g.nslab;
+  hipLaunchKernelGGL(gn_zero_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, ctr, n);
+}
+
 }  // namespace
 
 void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M, int C, hipStream_t st);
 
-// dt: 0 bf16, 1 fp16, 2 fp32
-long long gn_workspace_floats(int, long long B, long long, int C, int, int bwd) { return bwd ? 2 * B * C : 0; }
+// polls of a cluster's wait (tests set 0: every workgroup then computes all sums itself)
+void gn_set_wait(int polls) { g_wait = polls < 0 ? 0 : polls; }
+
+// dt: 0 bf16, 1 fp16, 2 fp32.  Forward and backward, with and without a checkpoint: the largest.
+long long gn_workspace_floats(int dt, long long B, long long S, int C, int G, int bwd) {
+  if (B * S <= 0) return 0;
+  return std::max(gn_ws(gn_plan(dt, B, S, C, G, false, bwd), bwd).total,
+                  gn_ws(gn_plan(dt, B, S, C, G, true, bwd), bwd).total);
+}
 
 void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                    uint8_t *q, uint8_t *qs, float *ws, long long B, long long S, int C, int G, float eps, int act,
                    hipStream_t st) {
-  (void)ws;
-  const long long n = B * S * C;
-#define FWD(T)                                                                                                     \
-  hipLaunchKernelGGL(gn_stats_kernel<T>, dim3((unsigned)(B * G)), dim3(256), 0, st, (const T *)x, mean, rstd, S, C, G, \
-                     eps);                                                                                          \
-  hipLaunchKernelGGL(gn_apply_kernel<T>, dim3(gn_grid(n)), dim3(256), 0, st, (const T *)x, gamma, beta, mean, rstd,  \
-                     (T *)y, n, S *C, C, G, act)
-  if (dt == 0) { FWD(bf16_t); }
-  else if (dt == 1) { FWD(_Float16); }
-  else { FWD(float); }
-#undef FWD
-  if (q) launch_mx8_pack(dt, x, q, qs, B * S, C, st);
+  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, false);
+  const Ws w = gn_ws(p, false);
+  const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<int *>(ws) + w.ctr, ws + w.part, eps, act};
+  gn_zero(p, a.ctr, st);
+  if (p.mode == WIDE) {
+    const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));
+    hipLaunchKernelGGL(gn_wide_stats_kernel, dim3((unsigned)p.wgs), dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_apply_kernel, grid, dim3(256), 0, st, a, dt);
+    if (q) launch_mx8_pack(dt, x, q, qs, B * S, C, st);
+    return;
+  }
+  (dt == 0 ? fwd_bf16 : dt == 1 ? fwd_fp16 : fwd_fp32)(p, gn_lds(p, false), a, st);
 }
 
 void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, const uint8_t *qs, const float *gamma,
                    const float *beta, const float *mean, const float *rstd, void *dx, float *dgb, float *ws,
                    long long B, long long S, int C, int G, int act, hipStream_t st) {
-  const long long n = B * S * C;
-#define BWD(T)                                                                                                    \
-  hipLaunchKernelGGL(gn_bwd_sums_kernel<T>, dim3((unsigned)(B * C)), dim3(256), 0, st, (const T *)dy, (const T *)x, q, \
-                     qs, gamma, beta, mean, rstd, ws, S, C, G, act);                                               \
-  hipLaunchKernelGGL(gn_bwd_apply_kernel<T>, dim3(gn_grid(n)), dim3(256), 0, st, (const T *)dy, (const T *)x, q, qs,  \
-                     gamma, beta, mean, rstd, ws, (T *)dx, n, S, C, G, act)
-  if (dt == 0) { BWD(bf16_t); }
-  else if (dt == 1) { BWD(_Float16); }
-  else { BWD(float); }
-#undef BWD
-  if (dgb) hipLaunchKernelGGL(gn_dparam_kernel, dim3((2 * C + 255) / 256), dim3(256), 0, st, ws, dgb, B, 2 * C);
+  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, true);
+  const Ws w = gn_ws(p, true);
+  const BwdArgs a{p.g, dy, x, q, qs, gamma, beta, mean, rstd, dx, reinterpret_cast<int *>(ws) + w.ctr, ws + w.part,
+                  dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act == GN_SILU, act == GN_NONE ? -INFINITY : 0.f,
+                  act == GN_RELU6 ? 6.f : INFINITY};
+  gn_zero(p, a.ctr, st);
+  if (p.mode == WIDE) {
+    if (B * C > 0x7fffffff) throw std::invalid_argument("gn_bwd: B * C is too large");
+    const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));
+    hipLaunchKernelGGL(gn_wide_dsums_kernel, dim3((unsigned)(B * C)), dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_gsums_kernel, dim3((unsigned)p.wgs), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(gn_wide_dx_kernel, grid, dim3(256), 0, st, a, dt);
+  } else {
+    (dt == 0 ? bwd_bf16 : dt == 1 ? bwd_fp16 : bwd_fp32)(p, gn_lds(p, true), a, st);
+  }
+  if (!dgb) return;
+  const long long rows = B * p.g.k;
+  const unsigned nb = (2 * C + 63) / 64;
+  if (rows > 16 * kSplitRows) {
+    const int split = (int)((rows + kSplitRows - 1) / kSplitRows), ns = (int)((rows + split - 1) / split);
+    hipLaunchKernelGGL(gn_dparam_kernel, dim3(nb, ns), dim3(1024), 0, st, ws + w.dpart, ws + w.lvl, rows, 2 * C, split);
+    hipLaunchKernelGGL(gn_dparam_kernel, dim3(nb), dim3(1024), 0, st, ws + w.lvl, dgb, (long long)ns, 2 * C, ns);
+  } else {
+    hipLaunchKernelGGL(gn_dparam_kernel, dim3(nb), dim3(1024), 0, st, ws + w.dpart, dgb, rows, 2 * C, (int)rows);
+  }
 }

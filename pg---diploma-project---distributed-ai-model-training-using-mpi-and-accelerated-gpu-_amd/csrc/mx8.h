@@ -42,4 +42,15 @@ PG_DEVICE uint32_t mx8_enc4(float a, float b, float c, float d) {
   return (uint32_t)mx8_enc2<true>(c, d, mx8_enc2<false>(a, b, 0));
 }
 PG_DEVICE uint8_t mx8_enc1(float a) { return (uint8_t)(mx8_enc2<false>(a, 0.f, 0) & 0xff); }
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+// codes of the low or high half of w -> values (code times sc)
+template <bool HI> PG_DEVICE void mx8_dec2(uint32_t w, float sc, float &a, float &b) {
+  const f32x2_t v = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, HI);
+  a = v.x * sc;
+  b = v.y * sc;
+}
+PG_DEVICE void mx8_dec4(uint32_t w, float sc, float &a, float &b, float &c, float &d) {
+  mx8_dec2<false>(w, sc, a, b);
+  mx8_dec2<true>(w, sc, c, d);
+}
 PG_DEVICE float mx8_dec1(uint8_t q) { return __builtin_amdgcn_cvt_f32_fp8((int)q, 0); }

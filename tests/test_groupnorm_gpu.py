@@ -126,6 +126,52 @@ def test_backward_against_differences(act):
         assert abs(num - terms.sum().item()) <= 1e-5 * terms.abs().sum().item() + 1e-6
 
 
+# groups of more vectors than a workgroup has threads; maps of more tiles than wait for one another
+FAR_SIZES = [(2, 9, 2049, 1), (1, 5, 4100, 2), (2, 3, 9000, 1), (1, 400000, 32, 4), (1, 300001, 12, 3), (2, 130000, 75, 5)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("i", range(len(FAR_SIZES)))
+def test_wide_groups_and_long_maps(i, dtype):
+    B, S, C, G = FAR_SIZES[i]
+    act = (0, 1, 3, 2, 3, 1)[i]
+    x, gamma, beta, dy = make(B, S, C, DT[dtype], 70 + i)
+    y, mean, rstd, q, qs = call_fwd(x, gamma, beta, B, S, C, G, act, True)
+    want, bound = O.fwd(x, gamma, beta, B, S, C, G, EPS, act)
+    for got, w, b in zip((y, mean, rstd), want, bound):
+        O.within(got, w, b)
+    wq, ws = O.pack(x.view(B * S, C))
+    assert torch.equal(qs, ws) and torch.equal(q, wq)
+    for ck in (False, True):
+        v = O.unpack(q, qs) if ck else x
+        dx, dgb = call_bwd(dy, None if ck else x, gamma, beta, mean, rstd, B, S, C, G, act, q if ck else None,
+                           qs if ck else None)
+        want, bound = O.bwd(dy, v, gamma, beta, mean, rstd, B, S, C, G, act)
+        for got, w, b in zip((dx, dgb[0], dgb[1]), want, bound):
+            O.within(got, w, b)
+
+
+@pytest.mark.parametrize("size", [(2, 12544, 96, 12), (3, 6001, 33, 3), (2, 3136, 144, 18)])
+def test_a_peer_that_does_not_come(size):
+    """With no polls left a workgroup computes its peers' sums itself, to the same bits."""
+    B, S, C, G = size
+    lib = K.lib()
+    for dt in (torch.bfloat16, torch.float32):
+        x, gamma, beta, dy = make(B, S, C, dt, 8)
+        out = []
+        try:
+            for polls in (1 << 20, 0):
+                lib.gn_set_wait(polls)
+                for act in (2, 3):
+                    y, mean, rstd, q, qs = call_fwd(x, gamma, beta, B, S, C, G, act, True)
+                    out.append((y, mean, rstd, q, qs, *call_bwd(dy, x, gamma, beta, mean, rstd, B, S, C, G, act),
+                                *call_bwd(dy, None, gamma, beta, mean, rstd, B, S, C, G, act, q, qs)))
+        finally:
+            lib.gn_set_wait(1 << 20)
+        for a, b in zip(out[:2], out[2:]):
+            assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
 def test_far_mean_keeps_its_variance():
     """mean 1000, deviation 1: the squares are taken about the mean, not as E[x^2] - mean^2."""
     for B, S, C, G in ((1, 196, 32, 4), (1, 60000, 8, 1), (2, 12544, 64, 2)):

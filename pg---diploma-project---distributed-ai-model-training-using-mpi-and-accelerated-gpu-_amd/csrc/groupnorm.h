@@ -5,17 +5,19 @@
 //   dz = dy act'(z), xh = (x - mean) rstd:  dgamma = sum dz xh, dbeta = sum dz,
 //   dx = rstd (dz gamma - (s1 + xh s2) / m), s1 = sum_g dz gamma, s2 = sum_g dz gamma xh
 //
-// Both are bound by memory: what matters is to read every value once.  A workgroup therefore keeps
-// its rows x channels tile in registers between the statistics and the use of them:
-//   solo     the tile is all S rows of a slab of whole groups: one launch, nothing exchanged
-//   cluster  the S rows are split over k workgroups; each publishes its tile's sums, waits for the
-//            other k - 1 and goes on with the tile it still holds.  Also one read.
-//   split    k is larger than what is sure to be resident together: sums and use are two launches
-//            and the tile is read twice.
+// Both are bound by memory.  What reads a tile twice is kept close to where it was read first:
+//   solo     a workgroup holds all S rows of a slab of whole groups in registers: one read
+//   staged   longer maps: the S rows are k tiles.  One launch holds a sums and a use workgroup for
+//            every tile; the use of an image's tiles is queued `lead` images behind its sums, so
+//            that it hardly ever waits for them and finds the tile in the memory-side cache
+//            (256 MB).  HBM sees every value once.
 //   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
 //            one workgroup per (image, group), then one value a thread.
+// (Holding the tiles in registers while the k workgroups of an image exchange their sums also reads
+// once, but the chain load - sum - publish - wait - join - store of one workgroup is some 60 us and
+// only two of them fit a CU: 128 x 12544 x 96 backward took 1129 us.)
 // A thread owns one vector of V channels (16 bytes where C allows) and every R-th row of the tile.
-// Sums are taken in a fixed order in all three, so results do not vary from run to run.
+// Sums are taken in a fixed order, so results do not vary from run to run.
 #pragma once
 #include "mx8.h"
 #include "reduce.h"
@@ -24,7 +26,7 @@
 
 namespace gn {
 enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_RELU6 = 2, GN_SILU = 3 };
-enum GnMode : int { SOLO = 0, CLUSTER = 1, SUMS = 2, APPLY = 3, WIDE = 4 };
+enum GnMode : int { SOLO = 0, STAGED = 1, WIDE = 2 };
 
 // ---- vectors of V channels -------------------------------------------------------------------
 template <int BYTES> struct RawOf;
@@ -86,25 +88,52 @@ struct Geo {
   int nslab;
   int CVp;      // vector columns of a tile row (padded to whole 32-channel blocks for checkpoints)
   int R;        // tile rows per sweep: blockDim / CVp
-  int k;        // tiles per (image, slab)
+  int k;        // tiles per unit, a unit being one (image, slab)
   int gs;       // groups of a full slab
-  int wait;     // polls before a workgroup computes the others' sums itself
+  long long lead;   // tiles that sums workgroups are ahead of use workgroups: a multiple of k
+  int wait;     // polls after which a use workgroup takes its sums from the tensor itself
 };
 
 // this workgroup's place
 struct Place {
-  long long b, bs;   // image; image * nslab + slab
+  long long b, unit;   // image; image * nslab + slab
   int chunk, c0, csl, ng, g0;
   int col, row, c;
-  bool on;           // this thread has a column
+  bool on;             // this thread has a column
+  bool use;            // staged: applies the sums (else: makes them)
 };
-template <int V> PG_DEVICE Place place(const Geo &g) {
+// Staged order: `lead` sums tiles, then the remaining sums tiles alternating, 8 and 8 (one round of
+// the 8 XCDs each), with the use tiles `lead` behind them, then the last `lead` use tiles.  A use
+// workgroup waits only for sums workgroups of lower index, which each XCD starts first, and those
+// wait for nobody.  (Handing the places out by an atomic counter makes that order certain, but one
+// address takes 32 ns an increment: 128 x 12544 x 96 backward 630 us.  Should the order ever be
+// another, the wait is bounded and the work is done without the peers.)
+template <int V, int MODE> PG_DEVICE Place place(const Geo &g) {
   Place p;
-  const int id = blockIdx.x;
-  p.chunk = id % g.k;
-  p.bs = id / g.k;
-  const int slab = (int)(p.bs % g.nslab);
-  p.b = p.bs / g.nslab;
+  long long id = blockIdx.x;
+  p.use = false;
+  if constexpr (MODE == STAGED) {
+    const long long both = g.B * g.nslab * g.k - g.lead, even = both & ~7ll;
+    if (id >= g.lead) {
+      id -= g.lead;
+      if (id < 2 * even) {
+        p.use = (id >> 3) & 1;
+        id = (id >> 4) * 8 + (id & 7);
+      } else if (id < 2 * both) {
+        const int r = (int)(id - 2 * even), rest = (int)(both - even);
+        p.use = r >= rest;
+        id = even + (p.use ? r - rest : r);
+      } else {
+        p.use = true;
+        id -= both;
+      }
+      if (!p.use) id += g.lead;
+    }
+  }
+  p.chunk = (int)(id % g.k);
+  p.unit = id / g.k;
+  const int slab = (int)(p.unit % g.nslab);
+  p.b = p.unit / g.nslab;
   p.c0 = slab * g.cs;
   p.csl = min(g.cs, g.C - p.c0);
   p.ng = p.csl / g.cg;
@@ -165,22 +194,53 @@ PG_DEVICE void group_sums(const Geo &g, const Place &p, const float (&acc)[V], f
   __syncthreads();
 }
 
-// One arrival of this workgroup, then the wait for all k.  Published values were stored with st_sc1.
-// True: all have arrived.  False (uniformly): not within `polls`, the caller does the work itself.
-PG_DEVICE bool arrive_and_wait(int *ctr, int k, int polls, int *flag) {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int n = __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
-    for (int i = 0; n < k && i < polls; ++i) {
-      __builtin_amdgcn_s_sleep(1);
-      n = __hip_atomic_load(ctr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    *flag = n >= k;
-  }
-  __syncthreads();
-  return *flag != 0;
+// Hand-over of a unit's sums: a tile's two sums of a group are one 64-bit word, written and read in
+// one piece at agent scope.  kNone, which no computed pair holds, says that they have not come.
+constexpr unsigned long long kNone = ~0ull;
+PG_DEVICE void pair_store(unsigned long long *p, float a, float b) {
+  const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b);   // a NaN of all ones: any other
+  __hip_atomic_store(p, (unsigned long long)(ua == ~0u ? 0x7fc00000u : ua) | ((unsigned long long)ub << 32),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+PG_DEVICE unsigned long long pair_load(const unsigned long long *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// the lane's pairs (tiles l, l + W, ..) of a group, in order; false: one of the wave's did not come
+template <class F> PG_DEVICE bool pairs(const unsigned long long *src, int gs, int k, int l, int W, int polls, F f) {
+  if (polls < 0) return false;
+  for (int c0 = 0; c0 < k; c0 += 4 * W) {   // four loads in flight
+    unsigned long long v[4];
+    for (int i = 0;; ++i) {
+      bool none = false;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int ch = c0 + u * W + l;
+        v[u] = pair_load(src + (long long)(ch < k ? ch : l < k ? l : 0) * gs);
+        none |= v[u] == kNone;
+      }
+      if (!__any(none)) break;
+      if (i >= polls) return false;
+      __builtin_amdgcn_s_sleep(4);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int ch = c0 + u * W + l;
+      if (ch < k) f(ch, __uint_as_float((unsigned)v[u]), __uint_as_float((unsigned)(v[u] >> 32)));
+    }
+  }
+  return true;
+}
+
+// count, mean and sum of squares about it; joined without ever forming E[x^2]
+struct Moments {
+  float n, m, v;
+  PG_DEVICE void join(float n2, float m2, float v2) {
+    const float t = n + n2, d = m2 - m, w = t > 0.f ? n2 / t : 0.f;
+    m = fmaf(d, w, m);
+    v += fmaf(d * d, n * w, v2);
+    n = t;
+  }
+};
 
 // ---- forward ---------------------------------------------------------------------------------
 struct FwdArgs {
@@ -190,8 +250,7 @@ struct FwdArgs {
   void *y;
   float *mean, *rstd;
   uint8_t *q, *qs;
-  int *ctr;      // [B * nslab] arrivals (cluster)
-  float *part;   // [B * nslab][k][gs][2]: mean and sum of squares about it of every tile and group
+  unsigned long long *part;   // [B * nslab][k][gs]: mean and sum of squares about it of every tile and group
   float eps;
   int act;
 };
@@ -209,9 +268,8 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(const FwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   const Geo &g = a.g;
-  const Place p = place<V>(g);
+  const Place p = place<V, MODE>(g);
   float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
-  __shared__ int flag;
   const int tile = g.R * NV;
   constexpr int VG = FOLD ? 1 : V;
   int gi[VG];   // slab group of each channel (FOLD: of all)
@@ -266,68 +324,14 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(const FwdArgs a) {
     for (int i = threadIdx.x + blockDim.x; i < p.ng; i += blockDim.x) gm[i] *= rn;
     group_sums<V, FOLD>(g, p, acc, red, gr);
   };
-  auto publish = [&](int chunk) {
-    float *dst = a.part + ((p.bs * g.k + chunk) * g.gs) * 2;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
-      st_sc1(dst + 2 * i, gm[i]);
-      st_sc1(dst + 2 * i + 1, gr[i]);
-    }
+  auto publish = [&]() {
+    unsigned long long *dst = a.part + (p.unit * g.k + p.chunk) * g.gs;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(dst + i, gm[i], gr[i]);
   };
 
-  if constexpr (MODE == CLUSTER) {
-    // The first round is this workgroup's own tile.  Where a peer does not come in time the others
-    // follow, computed here to the same bits as theirs, its own again at the end.
-    for (int i = 0, ch = p.chunk;;) {
-      load(ch);
-      __syncthreads();
-      sums();
-      publish(ch);
-      if (i == 0 ? arrive_and_wait(a.ctr + p.bs, g.k, g.wait, &flag) : i == g.k) break;
-      ++i;
-      ch = p.chunk + i < g.k ? p.chunk + i : p.chunk + i - g.k;
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  } else {
-    load(p.chunk);
-    if constexpr (MODE != APPLY) sums();
-    if constexpr (MODE == SUMS) {
-      publish(p.chunk);
-      return;
-    }
-  }
-  const float n = (float)g.S * (float)g.cg;
-  if constexpr (MODE == SOLO) {
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
-  } else {   // join the tiles: W lanes a group
-    const float *src = a.part + p.bs * g.k * g.gs * 2;
-    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-    auto count = [&](int ch) { return (float)min((long long)tile, g.S - (long long)ch * tile) * (float)g.cg; };
-    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-      float m = 0.f, v = 0.f;
-      if (i < p.ng)
-        for (int ch = l; ch < g.k; ch += W) m += count(ch) * ld_sc1(src + (ch * g.gs + i) * 2);
-      m = seg_sum(m, W) / n;
-      if (i < p.ng)
-        for (int ch = l; ch < g.k; ch += W) {
-          const float dm = ld_sc1(src + (ch * g.gs + i) * 2) - m;
-          v += ld_sc1(src + (ch * g.gs + i) * 2 + 1) + count(ch) * dm * dm;
-        }
-      v = seg_sum(v, W);
-      if (l == 0 && i < p.ng) {
-        gm[i] = m;
-        gr[i] = 1.f / sqrtf(v / n + a.eps);
-      }
-    }
-  }
-  __syncthreads();
-  if (p.chunk == 0)
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
-      a.mean[p.b * g.G + p.g0 + i] = gm[i];
-      a.rstd[p.b * g.G + p.g0 + i] = gr[i];
-    }
-  if constexpr (CK) {
-    // the checkpoint: 32 channels are 32 / V neighbouring lanes (CVp is a multiple of that).
+  load(p.chunk);
+  if (CK && !p.use) {
+    // the checkpoint leaves first; 32 channels are 32 / V neighbouring lanes (CVp is a multiple of that).
     const long long r0 = p.b * g.S + (long long)p.chunk * tile;
     const int nb = (g.C + kMxBlock - 1) / kMxBlock;
 #pragma unroll
@@ -346,6 +350,44 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(const FwdArgs a) {
       }
     }
   }
+  if constexpr (MODE == SOLO) {
+    sums();
+    const float n = (float)g.S * (float)g.cg;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
+  } else {
+    if (!p.use) {
+      sums();
+      publish();
+      return;
+    }
+    // join the tiles: W lanes a group
+    const unsigned long long *src = a.part + p.unit * g.k * g.gs;
+    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+      Moments t{0.f, 0.f, 0.f};
+      const int gc = min(i, p.ng - 1);
+      if (!pairs(src + gc, g.gs, g.k, l, W, g.wait, [&](int ch, float m, float v) {
+            t.join((float)min((long long)tile, g.S - (long long)ch * tile) * (float)g.cg, m, v);
+          })) {
+        // without the peers: every W-th value of the group, from the tensor
+        const T *base = static_cast<const T *>(a.x) + p.b * g.S * g.C + p.c0 + gc * g.cg;
+        t = Moments{0.f, 0.f, 0.f};
+        for (long long r = l; r < g.S; r += W)
+          for (int c = 0; c < g.cg; ++c) t.join(1.f, tof(base[r * g.C + c]), 0.f);
+      }
+      for (int o = 1; o < W; o <<= 1) t.join(__shfl_xor(t.n, o, 64), __shfl_xor(t.m, o, 64), __shfl_xor(t.v, o, 64));
+      if (l == 0 && i < p.ng) {
+        gm[i] = t.m;
+        gr[i] = 1.f / sqrtf(t.v / t.n + a.eps);
+      }
+    }
+  }
+  __syncthreads();
+  if (p.chunk == 0)
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
+      a.mean[p.b * g.G + p.g0 + i] = gm[i];
+      a.rstd[p.b * g.G + p.g0 + i] = gr[i];
+    }
   if (!p.on) return;
   float mu[VG], sc[V], be[V];
 #pragma unroll
@@ -382,8 +424,7 @@ struct BwdArgs {
   const uint8_t *q, *qs;
   const float *gamma, *beta, *mean, *rstd;
   void *dx;
-  int *ctr;       // [B * nslab]
-  float *part;    // [B * nslab][k][gs][2]: s1, s2 of every tile and group
+  unsigned long long *part;   // [B * nslab][k][gs]: s1, s2 of every tile and group
   float *dpart;   // [B * k][2][C]: dgamma, dbeta of every tile, or null
   int silu;
   float lo, hi;   // the other activations' borders
@@ -439,10 +480,9 @@ __global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   const Geo &g = a.g;
-  const Place p = place<V>(g);
+  const Place p = place<V, MODE>(g);
   // sums of the slab's groups, its channels' sums, the reduction's rows
   float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
-  __shared__ int flag;
   const int tile = g.R * NV, nb = (g.C + kMxBlock - 1) / kMxBlock;
   const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
   constexpr int VG = FOLD ? 1 : V;
@@ -553,46 +593,51 @@ __global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
     }
     __syncthreads();
   };
-  auto publish = [&](int chunk) {
-    float *dst = a.part + ((p.bs * g.k + chunk) * g.gs) * 2;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
-      st_sc1(dst + 2 * i, g1[i]);
-      st_sc1(dst + 2 * i + 1, g2[i]);
-    }
+  auto publish = [&]() {
+    unsigned long long *dst = a.part + (p.unit * g.k + p.chunk) * g.gs;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(dst + i, g1[i], g2[i]);
   };
-  for (int i = 0, ch = p.chunk;;) {   // more than one round only as in the forward
-    load(ch);
-    if constexpr (MODE == APPLY) break;
-    if constexpr (MODE == CLUSTER) __syncthreads();
+  load(p.chunk);
+  if (MODE == SOLO || !p.use) {
     sums();
-    if (i == 0 && a.dpart) {
-      float *dst = a.dpart + (p.b * g.k + ch) * 2 * g.C + p.c0;
+    if (a.dpart) {
+      float *dst = a.dpart + (p.b * g.k + p.chunk) * 2 * g.C + p.c0;
       for (int j = threadIdx.x; j < p.csl; j += blockDim.x) {
         dst[j] = tot[j];
         dst[g.C + j] = tot[g.cs + j];
       }
     }
-    if constexpr (MODE == SOLO) break;
-    publish(ch);
-    if constexpr (MODE == SUMS) return;
-    if (i == 0 ? arrive_and_wait(a.ctr + p.bs, g.k, g.wait, &flag) : i == g.k) break;
-    ++i;
-    ch = p.chunk + i < g.k ? p.chunk + i : p.chunk + i - g.k;
-  }
-  if constexpr (MODE == CLUSTER) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    if constexpr (MODE == STAGED) {
+      publish();
+      return;
+    }
   }
   if constexpr (MODE != SOLO) {
-    const float *src = a.part + p.bs * g.k * g.gs * 2;
+    const unsigned long long *src = a.part + p.unit * g.k * g.gs;
     const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
     for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
       float u = 0.f, v = 0.f;
-      if (i < p.ng)
-        for (int ch = l; ch < g.k; ch += W) {
-          u += ld_sc1(src + (ch * g.gs + i) * 2);
-          v += ld_sc1(src + (ch * g.gs + i) * 2 + 1);
-        }
+      const int gc = min(i, p.ng - 1);
+      if (!pairs(src + gc, g.gs, g.k, l, W, g.wait, [&](int, float s1, float s2) {
+            u += s1;
+            v += s2;
+          })) {   // as in the forward
+        u = v = 0.f;
+        const float m = mean[gc], rs = rstd[gc];
+        for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
+          for (int c = p.c0 + gc * g.cg; c < p.c0 + (gc + 1) * g.cg; ++c) {
+            const float ga = a.gamma ? a.gamma[c] : 1.f;
+            float x[1], df[1], z[1] = {tof(static_cast<const T *>(a.dy)[r * g.C + c])};
+            if constexpr (CK) x[0] = mx8_dec1(a.q[r * g.C + c]) * mx8_scale(a.qs[r * nb + c / kMxBlock]);
+            else x[0] = tof(static_cast<const T *>(a.x)[r * g.C + c]);
+            df[0] = x[0] - m;
+            const float s[1] = {rs * ga}, b[1] = {a.beta ? a.beta[c] : 0.f};
+            const int at0[1] = {gc};
+            gn_dz<SILU, 1, 1>(df, x, s, b, z, a, mean, rstd, at0, c);
+            u = fmaf(ga, z[0], u);
+            v = fmaf(ga * rs * df[0], z[0], v);
+          }
+      }
       u = seg_sum(u, W);
       v = seg_sum(v, W);
       if (l == 0 && i < p.ng) {
@@ -613,7 +658,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
     k2[j] = rs * rs * g2[gi[j]] * rm;
   }
   T *dst = static_cast<T *>(a.dx) + (p.b * g.S + (long long)p.chunk * tile) * g.C;
-  constexpr bool masked = !SILU && MODE != APPLY;
+  constexpr bool masked = !SILU && MODE == SOLO;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int r = p.row + i * g.R;
@@ -634,7 +679,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
 // ---- launch ------------------------------------------------------------------------------------
 struct Plan {
   Geo g;
-  int V, NV, TH, mode;   // mode SUMS: SUMS, then APPLY
+  int V, NV, TH, mode;
   long long wgs;
 };
 
@@ -655,11 +700,7 @@ template <class D, class T, int V, int NV, bool CK, bool FOLD, bool SILU>
 void launch_mode(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(p.TH), lds, st, a); };
   if (p.mode == SOLO) go(D::template kernel<T, V, NV, SOLO, CK, FOLD, SILU>());
-  else if (p.mode == CLUSTER) go(D::template kernel<T, V, NV, CLUSTER, CK, FOLD, SILU>());
-  else {
-    go(D::template kernel<T, V, NV, SUMS, CK, FOLD, SILU>());
-    go(D::template kernel<T, V, NV, APPLY, CK, FOLD, SILU>());
-  }
+  else go(D::template kernel<T, V, NV, STAGED, CK, FOLD, SILU>());
 }
 // the plan gives NV 2, 4 (forward: 8) to full vectors of one group each, 2 to full vectors that
 // straddle groups (their constants take the registers), 4 to narrower ones

@@ -106,8 +106,7 @@ __global__ __launch_bounds__(256) void gn_wide_gsums_kernel(const BwdArgs a) {
   u = block_sum(u);
   v = block_sum(v);
   if (threadIdx.x == 0) {
-    a.part[2ll * blockIdx.x] = u;
-    a.part[2ll * blockIdx.x + 1] = v;
+    pair_store(a.part + blockIdx.x, u, v);
   }
 }
 __global__ __launch_bounds__(256) void gn_wide_dx_kernel(const BwdArgs a, int dt) {
@@ -120,8 +119,9 @@ __global__ __launch_bounds__(256) void gn_wide_dx_kernel(const BwdArgs a, int dt
     float df, al, dz;
     wide_dz(a, dt, r, c, df, al, dz);
     const long long k = r / g.S * g.G + c / g.cg;
-    const float rs = a.rstd[k];
-    store_one(a.dx, dt, i, fmaf(dz, al, -fmaf(df, rs * rs * a.part[2 * k + 1] * rm, rs * a.part[2 * k] * rm)));
+    const unsigned long long w = a.part[k];
+    const float rs = a.rstd[k], s1 = __uint_as_float((unsigned)w), s2 = __uint_as_float((unsigned)(w >> 32));
+    store_one(a.dx, dt, i, fmaf(dz, al, -fmaf(df, rs * rs * s2 * rm, rs * s1 * rm)));
   }
 }
 
@@ -145,15 +145,15 @@ __global__ __launch_bounds__(1024) void gn_dparam_kernel(const float *__restrict
   }
 }
 
-__global__ __launch_bounds__(256) void gn_zero_kernel(int *__restrict__ p, long long n) {
-  const long long i = blockIdx.x * 256ll + threadIdx.x;
-  if (i < n) p[i] = 0;
+// no pair has come yet
+__global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__restrict__ p, long long n) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += (long long)gridDim.x * 256) p[i] = kNone;
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
-constexpr int kMaxCluster = 192;   // tiles that wait for one another; at least 512 are resident
+constexpr int kLead = 2048;        // sums workgroups ahead of the use workgroups at least: all that are resident
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
-int g_wait = 1 << 20;
+int g_wait = 1 << 24;
 
 int gcd_pow2(long long c, int most) {
   int v = most;
@@ -245,22 +245,22 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   if (only) p.NV = only;
   const long long k = tiles(p.NV);
   g.k = (int)k;
-  p.mode = g.k == 1 ? SOLO : g.k <= kMaxCluster ? CLUSTER : SUMS;
-  p.wgs = B * g.nslab * k;
+  p.mode = STAGED;
+  g.lead = std::min((kLead + k - 1) / k, B * g.nslab) * k;
+  p.wgs = 2 * B * g.nslab * k;
   check(k);
   return p;
 }
 
 struct Ws {
-  long long ctr, part, dpart, lvl, total;   // offsets in floats
+  long long part, dpart, lvl, total;   // offsets in floats
 };
 long long up4(long long n) { return (n + 3) / 4 * 4; }
 Ws gn_ws(const Plan &p, bool bwd) {
   Ws w{};
   const Geo &g = p.g;
   if (p.mode != SOLO) {
-    w.part = up4(g.B * g.nslab);
-    w.dpart = w.part + up4(p.wgs * g.gs * 2);
+    w.dpart = up4(g.B * g.nslab * g.k * g.gs * 2);
   }
   w.lvl = w.dpart;
   if (bwd) {
@@ -273,18 +273,17 @@ Ws gn_ws(const Plan &p, bool bwd) {
   return w;
 }
 
-void gn_zero(const Plan &p, int *ctr, hipStream_t st) {
-  if (p.mode != CLUSTER) return;
-  const long long n = p.g.B * p.g.nslab;
-  hipLaunchKernelGGL(gn_zero_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, ctr, n);
+void gn_none(const Plan &p, unsigned long long *part, hipStream_t st) {
+  if (p.mode != STAGED) return;
+  const long long n = p.g.B * p.g.nslab * p.g.k * p.g.gs;
+  hipLaunchKernelGGL(gn_none_kernel, dim3((unsigned)std::min<long long>((n + 255) / 256, 2048)), dim3(256), 0, st, part, n);
 }
-
 }  // namespace
 
 void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M, int C, hipStream_t st);
 
-// polls of a cluster's wait (tests set 0: every workgroup then computes all sums itself)
-void gn_set_wait(int polls) { g_wait = polls < 0 ? 0 : polls; }
+// looks of a staged wait, about a microsecond each (tests: -1, what has come is not looked at)
+void gn_set_wait(int polls) { g_wait = polls; }
 
 // dt: 0 bf16, 1 fp16, 2 fp32.  Forward and backward, with and without a checkpoint: the largest.
 long long gn_workspace_floats(int dt, long long B, long long S, int C, int G, int bwd) {
@@ -298,8 +297,8 @@ void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta,
                    hipStream_t st) {
   const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, false);
   const Ws w = gn_ws(p, false);
-  const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<int *>(ws) + w.ctr, ws + w.part, eps, act};
-  gn_zero(p, a.ctr, st);
+  const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<unsigned long long *>(ws + w.part), eps, act};
+  gn_none(p, a.part, st);
   if (p.mode == WIDE) {
     const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));
     hipLaunchKernelGGL(gn_wide_stats_kernel, dim3((unsigned)p.wgs), dim3(256), 0, st, a, dt);
@@ -315,10 +314,10 @@ void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, cons
                    long long B, long long S, int C, int G, int act, hipStream_t st) {
   const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, true);
   const Ws w = gn_ws(p, true);
-  const BwdArgs a{p.g, dy, x, q, qs, gamma, beta, mean, rstd, dx, reinterpret_cast<int *>(ws) + w.ctr, ws + w.part,
+  const BwdArgs a{p.g, dy, x, q, qs, gamma, beta, mean, rstd, dx, reinterpret_cast<unsigned long long *>(ws + w.part),
                   dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act == GN_SILU, act == GN_NONE ? -INFINITY : 0.f,
                   act == GN_RELU6 ? 6.f : INFINITY};
-  gn_zero(p, a.ctr, st);
+  gn_none(p, a.part, st);
   if (p.mode == WIDE) {
     if (B * C > 0x7fffffff) throw std::invalid_argument("gn_bwd: B * C is too large");
     const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));

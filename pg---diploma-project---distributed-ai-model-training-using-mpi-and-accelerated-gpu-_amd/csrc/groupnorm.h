@@ -22,6 +22,7 @@
 #include "mx8.h"
 #include "reduce.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace gn {
@@ -39,10 +40,26 @@ template <> struct RawOf<1> { typedef uint8_t type; };
 template <class T, int V> struct Vec {
   typedef typename RawOf<V * (int)sizeof(T)>::type raw;
   struct alignas(sizeof(raw)) arr { T v[V]; };
+  // by 32-bit words: taken apart into 16-bit values, rows held over a loop cost twice the registers
   static PG_DEVICE void unpack(const raw &r, float (&f)[V]) {
-    const arr a = __builtin_bit_cast(arr, r);
+    if constexpr (sizeof(T) == 2 && V >= 2) {
+      struct alignas(sizeof(raw)) Words { uint32_t w[V / 2]; };
+      const Words a = __builtin_bit_cast(Words, r);
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = tof(a.v[j]);
+      for (int j = 0; j < V / 2; ++j) {
+        if constexpr (__is_same(T, bf16_t)) {
+          f[2 * j] = __uint_as_float(a.w[j] << 16);
+          f[2 * j + 1] = __uint_as_float(a.w[j] & 0xffff0000u);
+        } else {
+          f[2 * j] = (float)__builtin_bit_cast(_Float16, (uint16_t)a.w[j]);
+          f[2 * j + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(a.w[j] >> 16));
+        }
+      }
+    } else {
+      const arr a = __builtin_bit_cast(arr, r);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = tof(a.v[j]);
+    }
   }
   static PG_DEVICE raw pack(const float (&f)[V]) {
     if constexpr (sizeof(T) == 2 && V >= 2 && __is_same(T, bf16_t)) {
@@ -91,6 +108,7 @@ struct Geo {
   int k;        // tiles per unit, a unit being one (image, slab)
   int gs;       // groups of a full slab
   long long lead;   // tiles that sums workgroups are ahead of use workgroups: a multiple of k
+  int rows;     // rows of a tile
   int wait;     // polls after which a use workgroup takes its sums from the tensor itself
 };
 
@@ -263,158 +281,256 @@ template <int ACT> PG_DEVICE float gn_act(float z) {
   else return z;
 }
 
-template <class T, int V, int NV, int MODE, bool CK, bool FOLD>
-__global__ __launch_bounds__(1024) void gn_fwd_kernel(const FwdArgs a) {
-  extern __shared__ float sm[];
-  typedef Vec<T, V> X;
-  const Geo &g = a.g;
-  const Place p = place<V, MODE>(g);
-  float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
-  const int tile = g.R * NV;
-  constexpr int VG = FOLD ? 1 : V;
-  int gi[VG];   // slab group of each channel (FOLD: of all)
+// the checkpoint of one row's V channels; 32 channels are 32 / V neighbouring lanes (CVp is a multiple
+// of that), all of which come here
+template <class T, int V>
+PG_DEVICE void gn_checkpoint(const FwdArgs &a, const Place &p, const typename Vec<T, V>::raw &raw, long long r, bool ok) {
+  float f[V], m = 0.f;
+  Vec<T, V>::unpack(raw, f);
 #pragma unroll
-  for (int j = 0; j < VG; ++j) gi[j] = (p.c - p.c0 + j) / g.cg;
-
-  typename X::raw d[NV];
-  int nr = 0;
-  // rows past the end (and threads without a column) read a row that exists and are masked
-  auto load = [&](int chunk) {
-    const long long s0 = (long long)chunk * tile;
-    nr = (int)min((long long)tile, g.S - s0);
-    const T *src = static_cast<const T *>(a.x) + (p.b * g.S + s0) * g.C;
+  for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(f[j]));
+  m = p.on ? m : 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t r = min(p.row + i * g.R, nr - 1);
-      d[i] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
-    }
-  };
-  // mean and sum of squares about it of the tile's groups -> gm, gr
-  auto sums = [&]() {
-    float acc[V], mu[VG];
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (p.row + i * g.R < nr) {
-        float f[V];
-        X::unpack(d[i], f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) acc[j] += f[j];
-      }
-    group_sums<V, FOLD>(g, p, acc, red, gm);
-    const float rn = 1.f / ((float)nr * (float)g.cg);
-#pragma unroll
-    for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]] * rn;
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (p.row + i * g.R < nr) {
-        float f[V];
-        X::unpack(d[i], f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float df = f[j] - mu[FOLD ? 0 : j];
-          acc[j] = fmaf(df, df, acc[j]);
-        }
-      }
-    __syncthreads();   // gm and red have been read
-    if (threadIdx.x < p.ng) gm[threadIdx.x] *= rn;
-    for (int i = threadIdx.x + blockDim.x; i < p.ng; i += blockDim.x) gm[i] *= rn;
-    group_sums<V, FOLD>(g, p, acc, red, gr);
-  };
-  auto publish = [&]() {
-    unsigned long long *dst = a.part + (p.unit * g.k + p.chunk) * g.gs;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(dst + i, gm[i], gr[i]);
-  };
-
-  load(p.chunk);
-  if (CK && !p.use) {
-    // the checkpoint leaves first; 32 channels are 32 / V neighbouring lanes (CVp is a multiple of that).
-    const long long r0 = p.b * g.S + (long long)p.chunk * tile;
-    const int nb = (g.C + kMxBlock - 1) / kMxBlock;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[V], m = 0.f;
-      X::unpack(d[i], f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(f[j]));
-      m = p.on ? m : 0.f;
-#pragma unroll
-      for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-      const int r = p.row + i * g.R, e = mx8_exp(m);
-      if (p.on && r < nr) {
-        at<typename Codes<V>::raw>(a.q + r0 * g.C, (uint32_t)r * g.C + p.c) = Codes<V>::encode(f, mx8_inv_scale(e));
-        if (p.c % kMxBlock == 0) at<uint8_t>(a.qs + r0 * nb, (uint32_t)r * nb + p.c / kMxBlock) = (uint8_t)e;
-      }
-    }
+  for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const int e = mx8_exp(m);
+  if (ok) {
+    *reinterpret_cast<typename Codes<V>::raw *>(a.q + r * a.g.C + p.c) = Codes<V>::encode(f, mx8_inv_scale(e));
+    if (p.c % kMxBlock == 0) a.qs[r * ((a.g.C + kMxBlock - 1) / kMxBlock) + p.c / kMxBlock] = (uint8_t)e;
   }
-  if constexpr (MODE == SOLO) {
-    sums();
-    const float n = (float)g.S * (float)g.cg;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
-  } else {
-    if (!p.use) {
-      sums();
-      publish();
-      return;
-    }
-    // join the tiles: W lanes a group
-    const unsigned long long *src = a.part + p.unit * g.k * g.gs;
-    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-      Moments t{0.f, 0.f, 0.f};
-      const int gc = min(i, p.ng - 1);
-      if (!pairs(src + gc, g.gs, g.k, l, W, g.wait, [&](int ch, float m, float v) {
-            t.join((float)min((long long)tile, g.S - (long long)ch * tile) * (float)g.cg, m, v);
-          })) {
-        // without the peers: every W-th value of the group, from the tensor
-        const T *base = static_cast<const T *>(a.x) + p.b * g.S * g.C + p.c0 + gc * g.cg;
-        t = Moments{0.f, 0.f, 0.f};
-        for (long long r = l; r < g.S; r += W)
-          for (int c = 0; c < g.cg; ++c) t.join(1.f, tof(base[r * g.C + c]), 0.f);
-      }
-      for (int o = 1; o < W; o <<= 1) t.join(__shfl_xor(t.n, o, 64), __shfl_xor(t.m, o, 64), __shfl_xor(t.v, o, 64));
-      if (l == 0 && i < p.ng) {
-        gm[i] = t.m;
-        gr[i] = 1.f / sqrtf(t.v / t.n + a.eps);
-      }
-    }
-  }
-  __syncthreads();
-  if (p.chunk == 0)
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
-      a.mean[p.b * g.G + p.g0 + i] = gm[i];
-      a.rstd[p.b * g.G + p.g0 + i] = gr[i];
-    }
-  if (!p.on) return;
-  float mu[VG], sc[V], be[V];
+}
+
+// y of one row's V channels
+template <class T, int V, int VG, int ACT>
+PG_DEVICE typename Vec<T, V>::raw gn_y(const typename Vec<T, V>::raw &raw, const float (&mu)[VG], const float (&sc)[V],
+                                       const float (&be)[V]) {
+  float f[V];
+  Vec<T, V>::unpack(raw, f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = gn_act<ACT>(fmaf(f[j] - mu[VG == 1 ? 0 : j], sc[j], be[j]));
+  return Vec<T, V>::pack(f);
+}
+// the activation as a compile-time constant
+template <class F> PG_DEVICE void with_act(int act, F f) {
+  if (act == GN_RELU6) f(std::integral_constant<int, GN_RELU6>());
+  else if (act == GN_RELU) f(std::integral_constant<int, GN_RELU>());
+  else if (act == GN_SILU) f(std::integral_constant<int, GN_SILU>());
+  else f(std::integral_constant<int, GN_NONE>());
+}
+
+// the statistics of the slab's groups (gm: mean, gr: rstd) as this thread's channels take them
+template <int V, int VG>
+PG_DEVICE void fwd_constants(const FwdArgs &a, const Place &p, const int (&gi)[VG], const float *gm, const float *gr,
+                             float (&mu)[VG], float (&sc)[V], float (&be)[V]) {
 #pragma unroll
   for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    sc[j] = gr[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
+    sc[j] = gr[gi[VG == 1 ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
     be[j] = a.beta ? a.beta[p.c + j] : 0.f;
   }
-  T *dst = static_cast<T *>(a.y) + (p.b * g.S + (long long)p.chunk * tile) * g.C;
-  auto apply = [&](auto act) {
+}
+PG_DEVICE void fwd_statistics(const FwdArgs &a, const Place &p, const float *gm, const float *gr) {
+  if (p.chunk == 0)
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) {
+      a.mean[p.b * a.g.G + p.g0 + i] = gm[i];
+      a.rstd[p.b * a.g.G + p.g0 + i] = gr[i];
+    }
+}
+
+// solo: the rows stay in NV registers a thread between the mean, the squares about it and y
+template <class T, int V, int NV, bool CK, bool FOLD>
+__global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  const Geo &g = a.g;
+  const Place p = place<V, SOLO>(g);
+  float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
+  constexpr int VG = FOLD ? 1 : V;
+  int gi[VG];   // slab group of each channel (FOLD: of all)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int r = p.row + i * g.R;
-      if (r < nr) {
-        float f[V];
-        X::unpack(d[i], f);
+  for (int j = 0; j < VG; ++j) gi[j] = (p.c - p.c0 + j) / g.cg;
+  const int nr = (int)g.S;
+  const T *src = static_cast<const T *>(a.x) + p.b * g.S * g.C;
+  T *dst = static_cast<T *>(a.y) + p.b * g.S * g.C;
+  // rows past the end (and threads without a column) read a row that exists and are masked
+  typename X::raw d[NV];
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = gn_act<decltype(act)::value>(fmaf(f[j] - mu[FOLD ? 0 : j], sc[j], be[j]));
-        at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = X::pack(f);
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t r = min(p.row + i * g.R, nr - 1);
+    d[i] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
+  }
+  float acc[V], mu[VG], sc[V], be[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p.row + i * g.R < nr) {
+      float f[V];
+      X::unpack(d[i], f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += f[j];
+    }
+  group_sums<V, FOLD>(g, p, acc, red, gm);
+  const float n = (float)g.S * (float)g.cg;
+#pragma unroll
+  for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]] / n;
+#pragma unroll
+  for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p.row + i * g.R < nr) {
+      float f[V];
+      X::unpack(d[i], f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float df = f[j] - mu[FOLD ? 0 : j];
+        acc[j] = fmaf(df, df, acc[j]);
       }
     }
+  __syncthreads();   // gm and red have been read
+  for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gm[i] = gm[i] / n;
+  if constexpr (CK) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      gn_checkpoint<T, V>(a, p, d[i], p.b * g.S + p.row + i * g.R, p.on && p.row + i * g.R < nr);
+  }
+  group_sums<V, FOLD>(g, p, acc, red, gr);
+  for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
+  __syncthreads();
+  fwd_statistics(a, p, gm, gr);
+  if (!p.on) return;
+  fwd_constants<V, VG>(a, p, gi, gm, gr, mu, sc, be);
+  with_act(a.act, [&](auto act) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (p.row + i * g.R < nr)
+        at<typename X::raw>(dst, ((uint32_t)(p.row + i * g.R) * g.C + p.c) * (uint32_t)sizeof(T)) =
+            gn_y<T, V, VG, decltype(act)::value>(d[i], mu, sc, be);
+  });
+}
+
+// staged: a tile is streamed, U rows a thread at a time, the next U already on their way
+template <class T, int V, bool CK, bool FOLD>
+__global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  constexpr int U = 4, VG = FOLD ? 1 : V;
+  const Geo &g = a.g;
+  const Place p = place<V, STAGED>(g);
+  float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
+  int gi[VG];
+#pragma unroll
+  for (int j = 0; j < VG; ++j) gi[j] = (p.c - p.c0 + j) / g.cg;
+  const long long s0 = (long long)p.chunk * g.rows, r0 = p.b * g.S + s0;
+  const int nr = (int)min((long long)g.rows, g.S - s0), step = U * g.R;
+  const T *src = static_cast<const T *>(a.x) + r0 * g.C;
+  T *dst = static_cast<T *>(a.y) + r0 * g.C;
+  auto load = [&](typename X::raw (&d)[U], int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t r = min(base + p.row + u * g.R, nr - 1);
+      d[u] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
+    }
   };
-  if (a.act == GN_RELU6) apply(std::integral_constant<int, GN_RELU6>());
-  else if (a.act == GN_RELU) apply(std::integral_constant<int, GN_RELU>());
-  else if (a.act == GN_SILU) apply(std::integral_constant<int, GN_SILU>());
-  else apply(std::integral_constant<int, GN_NONE>());
+  typename X::raw d[U], nx[U];
+  load(d, 0);
+  auto stream = [&](auto f) {
+#pragma unroll 1
+    for (int base = 0; base < nr; base += step) {
+      if (base + step < nr) load(nx, base + step);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        f(d[u], base + p.row + u * g.R);
+        __builtin_amdgcn_sched_barrier(0);   // one row's temporaries at a time
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) d[u] = nx[u];
+    }
+  };
+  if (!p.use) {
+    // Sums of x - K and its square, K this thread's first values: nothing is lost where the mean is
+    // far from 0, and a K that lies far out spoils one thread's share at most.
+    float K[VG], s1[VG], s2[VG], f[V], acc[V];
+    X::unpack(d[0], f);
+#pragma unroll
+    for (int j = 0; j < VG; ++j) {
+      K[j] = f[j];
+      s1[j] = s2[j] = 0.f;
+    }
+    if constexpr (FOLD) {
+#pragma unroll
+      for (int j = 1; j < V; ++j) K[0] += f[j];
+      K[0] *= 1.f / V;
+    }
+    int rows = 0;
+    stream([&](const typename X::raw &raw, int r) {
+      if constexpr (CK) gn_checkpoint<T, V>(a, p, raw, r0 + r, p.on && r < nr);
+      if (r < nr) {
+        float v[V];
+        X::unpack(raw, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float df = v[j] - K[FOLD ? 0 : j];
+          s1[FOLD ? 0 : j] += df;
+          s2[FOLD ? 0 : j] = fmaf(df, df, s2[FOLD ? 0 : j]);
+        }
+        ++rows;
+      }
+    });
+    // this thread's means, then the groups' mean, then the squares about that
+    const float n = (float)(FOLD ? rows * V : rows), rn = n > 0.f ? 1.f / n : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = FOLD && j ? 0.f : fmaf(n, K[FOLD ? 0 : j], s1[FOLD ? 0 : j]);
+    group_sums<V, FOLD>(g, p, acc, red, gm);
+    const float cn = 1.f / ((float)nr * (float)g.cg);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int k = FOLD ? 0 : j;
+      const float df = fmaf(s1[k], rn, K[k]) - gm[gi[k]] * cn;
+      acc[j] = FOLD && j ? 0.f : fmaxf(fmaf(-s1[k] * rn, s1[k], s2[k]), 0.f) + n * df * df;
+      if (s1[k] != s1[k]) acc[j] = s1[k];   // fmaxf drops a NaN
+    }
+    __syncthreads();
+    group_sums<V, FOLD>(g, p, acc, red, gr);
+    unsigned long long *out = a.part + (p.unit * g.k + p.chunk) * g.gs;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + i, gm[i] * cn, gr[i]);
+    return;
+  }
+  // join the tiles: W lanes a group
+  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
+  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+    Moments t{0.f, 0.f, 0.f};
+    const int gc = min(i, p.ng - 1);
+    if (!pairs(in + gc, g.gs, g.k, l, W, g.wait, [&](int ch, float m, float v) {
+          t.join((float)min((long long)g.rows, g.S - (long long)ch * g.rows) * (float)g.cg, m, v);
+        })) {
+      // without the peers: every W-th row of the group, from the tensor
+      const T *base = static_cast<const T *>(a.x) + p.b * g.S * g.C + p.c0 + gc * g.cg;
+      t = Moments{0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (long long r = l; r < g.S; r += W)
+#pragma unroll 1
+        for (int c = 0; c < g.cg; ++c) t.join(1.f, tof(base[r * g.C + c]), 0.f);
+    }
+    for (int o = 1; o < W; o <<= 1) t.join(__shfl_xor(t.n, o, 64), __shfl_xor(t.m, o, 64), __shfl_xor(t.v, o, 64));
+    if (l == 0 && i < p.ng) {
+      gm[i] = t.m;
+      gr[i] = 1.f / sqrtf(t.v / t.n + a.eps);
+    }
+  }
+  __syncthreads();
+  fwd_statistics(a, p, gm, gr);
+  if (!p.on) return;
+  float mu[VG], sc[V], be[V];
+  fwd_constants<V, VG>(a, p, gi, gm, gr, mu, sc, be);
+  with_act(a.act, [&](auto act) {
+    stream([&](const typename X::raw &raw, int r) {
+      if (r < nr)
+        at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) =
+            gn_y<T, V, VG, decltype(act)::value>(raw, mu, sc, be);
+    });
+  });
 }
 
 // ---- backward --------------------------------------------------------------------------------
@@ -435,26 +551,25 @@ struct BwdArgs {
 // operands as they are: within fp32's rounding of a border (z takes four roundings of terms no
 // larger than |z| + |beta|) z is formed again in 64 bits, once in some 10^5 vectors.
 template <bool SILU, int V, int VG>
-PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al)[V], const float (&be)[V],
-                     float (&dy)[V], const BwdArgs &a, const float *mean, const float *rstd, const int (&gi)[VG],
-                     int c) {
+PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al)[V], const float (&be)[V], float tol,
+                     const float (&dy)[V], float (&dz)[V], const BwdArgs &a, const float *mean, const float *rstd,
+                     const int (&gi)[VG], int c) {
   if constexpr (SILU) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float z = fmaf(df[j], al[j], be[j]);
       const float s = 1.f / (1.f + __expf(-z));
-      dy[j] *= s * fmaf(z, 1.f - s, 1.f);
+      dz[j] = dy[j] * (s * fmaf(z, 1.f - s, 1.f));
     }
   } else {
-    bool near = false, out[V];
+    float near = INFINITY;   // of the distances to the borders
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float z = fmaf(df[j], al[j], be[j]);
-      out[j] = z <= a.lo || z >= a.hi;
-      const float tol = 1e-6f * fabsf(be[j]);
-      near |= fabsf(z - a.lo) <= tol || fabsf(z - a.hi) <= tol + 8e-6f;
+      dz[j] = z <= a.lo || z >= a.hi ? 0.f : dy[j];
+      near = fminf(near, fminf(fabsf(z - a.lo), fabsf(z - a.hi)));
     }
-    if (near) {
+    if (near <= tol) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         // One value at a time, its operands read again and made opaque: together, or hoisted out
@@ -462,218 +577,304 @@ PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al
         int k = gi[VG == 1 ? 0 : j], cj = c + j;
         float b = be[j], v = x[j];
         asm volatile("" : "+v"(k), "+v"(cj), "+v"(b), "+v"(v));
-        const float tol = 1e-6f * fabsf(b), z = fmaf(df[j], al[j], b);
-        if (fabsf(z - a.lo) <= tol || fabsf(z - a.hi) <= tol + 8e-6f) {
+        const float z = fmaf(df[j], al[j], b);
+        if (fminf(fabsf(z - a.lo), fabsf(z - a.hi)) <= tol) {
           const double w = ((double)v - (double)mean[k]) * (double)rstd[k] * (a.gamma ? (double)a.gamma[cj] : 1.0) +
                            (double)b;
-          out[j] = w <= (double)a.lo || w >= (double)a.hi;
+          dz[j] = w <= (double)a.lo || w >= (double)a.hi ? 0.f : dy[j];
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) dy[j] = out[j] ? 0.f : dy[j];
   }
 }
+// how near to a border fp32 cannot tell the side of any of the channels
+template <int V> PG_DEVICE float gn_tol(const float (&be)[V]) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(be[j]));
+  return fmaf(m, 1e-6f, 8e-6f);
+}
 
-template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU>
-__global__ __launch_bounds__(1024) void gn_bwd_kernel(const BwdArgs a) {
-  extern __shared__ float sm[];
+// what a thread needs of its channels, and the rows it reads
+template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
   typedef Vec<T, V> X;
-  const Geo &g = a.g;
-  const Place p = place<V, MODE>(g);
-  // sums of the slab's groups, its channels' sums, the reduction's rows
-  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
-  const int tile = g.R * NV, nb = (g.C + kMxBlock - 1) / kMxBlock;
-  const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
-  constexpr int VG = FOLD ? 1 : V;
+  static constexpr int VG = FOLD ? 1 : V;
+  struct Row {
+    typename X::raw dy;
+    typename std::conditional<CK, typename Codes<V>::raw, typename X::raw>::type x;
+    float sc;
+  };
+  const float *mean, *rstd;   // of the slab's first group
   int gi[VG];
-  float mu[VG], al[V], be[V];
+  float mu[VG], al[V], be[V], tol;
+
+  PG_DEVICE BwdThread(const BwdArgs &a, const Place &p) {
+    mean = a.mean + p.b * a.g.G + p.g0;
+    rstd = a.rstd + p.b * a.g.G + p.g0;
 #pragma unroll
-  for (int j = 0; j < VG; ++j) {
-    gi[j] = (p.c - p.c0 + j) / g.cg;
-    mu[j] = mean[gi[j]];
-  }
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    al[j] = rstd[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
-    be[j] = a.beta ? a.beta[p.c + j] : 0.f;
-  }
-  typename X::raw dy[NV];
-  typename X::raw xr[CK ? 1 : NV];
-  typename Codes<V>::raw qr[CK ? NV : 1];
-  float sc[CK ? NV : 1];
-  int nr = 0;
-  auto load = [&](int chunk) {
-    const long long s0 = (long long)chunk * tile, r0 = p.b * g.S + s0;
-    nr = (int)min((long long)tile, g.S - s0);
-    const T *src = static_cast<const T *>(a.dy) + r0 * g.C;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const uint32_t r = min(p.row + i * g.R, nr - 1), o = r * g.C + p.c;
-      dy[i] = at<typename X::raw>(src, o * (uint32_t)sizeof(T));
-      if constexpr (CK) {
-        qr[i] = at<typename Codes<V>::raw>(a.q + r0 * g.C, o);
-        sc[i] = mx8_scale(at<uint8_t>(a.qs + r0 * nb, r * nb + p.c / kMxBlock));
-      } else {
-        xr[i] = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * g.C, o * (uint32_t)sizeof(T));
-      }
+    for (int j = 0; j < VG; ++j) {
+      gi[j] = (p.c - p.c0 + j) / a.g.cg;
+      mu[j] = mean[gi[j]];
     }
-  };
-  auto input = [&](int i, float (&f)[V]) {
-    if constexpr (CK) Codes<V>::decode(qr[i], sc[i], f);
-    else X::unpack(xr[i], f);
-  };
-  // tot[c] = dgamma, tot[cs + c] = dbeta of the tile; g1, g2 = s1, s2 of its groups
-  auto sums = [&]() {
-    float s0[V], s1[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (p.row + i * g.R < nr) {
-        float f[V], df[V], dz[V];
-        input(i, f);
-        X::unpack(dy[i], dz);
-#pragma unroll
-        for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
-        gn_dz<SILU, V, VG>(df, f, al, be, dz, a, mean, rstd, gi, p.c);
-        // dz is dy or 0 (all but silu): it takes dy's place for the second use
-        if constexpr (!SILU) dy[i] = X::pack(dz);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          s1[j] = fmaf(dz[j], df[j], s1[j]);
-          s0[j] += dz[j];
-        }
-      }
-    const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (p.on) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
-      }
-      __syncthreads();
-      if (nt <= 1) {
-        for (int o = t; o < n; o += blockDim.x) {
-          float s = 0.f;
-          for (int r = 0; r < g.R; ++r) s += red[r * ld + o];
-          tot[h * g.cs + o] = h ? s : s * rstd[o / g.cg];
-        }
-      } else {   // nt stripes of rows a channel
-        const int o = t % n, st = t / n;
-        if (st < nt) {
-          float s = 0.f;
-          for (int r = st; r < g.R; r += nt) s += red[r * ld + o];
-          red2[st * n + o] = s;
-        }
-        __syncthreads();
-        if (t < n) {
-          float s = 0.f;
-          for (int i = 0; i < nt; ++i) s += red2[i * n + t];
-          tot[h * g.cs + t] = h ? s : s * rstd[t / g.cg];
-        }
-      }
-      __syncthreads();
+    for (int j = 0; j < V; ++j) {
+      al[j] = rstd[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
+      be[j] = a.beta ? a.beta[p.c + j] : 0.f;
     }
-    const int W = seg_width(g.cg), per = 64 / W, lane = t & 63, l = lane & (W - 1);
-    for (int i = (t >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-      float u = 0.f, v = 0.f;
-      if (i < p.ng)
-        for (int c = i * g.cg + l; c < (i + 1) * g.cg; c += W) {
-          const float ga = a.gamma ? a.gamma[p.c0 + c] : 1.f;
-          u = fmaf(ga, tot[g.cs + c], u);
-          v = fmaf(ga, tot[c], v);
-        }
-      u = seg_sum(u, W);
-      v = seg_sum(v, W);
-      if (l == 0 && i < p.ng) {
-        g1[i] = u;
-        g2[i] = v;
-      }
+    tol = gn_tol(be);
+  }
+  // row r of the tile that begins at row r0 of the tensor
+  static PG_DEVICE void load(const BwdArgs &a, const Place &p, long long r0, uint32_t r, Row &d) {
+    const uint32_t o = r * a.g.C + p.c;
+    const int nb = (a.g.C + kMxBlock - 1) / kMxBlock;
+    d.dy = at<typename X::raw>(static_cast<const T *>(a.dy) + r0 * a.g.C, o * (uint32_t)sizeof(T));
+    if constexpr (CK) {
+      d.x = at<typename Codes<V>::raw>(a.q + r0 * a.g.C, o);
+      d.sc = mx8_scale(at<uint8_t>(a.qs + r0 * nb, r * nb + p.c / kMxBlock));
+    } else {
+      d.x = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * a.g.C, o * (uint32_t)sizeof(T));
+    }
+  }
+  // x - mean and dz of a row
+  template <bool DONE> PG_DEVICE void row(const BwdArgs &a, const Place &p, const Row &d, float (&df)[V], float (&dz)[V]) const {
+    float f[V];
+    if constexpr (CK) Codes<V>::decode(d.x, d.sc, f);
+    else X::unpack(d.x, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
+    if constexpr (DONE) {
+      X::unpack(d.dy, dz);
+    } else {
+      float dy[V];
+      X::unpack(d.dy, dy);
+      gn_dz<SILU, V, VG>(df, f, al, be, tol, dy, dz, a, mean, rstd, gi, p.c);
+    }
+  }
+};
+
+// s1 = sum dz (x - mean), s0 = sum dz of the thread -> tot[c] = dgamma, tot[cs + c] = dbeta of the
+// tile (and to dpart), g1, g2 = s1, s2 of its groups
+template <int V>
+PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, const float (&s1)[V], const float (&s0)[V],
+                        float *g1, float *g2, float *tot, float *red2, float *red) {
+  const Geo &g = a.g;
+  const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (p.on) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
     }
     __syncthreads();
-  };
-  auto publish = [&]() {
-    unsigned long long *dst = a.part + (p.unit * g.k + p.chunk) * g.gs;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(dst + i, g1[i], g2[i]);
-  };
-  load(p.chunk);
-  if (MODE == SOLO || !p.use) {
-    sums();
-    if (a.dpart) {
-      float *dst = a.dpart + (p.b * g.k + p.chunk) * 2 * g.C + p.c0;
-      for (int j = threadIdx.x; j < p.csl; j += blockDim.x) {
-        dst[j] = tot[j];
-        dst[g.C + j] = tot[g.cs + j];
+    if (nt <= 1) {
+      for (int o = t; o < n; o += blockDim.x) {
+        float s = 0.f;
+        for (int r = 0; r < g.R; ++r) s += red[r * ld + o];
+        tot[h * g.cs + o] = h ? s : s * rstd[o / g.cg];
       }
-    }
-    if constexpr (MODE == STAGED) {
-      publish();
-      return;
-    }
-  }
-  if constexpr (MODE != SOLO) {
-    const unsigned long long *src = a.part + p.unit * g.k * g.gs;
-    const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-    for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-      float u = 0.f, v = 0.f;
-      const int gc = min(i, p.ng - 1);
-      if (!pairs(src + gc, g.gs, g.k, l, W, g.wait, [&](int, float s1, float s2) {
-            u += s1;
-            v += s2;
-          })) {   // as in the forward
-        u = v = 0.f;
-        const float m = mean[gc], rs = rstd[gc];
-        for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
-          for (int c = p.c0 + gc * g.cg; c < p.c0 + (gc + 1) * g.cg; ++c) {
-            const float ga = a.gamma ? a.gamma[c] : 1.f;
-            float x[1], df[1], z[1] = {tof(static_cast<const T *>(a.dy)[r * g.C + c])};
-            if constexpr (CK) x[0] = mx8_dec1(a.q[r * g.C + c]) * mx8_scale(a.qs[r * nb + c / kMxBlock]);
-            else x[0] = tof(static_cast<const T *>(a.x)[r * g.C + c]);
-            df[0] = x[0] - m;
-            const float s[1] = {rs * ga}, b[1] = {a.beta ? a.beta[c] : 0.f};
-            const int at0[1] = {gc};
-            gn_dz<SILU, 1, 1>(df, x, s, b, z, a, mean, rstd, at0, c);
-            u = fmaf(ga, z[0], u);
-            v = fmaf(ga * rs * df[0], z[0], v);
-          }
+    } else {   // nt stripes of rows a channel
+      const int o = t % n, st = t / n;
+      if (st < nt) {
+        float s = 0.f;
+        for (int r = st; r < g.R; r += nt) s += red[r * ld + o];
+        red2[st * n + o] = s;
       }
-      u = seg_sum(u, W);
-      v = seg_sum(v, W);
-      if (l == 0 && i < p.ng) {
-        g1[i] = u;
-        g2[i] = v;
+      __syncthreads();
+      if (t < n) {
+        float s = 0.f;
+        for (int i = 0; i < nt; ++i) s += red2[i * n + t];
+        tot[h * g.cs + t] = h ? s : s * rstd[t / g.cg];
       }
     }
     __syncthreads();
   }
-  if (!p.on) return;
-  // dx = dz al - (k1 + (x - mean) k2)
+  if (a.dpart) {
+    float *dst = a.dpart + (p.b * g.k + p.chunk) * 2 * g.C + p.c0;
+    for (int j = t; j < n; j += blockDim.x) {
+      dst[j] = tot[j];
+      dst[g.C + j] = tot[g.cs + j];
+    }
+  }
+  const int W = seg_width(g.cg), per = 64 / W, lane = t & 63, l = lane & (W - 1);
+  for (int i = (t >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+    float u = 0.f, v = 0.f;
+    if (i < p.ng)
+      for (int c = i * g.cg + l; c < (i + 1) * g.cg; c += W) {
+        const float ga = a.gamma ? a.gamma[p.c0 + c] : 1.f;
+        u = fmaf(ga, tot[g.cs + c], u);
+        v = fmaf(ga, tot[c], v);
+      }
+    u = seg_sum(u, W);
+    v = seg_sum(v, W);
+    if (l == 0 && i < p.ng) {
+      g1[i] = u;
+      g2[i] = v;
+    }
+  }
+  __syncthreads();
+}
+
+// dx = dz al - (k1 + (x - mean) k2)
+template <class T, int V, int VG>
+PG_DEVICE typename Vec<T, V>::raw gn_dx(const float (&df)[V], const float (&dz)[V], const float (&al)[V],
+                                        const float (&k1)[VG], const float (&k2)[VG]) {
+  float f[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = fmaf(dz[j], al[j], -fmaf(df[j], k2[VG == 1 ? 0 : j], k1[VG == 1 ? 0 : j]));
+  return Vec<T, V>::pack(f);
+}
+template <int VG>
+PG_DEVICE void bwd_constants(const Geo &g, const float *rstd, const int (&gi)[VG], const float *g1, const float *g2,
+                             float (&k1)[VG], float (&k2)[VG]) {
   const float rm = 1.f / ((float)g.S * (float)g.cg);
-  float k1[VG], k2[VG];
 #pragma unroll
   for (int j = 0; j < VG; ++j) {
     const float rs = rstd[gi[j]];
     k1[j] = rs * g1[gi[j]] * rm;
     k2[j] = rs * rs * g2[gi[j]] * rm;
   }
-  T *dst = static_cast<T *>(a.dx) + (p.b * g.S + (long long)p.chunk * tile) * g.C;
-  constexpr bool masked = !SILU && MODE == SOLO;
+}
+
+template <class T, int V, int NV, bool CK, bool FOLD, bool SILU>
+__global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  typedef BwdThread<T, V, CK, FOLD, SILU> Th;
+  const Geo &g = a.g;
+  const Place p = place<V, SOLO>(g);
+  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
+  const int nr = (int)g.S;
+  const long long r0 = p.b * g.S;
+  typename Th::Row d[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) Th::load(a, p, r0, min(p.row + i * g.R, nr - 1), d[i]);
+  const Th th(a, p);
+  float s0[V], s1[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p.row + i * g.R < nr) {
+      float df[V], dz[V];
+      th.template row<false>(a, p, d[i], df, dz);
+      if constexpr (!SILU) d[i].dy = X::pack(dz);   // dy or 0: it takes dy's place for the second use
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s1[j] = fmaf(dz[j], df[j], s1[j]);
+        s0[j] += dz[j];
+      }
+    }
+  bwd_sums<V>(a, p, th.rstd, s1, s0, g1, g2, tot, red2, red);
+  if (!p.on) return;
+  float k1[Th::VG], k2[Th::VG];
+  bwd_constants<Th::VG>(g, th.rstd, th.gi, g1, g2, k1, k2);
+  T *dst = static_cast<T *>(a.dx) + r0 * g.C;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int r = p.row + i * g.R;
     if (r < nr) {
-      float f[V], df[V], dz[V];
-      input(i, f);
-      X::unpack(dy[i], dz);
-#pragma unroll
-      for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
-      if constexpr (!masked) gn_dz<SILU, V, VG>(df, f, al, be, dz, a, mean, rstd, gi, p.c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = fmaf(dz[j], al[j], -fmaf(df[j], k2[FOLD ? 0 : j], k1[FOLD ? 0 : j]));
-      *reinterpret_cast<typename X::raw *>(dst + (size_t)(uint32_t)r * (uint32_t)g.C + p.c) = X::pack(f);
+      float df[V], dz[V];
+      th.template row<!SILU>(a, p, d[i], df, dz);
+      at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
     }
   }
+}
+
+template <class T, int V, bool CK, bool FOLD, bool SILU>
+__global__ __launch_bounds__(512, 4) void gn_bwd_staged_kernel(const BwdArgs a) {
+  extern __shared__ float sm[];
+  typedef Vec<T, V> X;
+  typedef BwdThread<T, V, CK, FOLD, SILU> Th;
+  constexpr int U = 2;
+  const Geo &g = a.g;
+  const Place p = place<V, STAGED>(g);
+  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
+  const long long s0 = (long long)p.chunk * g.rows, r0 = p.b * g.S + s0;
+  const int nr = (int)min((long long)g.rows, g.S - s0), step = U * g.R;
+  auto load = [&](typename Th::Row (&d)[U], int base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) Th::load(a, p, r0, min(base + p.row + u * g.R, nr - 1), d[u]);
+  };
+  typename Th::Row d[U], nx[U];
+  load(d, 0);
+  const Th th(a, p);
+  auto stream = [&](auto f) {
+#pragma unroll 1
+    for (int base = 0; base < nr; base += step) {
+      if (base + step < nr) load(nx, base + step);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = base + p.row + u * g.R;
+        if (r < nr) {
+          float df[V], dz[V];
+          th.template row<false>(a, p, d[u], df, dz);
+          f(df, dz, r);
+        }
+        __builtin_amdgcn_sched_barrier(0);   // one row's temporaries at a time
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) d[u] = nx[u];
+    }
+  };
+  if (!p.use) {
+    float s0[V], s1[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+    stream([&](const float (&df)[V], const float (&dz)[V], int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        s1[j] = fmaf(dz[j], df[j], s1[j]);
+        s0[j] += dz[j];
+      }
+    });
+    bwd_sums<V>(a, p, th.rstd, s1, s0, g1, g2, tot, red2, red);
+    unsigned long long *out = a.part + (p.unit * g.k + p.chunk) * g.gs;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + i, g1[i], g2[i]);
+    return;
+  }
+  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
+  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+    float u = 0.f, v = 0.f;
+    const int gc = min(i, p.ng - 1);
+    if (!pairs(in + gc, g.gs, g.k, l, W, g.wait, [&](int, float s1, float s2) {
+          u += s1;
+          v += s2;
+        })) {   // as in the forward
+      u = v = 0.f;
+      const int nb = (g.C + kMxBlock - 1) / kMxBlock, at0[1] = {gc};
+      const float m = th.mean[gc], rs = th.rstd[gc];
+#pragma unroll 1
+      for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
+#pragma unroll 1
+        for (int c = p.c0 + gc * g.cg; c < p.c0 + (gc + 1) * g.cg; ++c) {
+          const float ga = a.gamma ? a.gamma[c] : 1.f;
+          float x[1], df[1], z[1];
+          const float dy[1] = {tof(static_cast<const T *>(a.dy)[r * g.C + c])};
+          if constexpr (CK) x[0] = mx8_dec1(a.q[r * g.C + c]) * mx8_scale(a.qs[r * nb + c / kMxBlock]);
+          else x[0] = tof(static_cast<const T *>(a.x)[r * g.C + c]);
+          df[0] = x[0] - m;
+          const float s[1] = {rs * ga}, b[1] = {a.beta ? a.beta[c] : 0.f};
+          gn_dz<SILU, 1, 1>(df, x, s, b, gn_tol(b), dy, z, a, th.mean, th.rstd, at0, c);
+          u = fmaf(ga, z[0], u);
+          v = fmaf(ga * rs * df[0], z[0], v);
+        }
+    }
+    u = seg_sum(u, W);
+    v = seg_sum(v, W);
+    if (l == 0 && i < p.ng) {
+      g1[i] = u;
+      g2[i] = v;
+    }
+  }
+  __syncthreads();
+  if (!p.on) return;
+  float k1[Th::VG], k2[Th::VG];
+  bwd_constants<Th::VG>(g, th.rstd, th.gi, g1, g2, k1, k2);
+  T *dst = static_cast<T *>(a.dx) + r0 * g.C;
+  stream([&](const float (&df)[V], const float (&dz)[V], int r) {
+    at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
+  });
 }
 
 // ---- launch ------------------------------------------------------------------------------------
@@ -685,35 +886,44 @@ struct Plan {
 
 struct Fwd {
   typedef FwdArgs Args;
-  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto kernel() {
-    return gn_fwd_kernel<T, V, NV, MODE, CK, FOLD>;
+  template <class T, int V, int NV, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
+    return gn_fwd_solo_kernel<T, V, NV, CK, FOLD>;
+  }
+  template <class T, int V, bool CK, bool FOLD, bool SILU> static constexpr auto staged() {
+    return gn_fwd_staged_kernel<T, V, CK, FOLD>;
   }
 };
 struct Bwd {
   typedef BwdArgs Args;
-  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto kernel() {
-    return gn_bwd_kernel<T, V, NV, MODE, CK, FOLD, SILU>;
+  template <class T, int V, int NV, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
+    return gn_bwd_solo_kernel<T, V, NV, CK, FOLD, SILU>;
+  }
+  template <class T, int V, bool CK, bool FOLD, bool SILU> static constexpr auto staged() {
+    return gn_bwd_staged_kernel<T, V, CK, FOLD, SILU>;
   }
 };
 
-template <class D, class T, int V, int NV, bool CK, bool FOLD, bool SILU>
-void launch_mode(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(p.TH), lds, st, a); };
-  if (p.mode == SOLO) go(D::template kernel<T, V, NV, SOLO, CK, FOLD, SILU>());
-  else go(D::template kernel<T, V, NV, STAGED, CK, FOLD, SILU>());
-}
 // the plan gives NV 2, 4 (forward: 8) to full vectors of one group each, 2 to full vectors that
 // straddle groups (their constants take the registers), 4 to narrower ones
 template <class D, class T, int VMAX, int MOST, bool CK, bool SILU>
 void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
-  if (p.V == VMAX && p.g.cg % VMAX == 0) {
-    if (p.NV == 2) launch_mode<D, T, VMAX, 2, CK, true, SILU>(p, lds, a, st);
-    else if (MOST == 4 || p.NV == 4) launch_mode<D, T, VMAX, 4, CK, true, SILU>(p, lds, a, st);
-    else launch_mode<D, T, VMAX, MOST, CK, true, SILU>(p, lds, a, st);
-  } else if (p.V == VMAX) launch_mode<D, T, VMAX, 2, CK, false, SILU>(p, lds, a, st);
-  else if (VMAX == 8 && p.V == 4) launch_mode<D, T, 4, 4, CK, false, SILU>(p, lds, a, st);
-  else if (p.V == 2) launch_mode<D, T, 2, 4, CK, false, SILU>(p, lds, a, st);
-  else launch_mode<D, T, 1, 4, CK, false, SILU>(p, lds, a, st);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(p.TH), lds, st, a); };
+  const bool full = p.V == VMAX, fold = full && p.g.cg % VMAX == 0;
+  if (p.mode == STAGED) {
+    if (fold) go(D::template staged<T, VMAX, CK, true, SILU>());
+    else if (full) go(D::template staged<T, VMAX, CK, false, SILU>());
+    else if (VMAX == 8 && p.V == 4) go(D::template staged<T, 4, CK, false, SILU>());
+    else if (p.V == 2) go(D::template staged<T, 2, CK, false, SILU>());
+    else go(D::template staged<T, 1, CK, false, SILU>());
+    return;
+  }
+  if (fold && p.NV == 2) go(D::template solo<T, VMAX, 2, CK, true, SILU>());
+  else if (fold && p.NV == 4) go(D::template solo<T, VMAX, 4, CK, true, SILU>());
+  else if (fold) go(D::template solo<T, VMAX, MOST, CK, true, SILU>());
+  else if (full) go(D::template solo<T, VMAX, 2, CK, false, SILU>());
+  else if (VMAX == 8 && p.V == 4) go(D::template solo<T, 4, 4, CK, false, SILU>());
+  else if (p.V == 2) go(D::template solo<T, 2, 4, CK, false, SILU>());
+  else go(D::template solo<T, 1, 4, CK, false, SILU>());
 }
 
 // one translation unit per direction and type

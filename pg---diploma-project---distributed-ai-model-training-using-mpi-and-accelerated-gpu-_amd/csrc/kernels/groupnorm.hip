@@ -67,9 +67,10 @@ PG_DEVICE void wide_dz(const BwdArgs &a, int dt, long long r, int c, float &df, 
   const float x[1] = {a.q ? mx8_dec1(a.q[i]) * mx8_scale(a.qs[r * nb + c / kMxBlock]) : load_one(a.x, dt, i)};
   const float d[1] = {x[0] - a.mean[k]}, s[1] = {a.rstd[k] * (a.gamma ? a.gamma[c] : 1.f)};
   const float b[1] = {a.beta ? a.beta[c] : 0.f};
-  float v[1] = {load_one(a.dy, dt, i)};
-  if (a.silu) gn_dz<true, 1, 1>(d, x, s, b, v, a, a.mean + k, a.rstd + k, gi, c);
-  else gn_dz<false, 1, 1>(d, x, s, b, v, a, a.mean + k, a.rstd + k, gi, c);
+  const float y[1] = {load_one(a.dy, dt, i)};
+  float v[1];
+  if (a.silu) gn_dz<true, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
+  else gn_dz<false, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
   df = d[0];
   al = s[0];
   dz = v[0];
@@ -151,7 +152,8 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
-constexpr int kLead = 2048;        // sums workgroups ahead of the use workgroups at least: all that are resident
+constexpr int kTiles = 2048;       // tiles wanted before tiles grow
+constexpr int kLead = 1024;        // sums workgroups ahead of the use workgroups at least: all that are resident
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
 int g_wait = 1 << 24;
 
@@ -192,7 +194,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     g.CVp = (g.cs / V + Q - 1) / Q * Q;
   };
   auto check = [&](long long k) {   // grid and in-tile offsets
-    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)g.R * p.NV * C * elt > 0x7fffffff)
+    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)std::max(g.rows, g.R * p.NV) * C * elt > 0x7fffffff)
       throw std::invalid_argument("group norm: sizes past the kernels' 32-bit grid and tile offsets");
   };
   const int most = bwd ? 512 : 1024;
@@ -222,14 +224,13 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     }
   }
   // whole rows where they fit a workgroup, the fewest slabs otherwise
-  long long slabs = 1;
-  for (;; ++slabs) {
+  p.TH = 512;
+  for (long long slabs = 1;; ++slabs) {
     cs = ((C + slabs - 1) / slabs + L - 1) / L * L;
     shape(cs);
-    if (g.CVp <= (bwd ? 512 : 1024) || cs == L) break;
+    if (g.CVp <= p.TH || cs == L) break;
   }
-  p.TH = std::max(512, (g.CVp + 63) / 64 * 64);
-  if (g.CVp > 1024 || gn_lds(p, bwd) > 65536) {
+  if (g.CVp > p.TH || gn_lds(p, bwd) > 65536) {
     p.mode = WIDE;
     g.k = 1;
     g.nslab = G;   // sums per (image, group)
@@ -238,12 +239,12 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     return p;
   }
   g.R = p.TH / g.CVp;
-  // fewer rows a tile while the tiles do not fill the chip
-  p.NV = nv_most;
-  auto tiles = [&](int nv) { return (S + (long long)g.R * nv - 1) / ((long long)g.R * nv); };
-  while (p.NV > 2 && B * g.nslab * tiles(p.NV) < 512) p.NV /= 2;
-  if (only) p.NV = only;
-  const long long k = tiles(p.NV);
+  // tiles of up to 8 rounds, fewer while the tiles do not fill the chip several times
+  const long long round = (long long)g.R * (bwd ? 2 : 4), all = (S + round - 1) / round;
+  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, 8);
+  const long long k = (all + it - 1) / it;
+  p.NV = 1;
+  g.rows = (int)(round * it);
   g.k = (int)k;
   p.mode = STAGED;
   g.lead = std::min((kLead + k - 1) / k, B * g.nslab) * k;

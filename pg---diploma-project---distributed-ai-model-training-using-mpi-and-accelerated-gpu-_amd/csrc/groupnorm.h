@@ -107,7 +107,8 @@ struct Geo {
   int R;        // tile rows per sweep: blockDim / CVp
   int k;        // tiles per unit, a unit being one (image, slab)
   int gs;       // groups of a full slab
-  long long lead;   // tiles that sums workgroups are ahead of use workgroups: a multiple of k
+  int tiles;    // of all units
+  int lead;     // tiles that sums workgroups are ahead of use workgroups: a multiple of k
   int rows;     // rows of a tile
   int wait;     // polls after which a use workgroup takes its sums from the tensor itself
 };
@@ -128,30 +129,31 @@ struct Place {
 // another, the wait is bounded and the work is done without the peers.)
 template <int V, int MODE> PG_DEVICE Place place(const Geo &g) {
   Place p;
-  long long id = blockIdx.x;
+  uint32_t id = blockIdx.x;   // the grid is below 2^31
   p.use = false;
   if constexpr (MODE == STAGED) {
-    const long long both = g.B * g.nslab * g.k - g.lead, even = both & ~7ll;
-    if (id >= g.lead) {
-      id -= g.lead;
+    const uint32_t lead = g.lead, both = g.tiles - lead, even = both & ~7u;
+    if (id >= lead) {
+      id -= lead;
       if (id < 2 * even) {
         p.use = (id >> 3) & 1;
         id = (id >> 4) * 8 + (id & 7);
       } else if (id < 2 * both) {
-        const int r = (int)(id - 2 * even), rest = (int)(both - even);
+        const uint32_t r = id - 2 * even, rest = both - even;
         p.use = r >= rest;
         id = even + (p.use ? r - rest : r);
       } else {
         p.use = true;
         id -= both;
       }
-      if (!p.use) id += g.lead;
+      if (!p.use) id += lead;
     }
   }
-  p.chunk = (int)(id % g.k);
-  p.unit = id / g.k;
-  const int slab = (int)(p.unit % g.nslab);
-  p.b = p.unit / g.nslab;
+  const uint32_t unit = id / (uint32_t)g.k;
+  p.chunk = id - unit * g.k;
+  p.unit = unit;
+  p.b = unit / (uint32_t)g.nslab;
+  const int slab = unit - (uint32_t)p.b * g.nslab;
   p.c0 = slab * g.cs;
   p.csl = min(g.cs, g.C - p.c0);
   p.ng = p.csl / g.cg;
@@ -223,22 +225,25 @@ PG_DEVICE void pair_store(unsigned long long *p, float a, float b) {
 PG_DEVICE unsigned long long pair_load(const unsigned long long *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// the lane's pairs (tiles l, l + W, ..) of a group, in order; false: one of the wave's did not come
-template <class F> PG_DEVICE bool pairs(const unsigned long long *src, int gs, int k, int l, int W, int polls, F f) {
+// The lane's pairs (tiles l, l + W, ..) of a group, in order; false: one of the wave's did not come.
+// v: the first four, asked for by pairs_ahead when the workgroup began.
+PG_DEVICE void pairs_ahead(const unsigned long long *src, int k, int l, int W, int c0, unsigned long long (&v)[4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int ch = c0 + u * W + l;
+    v[u] = pair_load(src + (ch < k ? ch : l < k ? l : 0));
+  }
+}
+template <class F>
+PG_DEVICE bool pairs(const unsigned long long *src, int k, int l, int W, int polls, unsigned long long (&v)[4], F f) {
   if (polls < 0) return false;
   for (int c0 = 0; c0 < k; c0 += 4 * W) {   // four loads in flight
-    unsigned long long v[4];
+    if (c0) pairs_ahead(src, k, l, W, c0, v);
     for (int i = 0;; ++i) {
-      bool none = false;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int ch = c0 + u * W + l;
-        v[u] = pair_load(src + (long long)(ch < k ? ch : l < k ? l : 0) * gs);
-        none |= v[u] == kNone;
-      }
-      if (!__any(none)) break;
+      if (!__any(v[0] == kNone || v[1] == kNone || v[2] == kNone || v[3] == kNone)) break;
       if (i >= polls) return false;
       __builtin_amdgcn_s_sleep(4);
+      pairs_ahead(src, k, l, W, c0, v);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -268,7 +273,7 @@ struct FwdArgs {
   void *y;
   float *mean, *rstd;
   uint8_t *q, *qs;
-  unsigned long long *part;   // [B * nslab][k][gs]: mean and sum of squares about it of every tile and group
+  unsigned long long *part;   // [B * nslab][gs][k]: mean and sum of squares about it of every tile and group
   float eps;
   int act;
 };
@@ -425,26 +430,35 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
   const int nr = (int)min((long long)g.rows, g.S - s0), step = U * g.R;
   const T *src = static_cast<const T *>(a.x) + r0 * g.C;
   T *dst = static_cast<T *>(a.y) + r0 * g.C;
-  auto load = [&](typename X::raw (&d)[U], int base) {
+  // byte offsets of this thread's rows; past the tile's end, the last row's
+  const uint32_t last = ((uint32_t)(nr - 1) * g.C + p.c) * (uint32_t)sizeof(T), hop = (uint32_t)g.R * g.C * (uint32_t)sizeof(T);
+  const uint32_t first = ((uint32_t)p.row * g.C + p.c) * (uint32_t)sizeof(T);
+  auto load = [&](typename X::raw (&d)[U], int round) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t r = min(base + p.row + u * g.R, nr - 1);
-      d[u] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
-    }
+    for (int u = 0; u < U; ++u) d[u] = at<typename X::raw>(src, min(first + (round * U + u) * hop, last));
   };
+  // where the tiles are joined: W lanes a group, the first group's pairs on their way
+  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
+  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  const int i0 = (threadIdx.x >> 6) * per + lane / W;
+  unsigned long long pv[4];
+  if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
   typename X::raw d[U], nx[U];
   load(d, 0);
   auto stream = [&](auto f) {
+    const int rounds = (nr + step - 1) / step;
+    auto work = [&](const typename X::raw (&v)[U], int round) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(v[u], p.row + (round * U + u) * g.R, first + (round * U + u) * hop);
+    };
 #pragma unroll 1
-    for (int base = 0; base < nr; base += step) {
-      if (base + step < nr) load(nx, base + step);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        f(d[u], base + p.row + u * g.R);
-        __builtin_amdgcn_sched_barrier(0);   // one row's temporaries at a time
+    for (int i = 0; i < rounds; i += 2) {
+      if (i + 1 < rounds) load(nx, i + 1);
+      work(d, i);
+      if (i + 1 < rounds) {
+        if (i + 2 < rounds) load(d, i + 2);
+        work(nx, i + 1);
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) d[u] = nx[u];
     }
   };
   if (!p.use) {
@@ -463,7 +477,7 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
       K[0] *= 1.f / V;
     }
     int rows = 0;
-    stream([&](const typename X::raw &raw, int r) {
+    stream([&](const typename X::raw &raw, int r, uint32_t) {
       if constexpr (CK) gn_checkpoint<T, V>(a, p, raw, r0 + r, p.on && r < nr);
       if (r < nr) {
         float v[V];
@@ -492,17 +506,15 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
     }
     __syncthreads();
     group_sums<V, FOLD>(g, p, acc, red, gr);
-    unsigned long long *out = a.part + (p.unit * g.k + p.chunk) * g.gs;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + i, gm[i] * cn, gr[i]);
+    unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, gm[i] * cn, gr[i]);
     return;
   }
-  // join the tiles: W lanes a group
-  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-  for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+  for (int i = i0; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
     Moments t{0.f, 0.f, 0.f};
     const int gc = min(i, p.ng - 1);
-    if (!pairs(in + gc, g.gs, g.k, l, W, g.wait, [&](int ch, float m, float v) {
+    if (i != i0) pairs_ahead(in + (long long)gc * g.k, g.k, l, W, 0, pv);
+    if (!pairs(in + (long long)gc * g.k, g.k, l, W, g.wait, pv, [&](int ch, float m, float v) {
           t.join((float)min((long long)g.rows, g.S - (long long)ch * g.rows) * (float)g.cg, m, v);
         })) {
       // without the peers: every W-th row of the group, from the tensor
@@ -525,9 +537,9 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
   float mu[VG], sc[V], be[V];
   fwd_constants<V, VG>(a, p, gi, gm, gr, mu, sc, be);
   with_act(a.act, [&](auto act) {
-    stream([&](const typename X::raw &raw, int r) {
+    stream([&](const typename X::raw &raw, int r, uint32_t off) {
       if (r < nr)
-        at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) =
+        at<typename X::raw>(dst, off) =
             gn_y<T, V, VG, decltype(act)::value>(raw, mu, sc, be);
     });
   });
@@ -540,15 +552,13 @@ struct BwdArgs {
   const uint8_t *q, *qs;
   const float *gamma, *beta, *mean, *rstd;
   void *dx;
-  unsigned long long *part;   // [B * nslab][k][gs]: s1, s2 of every tile and group
+  unsigned long long *part;   // [B * nslab][gs][k]: s1, s2 of every tile and group
   float *dpart;   // [B * k][2][C]: dgamma, dbeta of every tile, or null
-  int silu;
-  float lo, hi;   // the other activations' borders
+  int act;
 };
 
-// act'(z) dy of V channels (df = x - mean).  SILU, or dy where lo < z < hi and 0 elsewhere: none is
-// (-inf, inf), relu (0, inf), relu6 (0, 6).  Which side of a border z lies on is decided from the
-// operands as they are: within fp32's rounding of a border (z takes four roundings of terms no
+// act'(z) dy of V channels (df = x - mean).  Which side of relu's or relu6's border z lies on is
+// decided from the operands as they are: within fp32's rounding of a border (z takes four roundings of terms no
 // larger than |z| + |beta|) z is formed again in 64 bits, once in some 10^5 vectors.
 template <bool SILU, int V, int VG>
 PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al)[V], const float (&be)[V], float tol,
@@ -563,11 +573,23 @@ PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al
     }
   } else {
     float near = INFINITY;   // of the distances to the borders
+    if (a.act == GN_RELU6) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float z = fmaf(df[j], al[j], be[j]);
-      dz[j] = z <= a.lo || z >= a.hi ? 0.f : dy[j];
-      near = fminf(near, fminf(fabsf(z - a.lo), fabsf(z - a.hi)));
+      for (int j = 0; j < V; ++j) {
+        const float v = fabsf(fmaf(df[j], al[j], be[j]) - 3.f) - 3.f;   // below 0 between the borders
+        dz[j] = v < 0.f ? dy[j] : 0.f;
+        near = fminf(near, fabsf(v));
+      }
+    } else if (a.act == GN_RELU) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float z = fmaf(df[j], al[j], be[j]);
+        dz[j] = z > 0.f ? dy[j] : 0.f;
+        near = fminf(near, fabsf(z));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) dz[j] = dy[j];
     }
     if (near <= tol) {
 #pragma unroll
@@ -578,10 +600,10 @@ PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al
         float b = be[j], v = x[j];
         asm volatile("" : "+v"(k), "+v"(cj), "+v"(b), "+v"(v));
         const float z = fmaf(df[j], al[j], b);
-        if (fminf(fabsf(z - a.lo), fabsf(z - a.hi)) <= tol) {
+        if (fabsf(z) <= tol || fabsf(z - 6.f) <= tol) {
           const double w = ((double)v - (double)mean[k]) * (double)rstd[k] * (a.gamma ? (double)a.gamma[cj] : 1.0) +
                            (double)b;
-          dz[j] = w <= (double)a.lo || w >= (double)a.hi ? 0.f : dy[j];
+          dz[j] = w > 0.0 && (a.act == GN_RELU || w < 6.0) ? dy[j] : 0.f;
         }
       }
     }
@@ -602,11 +624,11 @@ template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
   struct Row {
     typename X::raw dy;
     typename std::conditional<CK, typename Codes<V>::raw, typename X::raw>::type x;
-    float sc;
+    uint8_t sc;   // checkpoint: the scale's byte
   };
   const float *mean, *rstd;   // of the slab's first group
   int gi[VG];
-  float mu[VG], al[V], be[V], tol;
+  float mu[VG], rs[VG], al[V], be[V], tol;
 
   PG_DEVICE BwdThread(const BwdArgs &a, const Place &p) {
     mean = a.mean + p.b * a.g.G + p.g0;
@@ -615,22 +637,22 @@ template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
     for (int j = 0; j < VG; ++j) {
       gi[j] = (p.c - p.c0 + j) / a.g.cg;
       mu[j] = mean[gi[j]];
+      rs[j] = rstd[gi[j]];
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      al[j] = rstd[gi[FOLD ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
+      al[j] = rs[FOLD ? 0 : j] * (a.gamma ? a.gamma[p.c + j] : 1.f);
       be[j] = a.beta ? a.beta[p.c + j] : 0.f;
     }
     tol = gn_tol(be);
   }
-  // row r of the tile that begins at row r0 of the tensor
-  static PG_DEVICE void load(const BwdArgs &a, const Place &p, long long r0, uint32_t r, Row &d) {
-    const uint32_t o = r * a.g.C + p.c;
+  // the row at element offset o (and scale offset os) of the tile that begins at row r0 of the tensor
+  static PG_DEVICE void load(const BwdArgs &a, long long r0, uint32_t o, uint32_t os, Row &d) {
     const int nb = (a.g.C + kMxBlock - 1) / kMxBlock;
     d.dy = at<typename X::raw>(static_cast<const T *>(a.dy) + r0 * a.g.C, o * (uint32_t)sizeof(T));
     if constexpr (CK) {
       d.x = at<typename Codes<V>::raw>(a.q + r0 * a.g.C, o);
-      d.sc = mx8_scale(at<uint8_t>(a.qs + r0 * nb, r * nb + p.c / kMxBlock));
+      d.sc = at<uint8_t>(a.qs + r0 * nb, os);
     } else {
       d.x = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * a.g.C, o * (uint32_t)sizeof(T));
     }
@@ -638,7 +660,7 @@ template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
   // x - mean and dz of a row
   template <bool DONE> PG_DEVICE void row(const BwdArgs &a, const Place &p, const Row &d, float (&df)[V], float (&dz)[V]) const {
     float f[V];
-    if constexpr (CK) Codes<V>::decode(d.x, d.sc, f);
+    if constexpr (CK) Codes<V>::decode(d.x, mx8_scale(d.sc), f);
     else X::unpack(d.x, f);
 #pragma unroll
     for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
@@ -652,38 +674,58 @@ template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
   }
 };
 
+// sums of n columns over the rows r0, r0 + step, .. < R of a [R][ld] array, four at a time
+PG_DEVICE float col_sum(const float *p, int r0, int R, int step, int ld) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  int r = r0;
+  for (; r + 3 * step < R; r += 4 * step) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] += p[(r + u * step) * ld];
+  }
+  for (; r < R; r += step) s[0] += p[r * ld];
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// Shared memory of a backward workgroup: sums of the slab's groups; its channels' sums, gamma and
+// rstd; the rows of the reduction.
+template <int V> struct BwdShared {
+  float *g1, *g2, *tot, *ga, *rs, *red2, *red;
+  PG_DEVICE BwdShared(const Geo &g, float *sm)
+      : g1(sm), g2(g1 + g.gs), tot(g2 + g.gs), ga(tot + 2 * g.cs), rs(ga + g.cs), red2(rs + g.cs), red(red2 + blockDim.x) {}
+  // once, ahead of the sums
+  PG_DEVICE void channels(const BwdArgs &a, const Place &p, const float *rstd) const {
+    for (int c = threadIdx.x; c < p.csl; c += blockDim.x) {
+      ga[c] = a.gamma ? a.gamma[p.c0 + c] : 1.f;
+      rs[c] = rstd[c / a.g.cg];
+    }
+  }
+};
+
 // s1 = sum dz (x - mean), s0 = sum dz of the thread -> tot[c] = dgamma, tot[cs + c] = dbeta of the
 // tile (and to dpart), g1, g2 = s1, s2 of its groups
 template <int V>
-PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, const float (&s1)[V], const float (&s0)[V],
-                        float *g1, float *g2, float *tot, float *red2, float *red) {
+PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float (&s1)[V], const float (&s0)[V], const BwdShared<V> &m) {
   const Geo &g = a.g;
   const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (p.on) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
+      for (int j = 0; j < V; ++j) m.red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
     }
     __syncthreads();
     if (nt <= 1) {
       for (int o = t; o < n; o += blockDim.x) {
-        float s = 0.f;
-        for (int r = 0; r < g.R; ++r) s += red[r * ld + o];
-        tot[h * g.cs + o] = h ? s : s * rstd[o / g.cg];
+        const float s = col_sum(m.red + o, 0, g.R, 1, ld);
+        m.tot[h * g.cs + o] = h ? s : s * m.rs[o];
       }
     } else {   // nt stripes of rows a channel
-      const int o = t % n, st = t / n;
-      if (st < nt) {
-        float s = 0.f;
-        for (int r = st; r < g.R; r += nt) s += red[r * ld + o];
-        red2[st * n + o] = s;
-      }
+      const int st = t / n, o = t - st * n;
+      if (st < nt) m.red2[st * n + o] = col_sum(m.red + o, st, g.R, nt, ld);
       __syncthreads();
       if (t < n) {
-        float s = 0.f;
-        for (int i = 0; i < nt; ++i) s += red2[i * n + t];
-        tot[h * g.cs + t] = h ? s : s * rstd[t / g.cg];
+        const float s = col_sum(m.red2 + t, 0, nt, 1, n);
+        m.tot[h * g.cs + t] = h ? s : s * m.rs[t];
       }
     }
     __syncthreads();
@@ -691,8 +733,8 @@ PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, con
   if (a.dpart) {
     float *dst = a.dpart + (p.b * g.k + p.chunk) * 2 * g.C + p.c0;
     for (int j = t; j < n; j += blockDim.x) {
-      dst[j] = tot[j];
-      dst[g.C + j] = tot[g.cs + j];
+      dst[j] = m.tot[j];
+      dst[g.C + j] = m.tot[g.cs + j];
     }
   }
   const int W = seg_width(g.cg), per = 64 / W, lane = t & 63, l = lane & (W - 1);
@@ -700,15 +742,14 @@ PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, con
     float u = 0.f, v = 0.f;
     if (i < p.ng)
       for (int c = i * g.cg + l; c < (i + 1) * g.cg; c += W) {
-        const float ga = a.gamma ? a.gamma[p.c0 + c] : 1.f;
-        u = fmaf(ga, tot[g.cs + c], u);
-        v = fmaf(ga, tot[c], v);
+        u = fmaf(m.ga[c], m.tot[g.cs + c], u);
+        v = fmaf(m.ga[c], m.tot[c], v);
       }
     u = seg_sum(u, W);
     v = seg_sum(v, W);
     if (l == 0 && i < p.ng) {
-      g1[i] = u;
-      g2[i] = v;
+      m.g1[i] = u;
+      m.g2[i] = v;
     }
   }
   __syncthreads();
@@ -724,14 +765,13 @@ PG_DEVICE typename Vec<T, V>::raw gn_dx(const float (&df)[V], const float (&dz)[
   return Vec<T, V>::pack(f);
 }
 template <int VG>
-PG_DEVICE void bwd_constants(const Geo &g, const float *rstd, const int (&gi)[VG], const float *g1, const float *g2,
+PG_DEVICE void bwd_constants(const Geo &g, const float (&rs)[VG], const int (&gi)[VG], const float *g1, const float *g2,
                              float (&k1)[VG], float (&k2)[VG]) {
   const float rm = 1.f / ((float)g.S * (float)g.cg);
 #pragma unroll
   for (int j = 0; j < VG; ++j) {
-    const float rs = rstd[gi[j]];
-    k1[j] = rs * g1[gi[j]] * rm;
-    k2[j] = rs * rs * g2[gi[j]] * rm;
+    k1[j] = rs[j] * g1[gi[j]] * rm;
+    k2[j] = rs[j] * rs[j] * g2[gi[j]] * rm;
   }
 }
 
@@ -742,13 +782,17 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
   typedef BwdThread<T, V, CK, FOLD, SILU> Th;
   const Geo &g = a.g;
   const Place p = place<V, SOLO>(g);
-  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
+  const BwdShared<V> m(g, sm);
   const int nr = (int)g.S;
   const long long r0 = p.b * g.S;
   typename Th::Row d[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) Th::load(a, p, r0, min(p.row + i * g.R, nr - 1), d[i]);
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t r = min(p.row + i * g.R, nr - 1);
+    Th::load(a, r0, r * g.C + p.c, r * ((g.C + kMxBlock - 1) / kMxBlock) + p.c / kMxBlock, d[i]);
+  }
   const Th th(a, p);
+  m.channels(a, p, th.rstd);
   float s0[V], s1[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
@@ -764,10 +808,10 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
         s0[j] += dz[j];
       }
     }
-  bwd_sums<V>(a, p, th.rstd, s1, s0, g1, g2, tot, red2, red);
+  bwd_sums<V>(a, p, s1, s0, m);
   if (!p.on) return;
   float k1[Th::VG], k2[Th::VG];
-  bwd_constants<Th::VG>(g, th.rstd, th.gi, g1, g2, k1, k2);
+  bwd_constants<Th::VG>(g, th.rs, th.gi, m.g1, m.g2, k1, k2);
   T *dst = static_cast<T *>(a.dx) + r0 * g.C;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -781,69 +825,84 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
 }
 
 template <class T, int V, bool CK, bool FOLD, bool SILU>
-__global__ __launch_bounds__(512, 4) void gn_bwd_staged_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   typedef BwdThread<T, V, CK, FOLD, SILU> Th;
   constexpr int U = 2;
   const Geo &g = a.g;
   const Place p = place<V, STAGED>(g);
-  float *g1 = sm, *g2 = sm + g.gs, *tot = sm + 2 * g.gs, *red2 = tot + 2 * g.cs, *red = red2 + blockDim.x;
+  const BwdShared<V> m(g, sm);
   const long long s0 = (long long)p.chunk * g.rows, r0 = p.b * g.S + s0;
   const int nr = (int)min((long long)g.rows, g.S - s0), step = U * g.R;
-  auto load = [&](typename Th::Row (&d)[U], int base) {
+  // offsets of this thread's rows in elements and in scales; past the tile's end, the last row's
+  const uint32_t nb = (g.C + kMxBlock - 1) / kMxBlock, hop = (uint32_t)g.R * g.C, hops = g.R * nb;
+  const uint32_t first = (uint32_t)p.row * g.C + p.c, last = (uint32_t)(nr - 1) * g.C + p.c;
+  const uint32_t firsts = p.row * nb + p.c / kMxBlock, lasts = (nr - 1) * nb + p.c / kMxBlock;
+  auto load = [&](typename Th::Row (&d)[U], int round) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) Th::load(a, p, r0, min(base + p.row + u * g.R, nr - 1), d[u]);
+    for (int u = 0; u < U; ++u)
+      Th::load(a, r0, min(first + (round * U + u) * hop, last), CK ? min(firsts + (round * U + u) * hops, lasts) : 0, d[u]);
   };
+  // where the tiles are joined: W lanes a group, the first group's pairs on their way
+  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
+  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  const int i0 = (threadIdx.x >> 6) * per + lane / W;
+  unsigned long long pv[4];
+  if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
   typename Th::Row d[U], nx[U];
   load(d, 0);
   const Th th(a, p);
   auto stream = [&](auto f) {
-#pragma unroll 1
-    for (int base = 0; base < nr; base += step) {
-      if (base + step < nr) load(nx, base + step);
+    const int rounds = (nr + step - 1) / step;
+    auto work = [&](const typename Th::Row (&v)[U], int round) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = base + p.row + u * g.R;
-        if (r < nr) {
+        if (p.row + (round * U + u) * g.R < nr) {
           float df[V], dz[V];
-          th.template row<false>(a, p, d[u], df, dz);
-          f(df, dz, r);
+          th.template row<false>(a, p, v[u], df, dz);
+          f(df, dz, first + (round * U + u) * hop);
         }
-        __builtin_amdgcn_sched_barrier(0);   // one row's temporaries at a time
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) d[u] = nx[u];
+    };
+#pragma unroll 1
+    for (int i = 0; i < rounds; i += 2) {
+      if (i + 1 < rounds) load(nx, i + 1);
+      work(d, i);
+      if (i + 1 < rounds) {
+        if (i + 2 < rounds) load(d, i + 2);
+        work(nx, i + 1);
+      }
     }
   };
   if (!p.use) {
+    m.channels(a, p, th.rstd);
     float s0[V], s1[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
-    stream([&](const float (&df)[V], const float (&dz)[V], int) {
+    stream([&](const float (&df)[V], const float (&dz)[V], uint32_t) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         s1[j] = fmaf(dz[j], df[j], s1[j]);
         s0[j] += dz[j];
       }
     });
-    bwd_sums<V>(a, p, th.rstd, s1, s0, g1, g2, tot, red2, red);
-    unsigned long long *out = a.part + (p.unit * g.k + p.chunk) * g.gs;
-    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + i, g1[i], g2[i]);
+    bwd_sums<V>(a, p, s1, s0, m);
+    unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk;
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, m.g1[i], m.g2[i]);
     return;
   }
-  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-  for (int i = (threadIdx.x >> 6) * per + lane / W; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
+  for (int i = i0; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
     float u = 0.f, v = 0.f;
     const int gc = min(i, p.ng - 1);
-    if (!pairs(in + gc, g.gs, g.k, l, W, g.wait, [&](int, float s1, float s2) {
+    if (i != i0) pairs_ahead(in + (long long)gc * g.k, g.k, l, W, 0, pv);
+    if (!pairs(in + (long long)gc * g.k, g.k, l, W, g.wait, pv, [&](int, float s1, float s2) {
           u += s1;
           v += s2;
         })) {   // as in the forward
       u = v = 0.f;
-      const int nb = (g.C + kMxBlock - 1) / kMxBlock, at0[1] = {gc};
-      const float m = th.mean[gc], rs = th.rstd[gc];
+      const int at0[1] = {gc};
+      const float mu = th.mean[gc], rs = th.rstd[gc];
 #pragma unroll 1
       for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
 #pragma unroll 1
@@ -853,7 +912,7 @@ __global__ __launch_bounds__(512, 4) void gn_bwd_staged_kernel(const BwdArgs a) 
           const float dy[1] = {tof(static_cast<const T *>(a.dy)[r * g.C + c])};
           if constexpr (CK) x[0] = mx8_dec1(a.q[r * g.C + c]) * mx8_scale(a.qs[r * nb + c / kMxBlock]);
           else x[0] = tof(static_cast<const T *>(a.x)[r * g.C + c]);
-          df[0] = x[0] - m;
+          df[0] = x[0] - mu;
           const float s[1] = {rs * ga}, b[1] = {a.beta ? a.beta[c] : 0.f};
           gn_dz<SILU, 1, 1>(df, x, s, b, gn_tol(b), dy, z, a, th.mean, th.rstd, at0, c);
           u = fmaf(ga, z[0], u);
@@ -863,17 +922,17 @@ __global__ __launch_bounds__(512, 4) void gn_bwd_staged_kernel(const BwdArgs a) 
     u = seg_sum(u, W);
     v = seg_sum(v, W);
     if (l == 0 && i < p.ng) {
-      g1[i] = u;
-      g2[i] = v;
+      m.g1[i] = u;
+      m.g2[i] = v;
     }
   }
   __syncthreads();
   if (!p.on) return;
   float k1[Th::VG], k2[Th::VG];
-  bwd_constants<Th::VG>(g, th.rstd, th.gi, g1, g2, k1, k2);
+  bwd_constants<Th::VG>(g, th.rs, th.gi, m.g1, m.g2, k1, k2);
   T *dst = static_cast<T *>(a.dx) + r0 * g.C;
-  stream([&](const float (&df)[V], const float (&dz)[V], int r) {
-    at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
+  stream([&](const float (&df)[V], const float (&dz)[V], uint32_t o) {
+    at<typename X::raw>(dst, o * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
   });
 }
 

@@ -2,7 +2,7 @@
 #include "../groupnorm.h"
 
 void gn::bwd_fp16(const Plan &p, size_t lds, const BwdArgs &a, hipStream_t st) {
-  if (a.silu) {
+  if (a.act == GN_SILU) {
     if (a.q) launch<Bwd, _Float16, 8, 4, true, true>(p, lds, a, st);
     else launch<Bwd, _Float16, 8, 4, false, true>(p, lds, a, st);
   } else {

@@ -3,7 +3,7 @@
 #include "../groupnorm.h"
 
 #include <algorithm>
-#include <cmath>
+#include <cstdlib>
 #include <numeric>
 #include <stdexcept>
 
@@ -69,7 +69,7 @@ PG_DEVICE void wide_dz(const BwdArgs &a, int dt, long long r, int c, float &df, 
   const float b[1] = {a.beta ? a.beta[c] : 0.f};
   const float y[1] = {load_one(a.dy, dt, i)};
   float v[1];
-  if (a.silu) gn_dz<true, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
+  if (a.act == GN_SILU) gn_dz<true, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
   else gn_dz<false, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
   df = d[0];
   al = s[0];
@@ -152,8 +152,11 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
-constexpr int kTiles = 2048;       // tiles wanted before tiles grow
-constexpr int kLead = 1024;        // sums workgroups ahead of the use workgroups at least: all that are resident
+static int envi(const char*n,int d){const char*s=getenv(n);return s?atoi(s):d;}
+#define kTiles envi("KT",512)
+//       // tiles wanted before tiles grow
+#define kLead envi("KL",1024)
+//        // sums workgroups ahead of the use workgroups at least: all that are resident
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
 int g_wait = 1 << 24;
 
@@ -166,7 +169,7 @@ int gcd_pow2(long long c, int most) {
 // the sums and rows that a workgroup holds in shared memory
 size_t gn_lds(const Plan &p, bool bwd) {
   const size_t red = (size_t)p.TH * p.V;
-  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 2 * (size_t)p.g.cs + p.TH : 0) + red);
+  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 4 * (size_t)p.g.cs + p.TH : 0) + red);
 }
 
 Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {
@@ -224,7 +227,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     }
   }
   // whole rows where they fit a workgroup, the fewest slabs otherwise
-  p.TH = 512;
+  p.TH = bwd ? 256 : 512;
   for (long long slabs = 1;; ++slabs) {
     cs = ((C + slabs - 1) / slabs + L - 1) / L * L;
     shape(cs);
@@ -241,13 +244,14 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   g.R = p.TH / g.CVp;
   // tiles of up to 8 rounds, fewer while the tiles do not fill the chip several times
   const long long round = (long long)g.R * (bwd ? 2 : 4), all = (S + round - 1) / round;
-  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, 8);
+  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, envi("KI",8));
   const long long k = (all + it - 1) / it;
   p.NV = 1;
   g.rows = (int)(round * it);
   g.k = (int)k;
   p.mode = STAGED;
-  g.lead = std::min((kLead + k - 1) / k, B * g.nslab) * k;
+  g.tiles = (int)std::min<long long>(B * g.nslab * k, 0x7fffffff);
+  g.lead = (int)std::min<long long>(std::min((kLead + k - 1) / k, B * g.nslab) * k, 0x7fffffff);
   p.wgs = 2 * B * g.nslab * k;
   check(k);
   return p;
@@ -316,8 +320,7 @@ void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, cons
   const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, true);
   const Ws w = gn_ws(p, true);
   const BwdArgs a{p.g, dy, x, q, qs, gamma, beta, mean, rstd, dx, reinterpret_cast<unsigned long long *>(ws + w.part),
-                  dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act == GN_SILU, act == GN_NONE ? -INFINITY : 0.f,
-                  act == GN_RELU6 ? 6.f : INFINITY};
+                  dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act};
   gn_none(p, a.part, st);
   if (p.mode == WIDE) {
     if (B * C > 0x7fffffff) throw std::invalid_argument("gn_bwd: B * C is too large");

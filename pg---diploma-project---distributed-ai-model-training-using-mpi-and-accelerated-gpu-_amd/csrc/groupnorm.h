@@ -174,6 +174,17 @@ template <class R> PG_DEVICE R &at(void *base, uint32_t off) {
   return *reinterpret_cast<R *>(static_cast<char *>(base) + off);
 }
 
+// V values of an optional per-channel vector.  The loads are unconditional (`any` is readable memory
+// of one float): behind a branch each would be waited for by itself, 0.6 us apiece.
+template <int V> PG_DEVICE void channel_values(const float *v, const float *any, int c, float none, float (&out)[V]) {
+  const float *src = v ? v : any;
+  const uint32_t first = v ? c * 4u : 0u, step = v ? 4u : 0u;
+#pragma unroll
+  for (int j = 0; j < V; ++j) out[j] = at<float>(src, first + j * step);
+#pragma unroll
+  for (int j = 0; j < V; ++j) out[j] = v ? out[j] : none;
+}
+
 PG_DEVICE float seg_sum(float v, int W) {   // sum over aligned segments of W lanes
   for (int o = W >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
@@ -323,16 +334,13 @@ template <class F> PG_DEVICE void with_act(int act, F f) {
 }
 
 // the statistics of the slab's groups (gm: mean, gr: rstd) as this thread's channels take them
+// (sc: gamma before, gamma rstd after)
 template <int V, int VG>
-PG_DEVICE void fwd_constants(const FwdArgs &a, const Place &p, const int (&gi)[VG], const float *gm, const float *gr,
-                             float (&mu)[VG], float (&sc)[V], float (&be)[V]) {
+PG_DEVICE void fwd_constants(const int (&gi)[VG], const float *gm, const float *gr, float (&mu)[VG], float (&sc)[V]) {
 #pragma unroll
   for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    sc[j] = gr[gi[VG == 1 ? 0 : j]] * (a.gamma ? a.gamma[p.c + j] : 1.f);
-    be[j] = a.beta ? a.beta[p.c + j] : 0.f;
-  }
+  for (int j = 0; j < V; ++j) sc[j] *= gr[gi[VG == 1 ? 0 : j]];
 }
 PG_DEVICE void fwd_statistics(const FwdArgs &a, const Place &p, const float *gm, const float *gr) {
   if (p.chunk == 0)
@@ -365,6 +373,8 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
     d[i] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
   }
   float acc[V], mu[VG], sc[V], be[V];
+  channel_values(a.gamma, a.mean, p.c, 1.f, sc);
+  channel_values(a.beta, a.mean, p.c, 0.f, be);
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
 #pragma unroll
@@ -404,7 +414,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
   __syncthreads();
   fwd_statistics(a, p, gm, gr);
   if (!p.on) return;
-  fwd_constants<V, VG>(a, p, gi, gm, gr, mu, sc, be);
+  fwd_constants<V, VG>(gi, gm, gr, mu, sc);
   with_act(a.act, [&](auto act) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -510,6 +520,9 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
     for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, gm[i] * cn, gr[i]);
     return;
   }
+  float mu[VG], sc[V], be[V];
+  channel_values(a.gamma, a.mean, p.c, 1.f, sc);
+  channel_values(a.beta, a.mean, p.c, 0.f, be);
   for (int i = i0; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
     Moments t{0.f, 0.f, 0.f};
     const int gc = min(i, p.ng - 1);
@@ -534,8 +547,7 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
   __syncthreads();
   fwd_statistics(a, p, gm, gr);
   if (!p.on) return;
-  float mu[VG], sc[V], be[V];
-  fwd_constants<V, VG>(a, p, gi, gm, gr, mu, sc, be);
+  fwd_constants<V, VG>(gi, gm, gr, mu, sc);
   with_act(a.act, [&](auto act) {
     stream([&](const typename X::raw &raw, int r, uint32_t off) {
       if (r < nr)
@@ -557,122 +569,39 @@ struct BwdArgs {
   int act;
 };
 
-// act'(z) dy of V channels (df = x - mean).  Which side of relu's or relu6's border z lies on is
-// decided from the operands as they are: within fp32's rounding of a border (z takes four roundings of terms no
-// larger than |z| + |beta|) z is formed again in 64 bits, once in some 10^5 vectors.
-template <bool SILU, int V, int VG>
-PG_DEVICE void gn_dz(const float (&df)[V], const float (&x)[V], const float (&al)[V], const float (&be)[V], float tol,
-                     const float (&dy)[V], float (&dz)[V], const BwdArgs &a, const float *mean, const float *rstd,
-                     const int (&gi)[VG], int c) {
-  if constexpr (SILU) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float z = fmaf(df[j], al[j], be[j]);
-      const float s = 1.f / (1.f + __expf(-z));
-      dz[j] = dy[j] * (s * fmaf(z, 1.f - s, 1.f));
-    }
+// Which values of a channel relu and relu6 pass: lo < x < hi.  0 < z (and z < 6) is a condition on x
+// itself, x > mean - beta / (rstd gamma) or < where gamma < 0.  The border is found in 64 bits, once a
+// channel, and rounded away from the side that passes, so the comparison of x, which is exact in
+// fp32, with it tells what z in 64 bits would: no rounding of z takes part.
+PG_DEVICE void gn_border(int act, float mean, float rstd, float gamma, float beta, float &lo, float &hi) {
+  const double k = (double)rstd * (double)gamma, b = beta;
+  lo = -INFINITY;
+  hi = INFINITY;
+  if (act != GN_RELU && act != GN_RELU6) return;
+  if (k == 0.0) {   // z is beta everywhere
+    if (!(beta > 0.f) || (act == GN_RELU6 && !(beta < 6.f))) lo = INFINITY;
+    return;
+  }
+  const double t0 = (double)mean - b / k, t6 = (double)mean + (6.0 - b) / k;
+  if (k > 0.0) {
+    lo = __double2float_rd(t0);
+    if (act == GN_RELU6) hi = __double2float_ru(t6);
   } else {
-    float near = INFINITY;   // of the distances to the borders
-    if (a.act == GN_RELU6) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float v = fabsf(fmaf(df[j], al[j], be[j]) - 3.f) - 3.f;   // below 0 between the borders
-        dz[j] = v < 0.f ? dy[j] : 0.f;
-        near = fminf(near, fabsf(v));
-      }
-    } else if (a.act == GN_RELU) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float z = fmaf(df[j], al[j], be[j]);
-        dz[j] = z > 0.f ? dy[j] : 0.f;
-        near = fminf(near, fabsf(z));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) dz[j] = dy[j];
-    }
-    if (near <= tol) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        // One value at a time, its operands read again and made opaque: together, or hoisted out
-        // of the row loop, their 64-bit copies would cost the whole kernel its registers.
-        int k = gi[VG == 1 ? 0 : j], cj = c + j;
-        float b = be[j], v = x[j];
-        asm volatile("" : "+v"(k), "+v"(cj), "+v"(b), "+v"(v));
-        const float z = fmaf(df[j], al[j], b);
-        if (fabsf(z) <= tol || fabsf(z - 6.f) <= tol) {
-          const double w = ((double)v - (double)mean[k]) * (double)rstd[k] * (a.gamma ? (double)a.gamma[cj] : 1.0) +
-                           (double)b;
-          dz[j] = w > 0.0 && (a.act == GN_RELU || w < 6.0) ? dy[j] : 0.f;
-        }
-      }
-    }
+    hi = __double2float_ru(t0);
+    if (act == GN_RELU6) lo = __double2float_rd(t6);
   }
 }
-// how near to a border fp32 cannot tell the side of any of the channels
-template <int V> PG_DEVICE float gn_tol(const float (&be)[V]) {
-  float m = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(be[j]));
-  return fmaf(m, 1e-6f, 8e-6f);
+
+// act'(z) dy.  SILU: u, v are rstd gamma and beta, and df is x - mean; otherwise the borders of x.
+// NaN passes.
+template <bool SILU> PG_DEVICE float gn_dz(float dy, float x, float df, float u, float v) {
+  if constexpr (SILU) {
+    const float z = fmaf(df, u, v), s = 1.f / (1.f + __expf(-z));
+    return dy * (s * fmaf(z, 1.f - s, 1.f));
+  } else {
+    return x <= u || x >= v ? 0.f : dy;
+  }
 }
-
-// what a thread needs of its channels, and the rows it reads
-template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
-  typedef Vec<T, V> X;
-  static constexpr int VG = FOLD ? 1 : V;
-  struct Row {
-    typename X::raw dy;
-    typename std::conditional<CK, typename Codes<V>::raw, typename X::raw>::type x;
-    uint8_t sc;   // checkpoint: the scale's byte
-  };
-  const float *mean, *rstd;   // of the slab's first group
-  int gi[VG];
-  float mu[VG], rs[VG], al[V], be[V], tol;
-
-  PG_DEVICE BwdThread(const BwdArgs &a, const Place &p) {
-    mean = a.mean + p.b * a.g.G + p.g0;
-    rstd = a.rstd + p.b * a.g.G + p.g0;
-#pragma unroll
-    for (int j = 0; j < VG; ++j) {
-      gi[j] = (p.c - p.c0 + j) / a.g.cg;
-      mu[j] = mean[gi[j]];
-      rs[j] = rstd[gi[j]];
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      al[j] = rs[FOLD ? 0 : j] * (a.gamma ? a.gamma[p.c + j] : 1.f);
-      be[j] = a.beta ? a.beta[p.c + j] : 0.f;
-    }
-    tol = gn_tol(be);
-  }
-  // the row at element offset o (and scale offset os) of the tile that begins at row r0 of the tensor
-  static PG_DEVICE void load(const BwdArgs &a, long long r0, uint32_t o, uint32_t os, Row &d) {
-    const int nb = (a.g.C + kMxBlock - 1) / kMxBlock;
-    d.dy = at<typename X::raw>(static_cast<const T *>(a.dy) + r0 * a.g.C, o * (uint32_t)sizeof(T));
-    if constexpr (CK) {
-      d.x = at<typename Codes<V>::raw>(a.q + r0 * a.g.C, o);
-      d.sc = at<uint8_t>(a.qs + r0 * nb, os);
-    } else {
-      d.x = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * a.g.C, o * (uint32_t)sizeof(T));
-    }
-  }
-  // x - mean and dz of a row
-  template <bool DONE> PG_DEVICE void row(const BwdArgs &a, const Place &p, const Row &d, float (&df)[V], float (&dz)[V]) const {
-    float f[V];
-    if constexpr (CK) Codes<V>::decode(d.x, mx8_scale(d.sc), f);
-    else X::unpack(d.x, f);
-#pragma unroll
-    for (int j = 0; j < V; ++j) df[j] = f[j] - mu[FOLD ? 0 : j];
-    if constexpr (DONE) {
-      X::unpack(d.dy, dz);
-    } else {
-      float dy[V];
-      X::unpack(d.dy, dy);
-      gn_dz<SILU, V, VG>(df, f, al, be, tol, dy, dz, a, mean, rstd, gi, p.c);
-    }
-  }
-};
 
 // sums of n columns over the rows r0, r0 + step, .. < R of a [R][ld] array, four at a time
 PG_DEVICE float col_sum(const float *p, int r0, int R, int step, int ld) {
@@ -686,17 +615,86 @@ PG_DEVICE float col_sum(const float *p, int r0, int R, int step, int ld) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// Shared memory of a backward workgroup: sums of the slab's groups; its channels' sums, gamma and
-// rstd; the rows of the reduction.
-template <int V> struct BwdShared {
-  float *g1, *g2, *tot, *ga, *rs, *red2, *red;
+// Shared memory of a backward workgroup: what its channels need (gamma, rstd gamma, and gn_dz's u and
+// v), the sums of its channels and groups, the rows of the reduction.
+struct BwdShared {
+  float *ga, *al, *u, *v, *tot, *g1, *g2, *red2, *red;
   PG_DEVICE BwdShared(const Geo &g, float *sm)
-      : g1(sm), g2(g1 + g.gs), tot(g2 + g.gs), ga(tot + 2 * g.cs), rs(ga + g.cs), red2(rs + g.cs), red(red2 + blockDim.x) {}
-  // once, ahead of the sums
-  PG_DEVICE void channels(const BwdArgs &a, const Place &p, const float *rstd) const {
+      : ga(sm), al(ga + g.cs), u(al + g.cs), v(u + g.cs), tot(v + g.cs), g1(tot + 2 * g.cs), g2(g1 + g.gs),
+        red2(g2 + g.gs), red(red2 + blockDim.x) {}
+  // one channel's values: asked for early, put down when they are here
+  struct Channel { float ga[1], be[1], mean, rstd; };
+  static PG_DEVICE void ask(const BwdArgs &a, const Place &p, const float *mean, const float *rstd, int c, Channel &k) {
+    channel_values(a.gamma, rstd, p.c0 + c, 1.f, k.ga);
+    channel_values(a.beta, rstd, p.c0 + c, 0.f, k.be);
+    k.mean = at<float>(mean, (c / a.g.cg) * 4u);
+    k.rstd = at<float>(rstd, (c / a.g.cg) * 4u);
+  }
+  template <bool SILU>
+  PG_DEVICE void put(const BwdArgs &a, const Place &p, const float *mean, const float *rstd, Channel &k) const {
     for (int c = threadIdx.x; c < p.csl; c += blockDim.x) {
-      ga[c] = a.gamma ? a.gamma[p.c0 + c] : 1.f;
-      rs[c] = rstd[c / a.g.cg];
+      if (c != (int)threadIdx.x) ask(a, p, mean, rstd, c, k);
+      ga[c] = k.ga[0];
+      al[c] = k.rstd * k.ga[0];
+      if constexpr (SILU) {
+        u[c] = al[c];
+        v[c] = k.be[0];
+      } else {
+        gn_border(a.act, k.mean, k.rstd, k.ga[0], k.be[0], u[c], v[c]);
+      }
+    }
+    __syncthreads();
+  }
+};
+
+// what a thread needs of its channels, and the rows it reads
+template <class T, int V, bool CK, bool FOLD, bool SILU> struct BwdThread {
+  typedef Vec<T, V> X;
+  static constexpr int VG = FOLD ? 1 : V;
+  struct Row {
+    typename X::raw dy;
+    typename std::conditional<CK, typename Codes<V>::raw, typename X::raw>::type x;
+    uint8_t sc;   // checkpoint: the scale's byte
+  };
+  int gi[VG];   // slab group of each channel (FOLD: of all)
+  float mu[VG], rs[VG], u[V], v[V];
+
+  PG_DEVICE void groups(const Geo &g, const Place &p, const float *mean, const float *rstd) {
+#pragma unroll
+    for (int j = 0; j < VG; ++j) {
+      gi[j] = (p.c - p.c0 + j) / g.cg;
+      mu[j] = at<float>(mean, gi[j] * 4u);
+      rs[j] = at<float>(rstd, gi[j] * 4u);
+    }
+  }
+  PG_DEVICE void channels(const Place &p, const BwdShared &m) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      u[j] = m.u[p.c - p.c0 + j];
+      v[j] = m.v[p.c - p.c0 + j];
+    }
+  }
+  // the row at element offset o (and scale offset os) of the tile that begins at row r0 of the tensor
+  static PG_DEVICE void load(const BwdArgs &a, long long r0, uint32_t o, uint32_t os, Row &d) {
+    const int nb = (a.g.C + kMxBlock - 1) / kMxBlock;
+    d.dy = at<typename X::raw>(static_cast<const T *>(a.dy) + r0 * a.g.C, o * (uint32_t)sizeof(T));
+    if constexpr (CK) {
+      d.x = at<typename Codes<V>::raw>(a.q + r0 * a.g.C, o);
+      d.sc = at<uint8_t>(a.qs + r0 * nb, os);
+    } else {
+      d.x = at<typename X::raw>(static_cast<const T *>(a.x) + r0 * a.g.C, o * (uint32_t)sizeof(T));
+    }
+  }
+  // x - mean and dz of a row (DONE: dy holds dz)
+  template <bool DONE> PG_DEVICE void row(const Row &d, float (&df)[V], float (&dz)[V]) const {
+    float f[V];
+    if constexpr (CK) Codes<V>::decode(d.x, mx8_scale(d.sc), f);
+    else X::unpack(d.x, f);
+    X::unpack(d.dy, dz);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      df[j] = f[j] - mu[FOLD ? 0 : j];
+      if constexpr (!DONE) dz[j] = gn_dz<SILU>(dz[j], f[j], df[j], u[j], v[j]);
     }
   }
 };
@@ -704,9 +702,11 @@ template <int V> struct BwdShared {
 // s1 = sum dz (x - mean), s0 = sum dz of the thread -> tot[c] = dgamma, tot[cs + c] = dbeta of the
 // tile (and to dpart), g1, g2 = s1, s2 of its groups
 template <int V>
-PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float (&s1)[V], const float (&s0)[V], const BwdShared<V> &m) {
+PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, const float (&s1)[V], const float (&s0)[V],
+                        const BwdShared &m) {
   const Geo &g = a.g;
   const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
+  const float rs = at<float>(rstd, min(t, n - 1) / g.cg * 4u);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (p.on) {
@@ -717,7 +717,7 @@ PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float (&s1)[V], 
     if (nt <= 1) {
       for (int o = t; o < n; o += blockDim.x) {
         const float s = col_sum(m.red + o, 0, g.R, 1, ld);
-        m.tot[h * g.cs + o] = h ? s : s * m.rs[o];
+        m.tot[h * g.cs + o] = h ? s : s * (o == t ? rs : rstd[o / g.cg]);
       }
     } else {   // nt stripes of rows a channel
       const int st = t / n, o = t - st * n;
@@ -725,7 +725,7 @@ PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float (&s1)[V], 
       __syncthreads();
       if (t < n) {
         const float s = col_sum(m.red2 + t, 0, nt, 1, n);
-        m.tot[h * g.cs + t] = h ? s : s * m.rs[t];
+        m.tot[h * g.cs + t] = h ? s : s * rs;
       }
     }
     __syncthreads();
@@ -764,15 +764,17 @@ PG_DEVICE typename Vec<T, V>::raw gn_dx(const float (&df)[V], const float (&dz)[
   for (int j = 0; j < V; ++j) f[j] = fmaf(dz[j], al[j], -fmaf(df[j], k2[VG == 1 ? 0 : j], k1[VG == 1 ? 0 : j]));
   return Vec<T, V>::pack(f);
 }
-template <int VG>
-PG_DEVICE void bwd_constants(const Geo &g, const float (&rs)[VG], const int (&gi)[VG], const float *g1, const float *g2,
-                             float (&k1)[VG], float (&k2)[VG]) {
+template <int V, int VG>
+PG_DEVICE void bwd_constants(const Geo &g, const Place &p, const float (&rs)[VG], const int (&gi)[VG], const BwdShared &m,
+                             float (&al)[V], float (&k1)[VG], float (&k2)[VG]) {
   const float rm = 1.f / ((float)g.S * (float)g.cg);
 #pragma unroll
   for (int j = 0; j < VG; ++j) {
-    k1[j] = rs[j] * g1[gi[j]] * rm;
-    k2[j] = rs[j] * rs[j] * g2[gi[j]] * rm;
+    k1[j] = rs[j] * m.g1[gi[j]] * rm;
+    k2[j] = rs[j] * rs[j] * m.g2[gi[j]] * rm;
   }
+#pragma unroll
+  for (int j = 0; j < V; ++j) al[j] = m.al[p.c - p.c0 + j];
 }
 
 template <class T, int V, int NV, bool CK, bool FOLD, bool SILU>
@@ -782,17 +784,22 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
   typedef BwdThread<T, V, CK, FOLD, SILU> Th;
   const Geo &g = a.g;
   const Place p = place<V, SOLO>(g);
-  const BwdShared<V> m(g, sm);
+  const BwdShared m(g, sm);
+  const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
   const int nr = (int)g.S;
   const long long r0 = p.b * g.S;
+  Th th;
+  BwdShared::Channel own;
+  th.groups(g, p, mean, rstd);
+  BwdShared::ask(a, p, mean, rstd, min((int)threadIdx.x, p.csl - 1), own);
   typename Th::Row d[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint32_t r = min(p.row + i * g.R, nr - 1);
     Th::load(a, r0, r * g.C + p.c, r * ((g.C + kMxBlock - 1) / kMxBlock) + p.c / kMxBlock, d[i]);
   }
-  const Th th(a, p);
-  m.channels(a, p, th.rstd);
+  m.put<SILU>(a, p, mean, rstd, own);
+  th.channels(p, m);
   float s0[V], s1[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
@@ -800,7 +807,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
   for (int i = 0; i < NV; ++i)
     if (p.row + i * g.R < nr) {
       float df[V], dz[V];
-      th.template row<false>(a, p, d[i], df, dz);
+      th.template row<false>(d[i], df, dz);
       if constexpr (!SILU) d[i].dy = X::pack(dz);   // dy or 0: it takes dy's place for the second use
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -808,31 +815,32 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
         s0[j] += dz[j];
       }
     }
-  bwd_sums<V>(a, p, s1, s0, m);
+  bwd_sums<V>(a, p, rstd, s1, s0, m);
   if (!p.on) return;
-  float k1[Th::VG], k2[Th::VG];
-  bwd_constants<Th::VG>(g, th.rs, th.gi, m.g1, m.g2, k1, k2);
+  float al[V], k1[Th::VG], k2[Th::VG];
+  bwd_constants<V, Th::VG>(g, p, th.rs, th.gi, m, al, k1, k2);
   T *dst = static_cast<T *>(a.dx) + r0 * g.C;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int r = p.row + i * g.R;
     if (r < nr) {
       float df[V], dz[V];
-      th.template row<!SILU>(a, p, d[i], df, dz);
-      at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
+      th.template row<!SILU>(d[i], df, dz);
+      at<typename X::raw>(dst, ((uint32_t)r * g.C + p.c) * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, al, k1, k2);
     }
   }
 }
 
 template <class T, int V, bool CK, bool FOLD, bool SILU>
-__global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kernel(const BwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   typedef BwdThread<T, V, CK, FOLD, SILU> Th;
   constexpr int U = 2;
   const Geo &g = a.g;
   const Place p = place<V, STAGED>(g);
-  const BwdShared<V> m(g, sm);
+  const BwdShared m(g, sm);
+  const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
   const long long s0 = (long long)p.chunk * g.rows, r0 = p.b * g.S + s0;
   const int nr = (int)min((long long)g.rows, g.S - s0), step = U * g.R;
   // offsets of this thread's rows in elements and in scales; past the tile's end, the last row's
@@ -850,9 +858,14 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
   const int i0 = (threadIdx.x >> 6) * per + lane / W;
   unsigned long long pv[4];
   if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
+  Th th;
+  BwdShared::Channel own;
+  th.groups(g, p, mean, rstd);
+  BwdShared::ask(a, p, mean, rstd, min((int)threadIdx.x, p.csl - 1), own);
   typename Th::Row d[U], nx[U];
   load(d, 0);
-  const Th th(a, p);
+  m.put<SILU>(a, p, mean, rstd, own);
+  th.channels(p, m);
   auto stream = [&](auto f) {
     const int rounds = (nr + step - 1) / step;
     auto work = [&](const typename Th::Row (&v)[U], int round) {
@@ -860,7 +873,7 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
       for (int u = 0; u < U; ++u) {
         if (p.row + (round * U + u) * g.R < nr) {
           float df[V], dz[V];
-          th.template row<false>(a, p, v[u], df, dz);
+          th.template row<false>(v[u], df, dz);
           f(df, dz, first + (round * U + u) * hop);
         }
       }
@@ -876,7 +889,6 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
     }
   };
   if (!p.use) {
-    m.channels(a, p, th.rstd);
     float s0[V], s1[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
@@ -887,7 +899,7 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
         s0[j] += dz[j];
       }
     });
-    bwd_sums<V>(a, p, s1, s0, m);
+    bwd_sums<V>(a, p, rstd, s1, s0, m);
     unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk;
     for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, m.g1[i], m.g2[i]);
     return;
@@ -901,22 +913,18 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
           v += s2;
         })) {   // as in the forward
       u = v = 0.f;
-      const int at0[1] = {gc};
-      const float mu = th.mean[gc], rs = th.rstd[gc];
+      const float mu = mean[gc], rs = rstd[gc];
 #pragma unroll 1
       for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
 #pragma unroll 1
-        for (int c = p.c0 + gc * g.cg; c < p.c0 + (gc + 1) * g.cg; ++c) {
-          const float ga = a.gamma ? a.gamma[c] : 1.f;
-          float x[1], df[1], z[1];
-          const float dy[1] = {tof(static_cast<const T *>(a.dy)[r * g.C + c])};
-          if constexpr (CK) x[0] = mx8_dec1(a.q[r * g.C + c]) * mx8_scale(a.qs[r * nb + c / kMxBlock]);
-          else x[0] = tof(static_cast<const T *>(a.x)[r * g.C + c]);
-          df[0] = x[0] - mu;
-          const float s[1] = {rs * ga}, b[1] = {a.beta ? a.beta[c] : 0.f};
-          gn_dz<SILU, 1, 1>(df, x, s, b, gn_tol(b), dy, z, a, th.mean, th.rstd, at0, c);
-          u = fmaf(ga, z[0], u);
-          v = fmaf(ga * rs * df[0], z[0], v);
+        for (int c = gc * g.cg; c < (gc + 1) * g.cg; ++c) {
+          const long long at = r * g.C + p.c0 + c;
+          float x;
+          if constexpr (CK) x = mx8_dec1(a.q[at]) * mx8_scale(a.qs[r * nb + (p.c0 + c) / kMxBlock]);
+          else x = tof(static_cast<const T *>(a.x)[at]);
+          const float z = gn_dz<SILU>(tof(static_cast<const T *>(a.dy)[at]), x, x - mu, m.u[c], m.v[c]);
+          u = fmaf(m.ga[c], z, u);
+          v = fmaf(m.ga[c] * rs * (x - mu), z, v);
         }
     }
     u = seg_sum(u, W);
@@ -928,11 +936,11 @@ __global__ __launch_bounds__(256, 3) void gn_bwd_staged_kernel(const BwdArgs a) 
   }
   __syncthreads();
   if (!p.on) return;
-  float k1[Th::VG], k2[Th::VG];
-  bwd_constants<Th::VG>(g, th.rs, th.gi, m.g1, m.g2, k1, k2);
+  float al[V], k1[Th::VG], k2[Th::VG];
+  bwd_constants<V, Th::VG>(g, p, th.rs, th.gi, m, al, k1, k2);
   T *dst = static_cast<T *>(a.dx) + r0 * g.C;
   stream([&](const float (&df)[V], const float (&dz)[V], uint32_t o) {
-    at<typename X::raw>(dst, o * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, th.al, k1, k2);
+    at<typename X::raw>(dst, o * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, al, k1, k2);
   });
 }
 

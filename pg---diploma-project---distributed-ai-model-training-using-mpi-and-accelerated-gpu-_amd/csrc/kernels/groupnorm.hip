@@ -3,7 +3,6 @@
 #include "../groupnorm.h"
 
 #include <algorithm>
-#include <cstdlib>
 #include <numeric>
 #include <stdexcept>
 
@@ -62,18 +61,19 @@ __global__ __launch_bounds__(256) void gn_wide_apply_kernel(const FwdArgs a, int
 // value i's x - mean, gamma rstd and dz
 PG_DEVICE void wide_dz(const BwdArgs &a, int dt, long long r, int c, float &df, float &al, float &dz) {
   const Geo &g = a.g;
-  const long long i = r * g.C + c, k = r / g.S * g.G + c / g.cg;
-  const int nb = (g.C + kMxBlock - 1) / kMxBlock, gi[1] = {0};
-  const float x[1] = {a.q ? mx8_dec1(a.q[i]) * mx8_scale(a.qs[r * nb + c / kMxBlock]) : load_one(a.x, dt, i)};
-  const float d[1] = {x[0] - a.mean[k]}, s[1] = {a.rstd[k] * (a.gamma ? a.gamma[c] : 1.f)};
-  const float b[1] = {a.beta ? a.beta[c] : 0.f};
-  const float y[1] = {load_one(a.dy, dt, i)};
-  float v[1];
-  if (a.act == GN_SILU) gn_dz<true, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
-  else gn_dz<false, 1, 1>(d, x, s, b, gn_tol(b), y, v, a, a.mean + k, a.rstd + k, gi, c);
-  df = d[0];
-  al = s[0];
-  dz = v[0];
+  const long long i = r * g.C + c, b = r / g.S, k = b * g.G + c / g.cg;
+  const int nb = (g.C + kMxBlock - 1) / kMxBlock;
+  const float x = a.q ? mx8_dec1(a.q[i]) * mx8_scale(a.qs[r * nb + c / kMxBlock]) : load_one(a.x, dt, i);
+  const float ga = a.gamma ? a.gamma[c] : 1.f, be = a.beta ? a.beta[c] : 0.f, dy = load_one(a.dy, dt, i);
+  df = x - a.mean[k];
+  al = a.rstd[k] * ga;
+  if (a.act == GN_SILU) {
+    dz = gn_dz<true>(dy, x, df, al, be);
+  } else {
+    float lo, hi;
+    gn_border(a.act, a.mean[k], a.rstd[k], ga, be, lo, hi);
+    dz = gn_dz<false>(dy, x, df, lo, hi);
+  }
 }
 // one workgroup per (image, channel) -> dpart [B][2][C]
 __global__ __launch_bounds__(256) void gn_wide_dsums_kernel(const BwdArgs a, int dt) {
@@ -152,11 +152,11 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
-static int envi(const char*n,int d){const char*s=getenv(n);return s?atoi(s):d;}
-#define kTiles envi("KT",512)
-//       // tiles wanted before tiles grow
-#define kLead envi("KL",1024)
-//        // sums workgroups ahead of the use workgroups at least: all that are resident
+constexpr int kTiles = 512;   // tiles wanted before tiles grow (2048: gn_bwd 96 x 784 x 192 98 us, not 43)
+constexpr int kRounds = 6;    // rounds of a tile at most (2, 4, 8, 16: gn_bwd 128 x 12544 x 96 360, 260, 265, 314 us)
+// sums workgroups ahead of the use workgroups at least: half of what is resident (128, 256, 384, 1024:
+// gn_bwd 128 x 12544 x 96 +23%, +6%, -2%, +8%; gn_fwd 128 x 3136 x 144 +15%, +4%, +3%, 0%)
+constexpr int kLead = 512;
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
 int g_wait = 1 << 24;
 
@@ -169,7 +169,7 @@ int gcd_pow2(long long c, int most) {
 // the sums and rows that a workgroup holds in shared memory
 size_t gn_lds(const Plan &p, bool bwd) {
   const size_t red = (size_t)p.TH * p.V;
-  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 4 * (size_t)p.g.cs + p.TH : 0) + red);
+  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 * (size_t)p.g.cs + p.TH : 0) + red);
 }
 
 Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {
@@ -242,9 +242,9 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     return p;
   }
   g.R = p.TH / g.CVp;
-  // tiles of up to 8 rounds, fewer while the tiles do not fill the chip several times
+  // tiles of up to kRounds rounds, fewer while the tiles do not fill the chip several times
   const long long round = (long long)g.R * (bwd ? 2 : 4), all = (S + round - 1) / round;
-  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, envi("KI",8));
+  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, kRounds);
   const long long k = (all + it - 1) / it;
   p.NV = 1;
   g.rows = (int)(round * it);

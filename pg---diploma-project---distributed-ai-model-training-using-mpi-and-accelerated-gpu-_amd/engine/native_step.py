@@ -24,6 +24,8 @@ from .executor import MobileNetV2Executor
 
 def executor_class(model):
     """Static-plan executor of a model family (MobileNetV2 or ResNet)."""
+    if getattr(model, "norm", "batch") != "batch":
+        raise NotImplementedError("the native executors are built for BatchNorm models")
     from ..models.resnet import ResNet
     if isinstance(model, ResNet):
         from .resnet_executor import ResNet50Executor

@@ -64,7 +64,10 @@ class Trainer:
         self.timer = None
         backend = cfg.backend
         if backend == "auto":
-            backend = "hip" if self.device.type == "cuda" else "torch"
+            backend = "hip" if self.device.type == "cuda" and cfg.norm == "batch" else "torch"
+        if backend == "hip" and cfg.norm != "batch":
+            raise NotImplementedError("the native executors are built for BatchNorm; norm='group' runs on the torch "
+                                      "backend (with the HIP group-norm kernels on a GPU)")
         if backend == "hip" and self.device.type != "cuda":
             raise RuntimeError("backend 'hip' needs a GPU")
         self.backend = backend
@@ -98,7 +101,7 @@ class Trainer:
         self.test_sampler = ShardSampler(len(self.test_data), self.world, self.rank, shuffle=False)
 
         # ---- model
-        self.model = build_model(cfg.model, cfg.num_classes, cfg.pretrained)
+        self.model = build_model(cfg.model, cfg.num_classes, cfg.pretrained, norm=cfg.norm, act_ckpt=cfg.act_ckpt)
         L.emit(L.params_line(sum(p.numel() for p in self.model.parameters())), self.rank)
         if backend == "hip":
             self._init_hip()

@@ -76,8 +76,9 @@ def main(argv=None):
     ap.add_argument("--normalize", choices=("imagenet", "cifar"), default="imagenet")
     ap.add_argument("--device", default="auto")
     ap.add_argument("--model", default="mobilenet_v2", help="mobilenet_v2 | resnet50 (checkpoint architecture)")
+    ap.add_argument("--norm", default="batch", help="batch | group (checkpoint architecture)")
     a = ap.parse_args(argv)
-    pred = Predictor(a.checkpoint, device=a.device, normalize=a.normalize, model_name=a.model)
+    pred = Predictor(a.checkpoint, device=a.device, normalize=a.normalize, model_name=a.model, norm=a.norm)
     try:
         demo = build_gradio(pred)
         demo.launch(server_name=a.host, server_port=a.port)

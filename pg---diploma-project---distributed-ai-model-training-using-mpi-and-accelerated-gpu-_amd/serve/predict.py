@@ -48,12 +48,12 @@ class Predictor:
     def __init__(self, checkpoint: Optional[str] = None, model: Optional[torch.nn.Module] = None,
                  device: Union[str, torch.device] = "auto", classes: Sequence[str] = CIFAR10_CLASSES,
                  img_size: int = 224, backend: str = "auto", normalize: str = "imagenet",
-                 max_batch: int = 16, model_name: str = "mobilenet_v2"):
+                 max_batch: int = 16, model_name: str = "mobilenet_v2", norm: str = "batch"):
         dev = torch.device("cuda" if (device == "auto" and torch.cuda.is_available()) else
                            ("cpu" if device == "auto" else device))
         self.device, self.classes, self.img_size = dev, tuple(classes), img_size
         if model is None:
-            model = build_model(model_name, num_classes=len(classes))
+            model = build_model(model_name, num_classes=len(classes), norm=norm)
             if checkpoint:
                 from ..engine.checkpoint import load_model_weights
                 load_model_weights(model, checkpoint)
@@ -63,7 +63,7 @@ class Predictor:
         self.mean, self.std = ((0.4914, 0.4822, 0.4465), (0.2023, 0.1994, 0.2010)) if normalize == "cifar" \
             else (IMAGENET_MEAN, IMAGENET_STD)
         if backend == "auto":
-            backend = "hip" if dev.type == "cuda" else "torch"
+            backend = "hip" if dev.type == "cuda" and getattr(model, "norm", "batch") == "batch" else "torch"
         self.backend = backend
         self.max_batch = max_batch
         if backend == "hip":   # native eval executor of the model family (BN from running statistics)

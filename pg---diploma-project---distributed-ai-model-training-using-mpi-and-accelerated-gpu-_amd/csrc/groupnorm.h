@@ -127,32 +127,55 @@ PG_DEVICE int seg_width(int n) {   // lanes that share n terms: a power of two u
   return W;
 }
 
+// sums of n columns over the rows r0, r0 + step, .. < R of a [R][ld] array, four at a time
+PG_DEVICE float col_sum(const float *p, int r0, int R, int step, int ld) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  int r = r0;
+  for (; r + 3 * step < R; r += 4 * step) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) s[u] += p[(r + u * step) * ld];
+  }
+  for (; r < R; r += step) s[0] += p[r * ld];
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
 // out[g] = sum over the tile of the values of group g; acc: this thread's column sums.
-// FOLD: C/G is a multiple of V, so the thread's channels are one group's.
+// FOLD: C/G is a multiple of V, so the thread's channels are one group's and count as one column.
+// Rows first (as many stripes of them as there are threads), then the stripes, then the columns.
+// red: blockDim * V floats and blockDim + slab channels more.
 template <int V, bool FOLD>
 PG_DEVICE void group_sums(const Geo &g, const Place &p, const float (&acc)[V], float *red, float *out) {
-  const int t = threadIdx.x;
+  const int t = threadIdx.x, TH = blockDim.x;
+  const int ld = FOLD ? g.CVp : g.CVp * V, width = FOLD ? g.cg / V : g.cg, n = p.ng * width, nt = TH / n;
+  float *red2 = red + TH * V, *tot = red2 + TH;
   if (p.on) {
     if constexpr (FOLD) {
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) s += acc[j];
-      red[p.row * g.CVp + p.col] = s;
+      red[p.row * ld + p.col] = s;
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) red[(p.row * g.CVp + p.col) * V + j] = acc[j];
+      for (int j = 0; j < V; ++j) red[p.row * ld + p.col * V + j] = acc[j];
     }
   }
   __syncthreads();
-  const int width = FOLD ? g.cg / V : g.cg, pitch = FOLD ? g.CVp : g.CVp * V;
-  const int E = g.R * width, W = seg_width(E), per = 64 / W;
-  const int lane = t & 63, l = lane & (W - 1);
-  for (int gi = (t >> 6) * per + lane / W; gi - lane / W < p.ng; gi += (blockDim.x >> 6) * per) {
+  if (nt <= 1) {
+    for (int o = t; o < n; o += TH) tot[o] = col_sum(red + o, 0, g.R, 1, ld);
+  } else {
+    const int st = t / n, o = t - st * n;
+    if (st < nt) red2[st * n + o] = col_sum(red + o, st, g.R, nt, ld);
+    __syncthreads();
+    if (t < n) tot[t] = col_sum(red2 + t, 0, nt, 1, n);
+  }
+  __syncthreads();
+  const int W = seg_width(width), per = 64 / W, lane = t & 63, l = lane & (W - 1);
+  for (int i = (t >> 6) * per + lane / W; i - lane / W < p.ng; i += (TH >> 6) * per) {
     float s = 0.f;
-    if (gi < p.ng)
-      for (int e = l; e < E; e += W) s += red[e / width * pitch + gi * width + e % width];
+    if (i < p.ng)
+      for (int c = l; c < width; c += W) s += tot[i * width + c];
     s = seg_sum(s, W);
-    if (l == 0 && gi < p.ng) out[gi] = s;
+    if (l == 0 && i < p.ng) out[i] = s;
   }
   __syncthreads();
 }
@@ -233,11 +256,9 @@ template <int ACT> PG_DEVICE float gn_act(float z) {
 // of that), all of which come here
 template <class T, int V>
 PG_DEVICE void gn_checkpoint(const FwdArgs &a, const Place &p, const typename Vec<T, V>::raw &raw, long long r, bool ok) {
-  float f[V], m = 0.f;
+  float f[V], m;
   Vec<T, V>::unpack(raw, f);
-#pragma unroll
-  for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(f[j]));
-  m = p.on ? m : 0.f;
+  m = p.on ? mx8_amax(f) : 0.f;
 #pragma unroll
   for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const int e = mx8_exp(m);
@@ -533,18 +554,6 @@ template <bool SILU> PG_DEVICE float gn_dz(float dy, float x, float df, float u,
   } else {
     return x <= u || x >= v ? 0.f : dy;
   }
-}
-
-// sums of n columns over the rows r0, r0 + step, .. < R of a [R][ld] array, four at a time
-PG_DEVICE float col_sum(const float *p, int r0, int R, int step, int ld) {
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  int r = r0;
-  for (; r + 3 * step < R; r += 4 * step) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s[u] += p[(r + u * step) * ld];
-  }
-  for (; r < R; r += step) s[0] += p[r * ld];
-  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // Shared memory of a backward workgroup: what its channels need (gamma, rstd gamma, and gn_dz's u and

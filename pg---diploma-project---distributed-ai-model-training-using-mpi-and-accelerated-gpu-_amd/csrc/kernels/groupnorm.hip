@@ -134,8 +134,18 @@ __global__ __launch_bounds__(1024) void gn_dparam_kernel(const float *__restrict
   const int col = threadIdx.x & 63, st = threadIdx.x >> 6, j = blockIdx.x * 64 + col;
   const long long r0 = (long long)blockIdx.y * split, r1 = min(rows, r0 + split);
   float s = 0.f;
-  if (j < n)
-    for (long long r = r0 + st; r < r1; r += 16) s += part[r * n + j];
+  if (j < n) {   // eight rows in flight
+    float v[8] = {};
+    long long r = r0 + st;
+    for (; r + 7 * 16 < r1; r += 8 * 16) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] += part[(r + u * 16) * n + j];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[0] += r + u * 16 < r1 ? part[(r + u * 16) * n + j] : 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
   sh[st][col] = s;
   __syncthreads();
   if (st == 0 && j < n) {
@@ -168,8 +178,8 @@ int gcd_pow2(long long c, int most) {
 
 // the sums and rows that a workgroup holds in shared memory
 size_t gn_lds(const Plan &p, bool bwd) {
-  const size_t red = (size_t)p.TH * p.V;
-  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 * (size_t)p.g.cs + p.TH : 0) + red);
+  const size_t red = (size_t)p.TH * (p.V + 1);
+  return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 : 1) * (size_t)p.g.cs + red);
 }
 
 Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {

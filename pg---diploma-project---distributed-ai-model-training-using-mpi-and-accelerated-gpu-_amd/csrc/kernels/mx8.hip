@@ -58,11 +58,9 @@ __global__ __launch_bounds__(kThreads) void mx8_pack_kernel(const T *__restrict_
     uint32_t slot;
     s.at(u, f, row, slot);
     const bool ok = row < M && slot * V < (uint32_t)C;
-    float v[V], m = 0.f;
+    float v[V];
     X::unpack(d[u], v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(v[j]));
-    m = ok ? m : 0.f;
+    float m = ok ? mx8_amax(v) : 0.f;
 #pragma unroll
     for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
     const int e = mx8_exp(m);

@@ -206,9 +206,18 @@ PG_DEVICE bool pairs(const unsigned long long *src, int k, int l, int W, int pol
   for (int c0 = 0; c0 < k; c0 += 4 * W) {   // four loads in flight
     if (c0) pairs_ahead(src, k, l, W, c0, v);
     for (int i = 0;; ++i) {
-      if (!__any(v[0] == kNone || v[1] == kNone || v[2] == kNone || v[3] == kNone)) break;
+      const bool none = v[0] == kNone || v[1] == kNone || v[2] == kNone || v[3] == kNone;
+      const unsigned long long who = __ballot(none);
+      if (!who) break;
+      // One lane looks for its first missing pair until it comes, then all look again: with every lane
+      // looking, the waiting waves' reads held up those that were waited for (7 x 3249 x 100: 19 us,
+      // not 13).
+      if ((int)(threadIdx.x & 63) == __ffsll((long long)who) - 1) {
+        const int u = v[0] == kNone ? 0 : v[1] == kNone ? 1 : v[2] == kNone ? 2 : 3, ch = c0 + u * W + l;
+        for (; i < polls && pair_load(src + (ch < k ? ch : l < k ? l : 0)) == kNone; ++i) __builtin_amdgcn_s_sleep(16);
+      }
+      i = __builtin_amdgcn_readlane(i, __ffsll((long long)who) - 1);
       if (i >= polls) return false;
-      __builtin_amdgcn_s_sleep(4);
       pairs_ahead(src, k, l, W, c0, v);
     }
 #pragma unroll
@@ -256,12 +265,9 @@ template <int ACT> PG_DEVICE float gn_act(float z) {
 // of that), all of which come here
 template <class T, int V>
 PG_DEVICE void gn_checkpoint(const FwdArgs &a, const Place &p, const typename Vec<T, V>::raw &raw, long long r, bool ok) {
-  float f[V], m;
+  float f[V];
   Vec<T, V>::unpack(raw, f);
-  m = p.on ? mx8_amax(f) : 0.f;
-#pragma unroll
-  for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const int e = mx8_exp(m);
+  const int e = mx8_exp(block_amax<T, V>(raw, p.on));
   if (ok) {
     *reinterpret_cast<typename Codes<V>::raw *>(a.q + r * a.g.C + p.c) = Codes<V>::encode(f, mx8_inv_scale(e));
     if (p.c % kMxBlock == 0) a.qs[r * ((a.g.C + kMxBlock - 1) / kMxBlock) + p.c / kMxBlock] = (uint8_t)e;
@@ -400,9 +406,9 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) d[u] = at<typename X::raw>(src, min(first + (round * U + u) * hop, last));
   };
-  // where the tiles are joined: W lanes a group, the first group's pairs on their way
+  // where the tiles are joined: W lanes a group, 4 pairs a lane, the first group's on their way
   const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  const int W = seg_width((g.k + 3) / 4), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
   const int i0 = (threadIdx.x >> 6) * per + lane / W;
   unsigned long long pv[4];
   if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
@@ -535,7 +541,7 @@ PG_DEVICE void gn_border(int act, float mean, float rstd, float gamma, float bet
     if (!(beta > 0.f) || (act == GN_RELU6 && !(beta < 6.f))) lo = INFINITY;
     return;
   }
-  const double t0 = (double)mean - b / k, t6 = (double)mean + (6.0 - b) / k;
+  const double r = 1.0 / k, t0 = fma(-b, r, (double)mean), t6 = fma(6.0 - b, r, (double)mean);
   if (k > 0.0) {
     lo = __double2float_rd(t0);
     if (act == GN_RELU6) hi = __double2float_ru(t6);
@@ -562,7 +568,7 @@ struct BwdShared {
   float *ga, *al, *u, *v, *tot, *g1, *g2, *red2, *red;
   PG_DEVICE BwdShared(const Geo &g, float *sm)
       : ga(sm), al(ga + g.cs), u(al + g.cs), v(u + g.cs), tot(v + g.cs), g1(tot + 2 * g.cs), g2(g1 + g.gs),
-        red2(g2 + g.gs), red(red2 + blockDim.x) {}
+        red2(g2 + g.gs), red(red2 + 2 * blockDim.x) {}
   // one channel's values: asked for early, put down when they are here
   struct Channel { float ga[1], be[1], mean, rstd; };
   static PG_DEVICE void ask(const BwdArgs &a, const Place &p, const float *mean, const float *rstd, int c, Channel &k) {
@@ -648,29 +654,32 @@ PG_DEVICE void bwd_sums(const BwdArgs &a, const Place &p, const float *rstd, con
   const Geo &g = a.g;
   const int ld = g.CVp * V, t = threadIdx.x, n = p.csl, nt = blockDim.x / n;
   const float rs = at<float>(rstd, min(t, n - 1) / g.cg * 4u);
+  float *redb = m.red + blockDim.x * V;
+  if (p.on) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (p.on) {
+    for (int j = 0; j < V; ++j) m.red[p.row * ld + p.col * V + j] = s1[j];
 #pragma unroll
-      for (int j = 0; j < V; ++j) m.red[p.row * ld + p.col * V + j] = h ? s0[j] : s1[j];
-    }
-    __syncthreads();
-    if (nt <= 1) {
-      for (int o = t; o < n; o += blockDim.x) {
-        const float s = col_sum(m.red + o, 0, g.R, 1, ld);
-        m.tot[h * g.cs + o] = h ? s : s * (o == t ? rs : rstd[o / g.cg]);
-      }
-    } else {   // nt stripes of rows a channel
-      const int st = t / n, o = t - st * n;
-      if (st < nt) m.red2[st * n + o] = col_sum(m.red + o, st, g.R, nt, ld);
-      __syncthreads();
-      if (t < n) {
-        const float s = col_sum(m.red2 + t, 0, nt, 1, n);
-        m.tot[h * g.cs + t] = h ? s : s * rs;
-      }
-    }
-    __syncthreads();
+    for (int j = 0; j < V; ++j) redb[p.row * ld + p.col * V + j] = s0[j];
   }
+  __syncthreads();
+  if (nt <= 1) {
+    for (int o = t; o < n; o += blockDim.x) {
+      m.tot[o] = col_sum(m.red + o, 0, g.R, 1, ld) * (o == t ? rs : rstd[o / g.cg]);
+      m.tot[g.cs + o] = col_sum(redb + o, 0, g.R, 1, ld);
+    }
+  } else {   // nt stripes of rows a channel
+    const int st = t / n, o = t - st * n;
+    if (st < nt) {
+      m.red2[st * n + o] = col_sum(m.red + o, st, g.R, nt, ld);
+      m.red2[blockDim.x + st * n + o] = col_sum(redb + o, st, g.R, nt, ld);
+    }
+    __syncthreads();
+    if (t < n) {
+      m.tot[t] = col_sum(m.red2 + t, 0, nt, 1, n) * rs;
+      m.tot[g.cs + t] = col_sum(m.red2 + blockDim.x + t, 0, nt, 1, n);
+    }
+  }
+  __syncthreads();
   if (a.dpart) {
     float *dst = a.dpart + (p.b * g.k + p.chunk) * 2 * g.C + p.c0;
     for (int j = t; j < n; j += blockDim.x) {
@@ -793,9 +802,9 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
     for (int u = 0; u < U; ++u)
       Th::load(a, r0, min(first + (round * U + u) * hop, last), CK ? min(firsts + (round * U + u) * hops, lasts) : 0, d[u]);
   };
-  // where the tiles are joined: W lanes a group, the first group's pairs on their way
+  // where the tiles are joined: W lanes a group, 4 pairs a lane, the first group's on their way
   const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width(g.k), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
+  const int W = seg_width((g.k + 3) / 4), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
   const int i0 = (threadIdx.x >> 6) * per + lane / W;
   unsigned long long pv[4];
   if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);

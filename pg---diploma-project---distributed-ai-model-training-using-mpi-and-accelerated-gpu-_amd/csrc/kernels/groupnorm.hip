@@ -178,7 +178,7 @@ int gcd_pow2(long long c, int most) {
 
 // the sums and rows that a workgroup holds in shared memory
 size_t gn_lds(const Plan &p, bool bwd) {
-  const size_t red = (size_t)p.TH * (p.V + 1);
+  const size_t red = (size_t)p.TH * (p.V + 1) * (bwd ? 2 : 1);
   return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 : 1) * (size_t)p.g.cs + red);
 }
 

@@ -60,10 +60,7 @@ __global__ __launch_bounds__(kThreads) void mx8_pack_kernel(const T *__restrict_
     const bool ok = row < M && slot * V < (uint32_t)C;
     float v[V];
     X::unpack(d[u], v);
-    float m = ok ? mx8_amax(v) : 0.f;
-#pragma unroll
-    for (int o = 1; o < kMxBlock / V; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const int e = mx8_exp(m);
+    const int e = mx8_exp(block_amax<T, V>(d[u], ok));
     if (ok) {
       *reinterpret_cast<typename Codes<V>::raw *>(q + row * C + slot * V) = Codes<V>::encode(v, mx8_inv_scale(e));
       if (slot % (kMxBlock / V) == 0) qs[row * nb + slot / (kMxBlock / V)] = (uint8_t)e;

@@ -34,18 +34,6 @@ PG_DEVICE int mx8_exp(float amax) {
 PG_DEVICE float mx8_scale(int byte) { return __uint_as_float((uint32_t)byte << 23); }            // 2^e
 PG_DEVICE float mx8_inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }   // 2^-e
 
-// the largest finite magnitude of V values (fmaxf drops a NaN; infinities take the long way)
-template <int V> PG_DEVICE float mx8_amax(const float (&v)[V]) {
-  float m = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) m = fmaxf(m, fabsf(v[j]));
-  if (m == INFINITY) {
-    m = 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) m = fmaxf(m, mx8_mag(v[j]));
-  }
-  return m;
-}
 // two values (already times 2^-e: 448 at most, or not finite) -> two codes in the low or high half of
 // w; the conversion gives NaN for infinities
 template <bool HI> PG_DEVICE int mx8_enc2(float a, float b, int w) { return __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, HI); }

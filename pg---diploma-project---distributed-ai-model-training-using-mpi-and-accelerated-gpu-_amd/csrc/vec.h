@@ -69,3 +69,45 @@ template <int V> struct Codes {
   }
 };
 
+// The largest finite magnitude of a 32-channel block, whose 32 / V neighbouring lanes (aligned) hold V
+// channels each; lanes without `on` count as zeros.  Magnitudes are compared as whole numbers, two
+// 16-bit ones an instruction; non-finite ones, the largest of all, take the long way.
+template <class T, int V> PG_DEVICE float block_amax(const typename Vec<T, V>::raw &raw, bool on) {
+  uint32_t m = 0;   // bits of the largest magnitude
+  constexpr uint32_t inf = sizeof(T) == 4 || __is_same(T, bf16_t) ? 0x7f800000u : 0x7c000000u;   // 16-bit: in the high half
+  if constexpr (sizeof(T) == 2 && V >= 2) {
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+    struct alignas(sizeof(raw)) Words { uint32_t w[V / 2]; };
+    const Words a = __builtin_bit_cast(Words, raw);
+    u16x2_t x = __builtin_bit_cast(u16x2_t, a.w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int j = 1; j < V / 2; ++j) x = __builtin_elementwise_max(x, __builtin_bit_cast(u16x2_t, a.w[j] & 0x7fff7fffu));
+    m = (uint32_t)(x.x > x.y ? x.x : x.y) << 16;
+  } else if constexpr (sizeof(T) == 2) {
+    m = ((uint32_t)__builtin_bit_cast(uint16_t, raw) & 0x7fffu) << 16;
+  } else {
+    struct alignas(sizeof(raw)) Words { uint32_t w[V]; };
+    const Words a = __builtin_bit_cast(Words, raw);
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max(m, a.w[j] & 0x7fffffffu);
+  }
+  if (m >= inf) {
+    m = 0;
+    float f[V];
+    Vec<T, V>::unpack(raw, f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const T t = fromf<T>(mx8_mag(f[j]));
+      if constexpr (sizeof(T) == 4) m = max(m, __builtin_bit_cast(uint32_t, t));
+      else m = max(m, (uint32_t)__builtin_bit_cast(uint16_t, t) << 16);
+    }
+  }
+  m = on ? m : 0;
+  // neighbours 1 and 2 apart within a quad, then further
+  if constexpr (kMxBlock / V > 1) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp((int)m, (int)m, 0xB1, 0xf, 0xf, false));
+  if constexpr (kMxBlock / V > 2) m = max(m, (uint32_t)__builtin_amdgcn_update_dpp((int)m, (int)m, 0x4E, 0xf, 0xf, false));
+#pragma unroll
+  for (int o = 4; o < kMxBlock / V; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  if constexpr (sizeof(T) == 4 || __is_same(T, bf16_t)) return __uint_as_float(m);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)(m >> 16));
+}

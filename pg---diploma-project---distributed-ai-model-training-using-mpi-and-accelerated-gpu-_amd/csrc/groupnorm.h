@@ -7,15 +7,17 @@
 //
 // Both are bound by memory.  What reads a tile twice is kept close to where it was read first:
 //   solo     a workgroup holds all S rows of a slab of whole groups in registers: one read
+//   held     the S rows are k tiles, and all tiles of the tensor are so few that their workgroups run
+//            together: each keeps its tile in registers, publishes its sums, waits for the k - 1
+//            others of its image and goes on.  One read.  (With more tiles than fit, a workgroup's
+//            chain load - sum - publish - wait - join - store is not hidden behind others':
+//            128 x 12544 x 96 backward took 1129 us.)
 //   staged   longer maps: the S rows are k tiles.  One launch holds a sums and a use workgroup for
 //            every tile; the use of an image's tiles is queued `lead` images behind its sums, so
 //            that it hardly ever waits for them and finds the tile in the memory-side cache
 //            (256 MB).  HBM sees every value once.
 //   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
 //            one workgroup per (image, group), then one value a thread.
-// (Holding the tiles in registers while the k workgroups of an image exchange their sums also reads
-// once, but the chain load - sum - publish - wait - join - store of one workgroup is some 60 us and
-// only two of them fit a CU: 128 x 12544 x 96 backward took 1129 us.)
 // A thread owns one vector of V channels (16 bytes where C allows) and every R-th row of the tile.
 // Sums are taken in a fixed order, so results do not vary from run to run.
 #pragma once
@@ -27,7 +29,7 @@
 
 namespace gn {
 enum GnAct : int { GN_NONE = 0, GN_RELU = 1, GN_RELU6 = 2, GN_SILU = 3 };
-enum GnMode : int { SOLO = 0, STAGED = 1, WIDE = 2 };
+enum GnMode : int { SOLO = 0, HELD = 1, STAGED = 2, WIDE = 3 };
 
 // ---- tile geometry ---------------------------------------------------------------------------
 struct Geo {
@@ -309,21 +311,64 @@ PG_DEVICE void fwd_statistics(const FwdArgs &a, const Place &p, const float *gm,
     }
 }
 
-// solo: the rows stay in NV registers a thread between the mean, the squares about it and y
-template <class T, int V, int NV, bool CK, bool FOLD>
+// where the tiles are joined: W lanes a group, 4 pairs a lane
+struct JoinLanes {
+  const unsigned long long *in;
+  int W, per, lane, l, i0;
+  PG_DEVICE JoinLanes(const Geo &g, const Place &p, const unsigned long long *part)
+      : in(part + p.unit * g.k * g.gs), W(seg_width((g.k + 3) / 4)), per(64 / W), lane(threadIdx.x & 63),
+        l(lane & (W - 1)), i0((threadIdx.x >> 6) * per + lane / W) {}
+  // the first group's pairs on their way
+  PG_DEVICE void ahead(const Geo &g, const Place &p, unsigned long long (&v)[4]) const {
+    pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, v);
+  }
+};
+
+// gm, gr = mean, rstd of the unit's groups
+template <class T>
+PG_DEVICE void fwd_join(const FwdArgs &a, const Place &p, const JoinLanes &q, unsigned long long (&pv)[4], float *gm, float *gr) {
+  const Geo &g = a.g;
+  for (int i = q.i0; i - q.lane / q.W < p.ng; i += (blockDim.x >> 6) * q.per) {
+    Moments t{0.f, 0.f, 0.f};
+    const int gc = min(i, p.ng - 1);
+    const unsigned long long *in = q.in + (long long)gc * g.k;
+    if (i != q.i0) pairs_ahead(in, g.k, q.l, q.W, 0, pv);
+    if (!pairs(in, g.k, q.l, q.W, g.wait, pv, [&](int ch, float m, float v) {
+          t.join((float)min((long long)g.rows, g.S - (long long)ch * g.rows) * (float)g.cg, m, v);
+        })) {
+      // without the peers: every W-th row of the group, from the tensor
+      const T *base = static_cast<const T *>(a.x) + p.b * g.S * g.C + p.c0 + gc * g.cg;
+      t = Moments{0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (long long r = q.l; r < g.S; r += q.W)
+#pragma unroll 1
+        for (int c = 0; c < g.cg; ++c) t.join(1.f, tof(base[r * g.C + c]), 0.f);
+    }
+    for (int o = 1; o < q.W; o <<= 1) t.join(__shfl_xor(t.n, o, 64), __shfl_xor(t.m, o, 64), __shfl_xor(t.v, o, 64));
+    if (q.l == 0 && i < p.ng) {
+      gm[i] = t.m;
+      gr[i] = 1.f / sqrtf(t.v / t.n + a.eps);
+    }
+  }
+  __syncthreads();
+}
+
+// solo, held: the rows stay in NV registers a thread between the mean, the squares about it and y
+template <class T, int V, int NV, int MODE, bool CK, bool FOLD>
 __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   const Geo &g = a.g;
-  const Place p = place<V, SOLO>(g);
+  const Place p = place<V, MODE>(g);
   float *gm = sm, *gr = sm + g.gs, *red = sm + 2 * g.gs;
   constexpr int VG = FOLD ? 1 : V;
   int gi[VG];   // slab group of each channel (FOLD: of all)
 #pragma unroll
   for (int j = 0; j < VG; ++j) gi[j] = (p.c - p.c0 + j) / g.cg;
-  const int nr = (int)g.S;
-  const T *src = static_cast<const T *>(a.x) + p.b * g.S * g.C;
-  T *dst = static_cast<T *>(a.y) + p.b * g.S * g.C;
+  const long long s0 = MODE == HELD ? (long long)p.chunk * g.rows : 0, r0 = p.b * g.S + s0;
+  const int nr = (int)(MODE == HELD ? min((long long)g.rows, g.S - s0) : g.S);
+  const T *src = static_cast<const T *>(a.x) + r0 * g.C;
+  T *dst = static_cast<T *>(a.y) + r0 * g.C;
   // rows past the end (and threads without a column) read a row that exists and are masked
   typename X::raw d[NV];
 #pragma unroll
@@ -345,7 +390,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
       for (int j = 0; j < V; ++j) acc[j] += f[j];
     }
   group_sums<V, FOLD>(g, p, acc, red, gm);
-  const float n = (float)g.S * (float)g.cg;
+  const float n = (float)nr * (float)g.cg;
 #pragma unroll
   for (int j = 0; j < VG; ++j) mu[j] = gm[gi[j]] / n;
 #pragma unroll
@@ -366,11 +411,20 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
   if constexpr (CK) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      gn_checkpoint<T, V>(a, p, d[i], p.b * g.S + p.row + i * g.R, p.on && p.row + i * g.R < nr);
+      gn_checkpoint<T, V>(a, p, d[i], r0 + p.row + i * g.R, p.on && p.row + i * g.R < nr);
   }
   group_sums<V, FOLD>(g, p, acc, red, gr);
-  for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
-  __syncthreads();
+  if constexpr (MODE == HELD) {
+    const JoinLanes jl(g, p, a.part);
+    unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk, pv[4];
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, gm[i], gr[i]);
+    __syncthreads();   // gm and gr have been read
+    jl.ahead(g, p, pv);
+    fwd_join<T>(a, p, jl, pv, gm, gr);
+  } else {
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) gr[i] = 1.f / sqrtf(gr[i] / n + a.eps);
+    __syncthreads();
+  }
   fwd_statistics(a, p, gm, gr);
   if (!p.on) return;
   fwd_constants<V, VG>(gi, gm, gr, mu, sc);
@@ -406,12 +460,9 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) d[u] = at<typename X::raw>(src, min(first + (round * U + u) * hop, last));
   };
-  // where the tiles are joined: W lanes a group, 4 pairs a lane, the first group's on their way
-  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width((g.k + 3) / 4), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-  const int i0 = (threadIdx.x >> 6) * per + lane / W;
+  const JoinLanes jl(g, p, a.part);
   unsigned long long pv[4];
-  if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
+  if (p.use) jl.ahead(g, p, pv);
   typename X::raw d[U], nx[U];
   load(d, 0);
   auto stream = [&](auto f) {
@@ -482,28 +533,7 @@ __global__ __launch_bounds__(512) void gn_fwd_staged_kernel(const FwdArgs a) {
   float mu[VG], sc[V], be[V];
   channel_values(a.gamma, a.mean, p.c, 1.f, sc);
   channel_values(a.beta, a.mean, p.c, 0.f, be);
-  for (int i = i0; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-    Moments t{0.f, 0.f, 0.f};
-    const int gc = min(i, p.ng - 1);
-    if (i != i0) pairs_ahead(in + (long long)gc * g.k, g.k, l, W, 0, pv);
-    if (!pairs(in + (long long)gc * g.k, g.k, l, W, g.wait, pv, [&](int ch, float m, float v) {
-          t.join((float)min((long long)g.rows, g.S - (long long)ch * g.rows) * (float)g.cg, m, v);
-        })) {
-      // without the peers: every W-th row of the group, from the tensor
-      const T *base = static_cast<const T *>(a.x) + p.b * g.S * g.C + p.c0 + gc * g.cg;
-      t = Moments{0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (long long r = l; r < g.S; r += W)
-#pragma unroll 1
-        for (int c = 0; c < g.cg; ++c) t.join(1.f, tof(base[r * g.C + c]), 0.f);
-    }
-    for (int o = 1; o < W; o <<= 1) t.join(__shfl_xor(t.n, o, 64), __shfl_xor(t.m, o, 64), __shfl_xor(t.v, o, 64));
-    if (l == 0 && i < p.ng) {
-      gm[i] = t.m;
-      gr[i] = 1.f / sqrtf(t.v / t.n + a.eps);
-    }
-  }
-  __syncthreads();
+  fwd_join<T>(a, p, jl, pv, gm, gr);
   fwd_statistics(a, p, gm, gr);
   if (!p.on) return;
   fwd_constants<V, VG>(gi, gm, gr, mu, sc);
@@ -727,17 +757,58 @@ PG_DEVICE void bwd_constants(const Geo &g, const Place &p, const float (&rs)[VG]
   for (int j = 0; j < V; ++j) al[j] = m.al[p.c - p.c0 + j];
 }
 
-template <class T, int V, int NV, bool CK, bool FOLD, bool SILU>
+// g1, g2 = s1, s2 of the unit's groups
+template <class T, bool CK, bool SILU>
+PG_DEVICE void bwd_join(const BwdArgs &a, const Place &p, const float *mean, const float *rstd, const JoinLanes &q,
+                        unsigned long long (&pv)[4], const BwdShared &m) {
+  const Geo &g = a.g;
+  for (int i = q.i0; i - q.lane / q.W < p.ng; i += (blockDim.x >> 6) * q.per) {
+    float u = 0.f, v = 0.f;
+    const int gc = min(i, p.ng - 1);
+    const unsigned long long *in = q.in + (long long)gc * g.k;
+    if (i != q.i0) pairs_ahead(in, g.k, q.l, q.W, 0, pv);
+    if (!pairs(in, g.k, q.l, q.W, g.wait, pv, [&](int, float s1, float s2) {
+          u += s1;
+          v += s2;
+        })) {   // as in the forward
+      u = v = 0.f;
+      const int nb = (g.C + kMxBlock - 1) / kMxBlock;
+      const float mu = mean[gc], rs = rstd[gc];
+#pragma unroll 1
+      for (long long r = p.b * g.S + q.l; r < (p.b + 1) * g.S; r += q.W)
+#pragma unroll 1
+        for (int c = gc * g.cg; c < (gc + 1) * g.cg; ++c) {
+          const long long at = r * g.C + p.c0 + c;
+          float x;
+          if constexpr (CK) x = mx8_dec1(a.q[at]) * mx8_scale(a.qs[r * nb + (p.c0 + c) / kMxBlock]);
+          else x = tof(static_cast<const T *>(a.x)[at]);
+          const float z = gn_dz<SILU>(tof(static_cast<const T *>(a.dy)[at]), x, x - mu, m.u[c], m.v[c]);
+          u = fmaf(m.ga[c], z, u);
+          v = fmaf(m.ga[c] * rs * (x - mu), z, v);
+        }
+    }
+    u = seg_sum(u, q.W);
+    v = seg_sum(v, q.W);
+    if (q.l == 0 && i < p.ng) {
+      m.g1[i] = u;
+      m.g2[i] = v;
+    }
+  }
+  __syncthreads();
+}
+
+// solo, held: as in the forward
+template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU>
 __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
   extern __shared__ float sm[];
   typedef Vec<T, V> X;
   typedef BwdThread<T, V, CK, FOLD, SILU> Th;
   const Geo &g = a.g;
-  const Place p = place<V, SOLO>(g);
+  const Place p = place<V, MODE>(g);
   const BwdShared m(g, sm);
   const float *mean = a.mean + p.b * g.G + p.g0, *rstd = a.rstd + p.b * g.G + p.g0;
-  const int nr = (int)g.S;
-  const long long r0 = p.b * g.S;
+  const long long s0 = MODE == HELD ? (long long)p.chunk * g.rows : 0, r0 = p.b * g.S + s0;
+  const int nr = (int)(MODE == HELD ? min((long long)g.rows, g.S - s0) : g.S);
   Th th;
   BwdShared::Channel own;
   th.groups(g, p, mean, rstd);
@@ -750,9 +821,9 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
   }
   m.put<SILU>(a, p, mean, rstd, own);
   th.channels(p, m);
-  float s0[V], s1[V];
+  float s1[V], s2[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
+  for (int j = 0; j < V; ++j) s1[j] = s2[j] = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (p.row + i * g.R < nr) {
@@ -762,10 +833,18 @@ __global__ __launch_bounds__(1024) void gn_bwd_solo_kernel(const BwdArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         s1[j] = fmaf(dz[j], df[j], s1[j]);
-        s0[j] += dz[j];
+        s2[j] += dz[j];
       }
     }
-  bwd_sums<V>(a, p, rstd, s1, s0, m);
+  bwd_sums<V>(a, p, rstd, s1, s2, m);
+  if constexpr (MODE == HELD) {
+    const JoinLanes jl(g, p, a.part);
+    unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk, pv[4];
+    for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, m.g1[i], m.g2[i]);
+    __syncthreads();   // g1 and g2 have been read
+    jl.ahead(g, p, pv);
+    bwd_join<T, CK, SILU>(a, p, mean, rstd, jl, pv, m);
+  }
   if (!p.on) return;
   float al[V], k1[Th::VG], k2[Th::VG];
   bwd_constants<V, Th::VG>(g, p, th.rs, th.gi, m, al, k1, k2);
@@ -802,12 +881,9 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
     for (int u = 0; u < U; ++u)
       Th::load(a, r0, min(first + (round * U + u) * hop, last), CK ? min(firsts + (round * U + u) * hops, lasts) : 0, d[u]);
   };
-  // where the tiles are joined: W lanes a group, 4 pairs a lane, the first group's on their way
-  const unsigned long long *in = a.part + p.unit * g.k * g.gs;
-  const int W = seg_width((g.k + 3) / 4), per = 64 / W, lane = threadIdx.x & 63, l = lane & (W - 1);
-  const int i0 = (threadIdx.x >> 6) * per + lane / W;
+  const JoinLanes jl(g, p, a.part);
   unsigned long long pv[4];
-  if (p.use) pairs_ahead(in + (long long)min(i0, p.ng - 1) * g.k, g.k, l, W, 0, pv);
+  if (p.use) jl.ahead(g, p, pv);
   Th th;
   BwdShared::Channel own;
   th.groups(g, p, mean, rstd);
@@ -854,37 +930,7 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
     for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, m.g1[i], m.g2[i]);
     return;
   }
-  for (int i = i0; i - lane / W < p.ng; i += (blockDim.x >> 6) * per) {
-    float u = 0.f, v = 0.f;
-    const int gc = min(i, p.ng - 1);
-    if (i != i0) pairs_ahead(in + (long long)gc * g.k, g.k, l, W, 0, pv);
-    if (!pairs(in + (long long)gc * g.k, g.k, l, W, g.wait, pv, [&](int, float s1, float s2) {
-          u += s1;
-          v += s2;
-        })) {   // as in the forward
-      u = v = 0.f;
-      const float mu = mean[gc], rs = rstd[gc];
-#pragma unroll 1
-      for (long long r = p.b * g.S + l; r < (p.b + 1) * g.S; r += W)
-#pragma unroll 1
-        for (int c = gc * g.cg; c < (gc + 1) * g.cg; ++c) {
-          const long long at = r * g.C + p.c0 + c;
-          float x;
-          if constexpr (CK) x = mx8_dec1(a.q[at]) * mx8_scale(a.qs[r * nb + (p.c0 + c) / kMxBlock]);
-          else x = tof(static_cast<const T *>(a.x)[at]);
-          const float z = gn_dz<SILU>(tof(static_cast<const T *>(a.dy)[at]), x, x - mu, m.u[c], m.v[c]);
-          u = fmaf(m.ga[c], z, u);
-          v = fmaf(m.ga[c] * rs * (x - mu), z, v);
-        }
-    }
-    u = seg_sum(u, W);
-    v = seg_sum(v, W);
-    if (l == 0 && i < p.ng) {
-      m.g1[i] = u;
-      m.g2[i] = v;
-    }
-  }
-  __syncthreads();
+  bwd_join<T, CK, SILU>(a, p, mean, rstd, jl, pv, m);
   if (!p.on) return;
   float al[V], k1[Th::VG], k2[Th::VG];
   bwd_constants<V, Th::VG>(g, p, th.rs, th.gi, m, al, k1, k2);
@@ -903,8 +949,8 @@ struct Plan {
 
 struct Fwd {
   typedef FwdArgs Args;
-  template <class T, int V, int NV, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
-    return gn_fwd_solo_kernel<T, V, NV, CK, FOLD>;
+  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
+    return gn_fwd_solo_kernel<T, V, NV, MODE, CK, FOLD>;
   }
   template <class T, int V, bool CK, bool FOLD, bool SILU> static constexpr auto staged() {
     return gn_fwd_staged_kernel<T, V, CK, FOLD>;
@@ -912,17 +958,17 @@ struct Fwd {
 };
 struct Bwd {
   typedef BwdArgs Args;
-  template <class T, int V, int NV, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
-    return gn_bwd_solo_kernel<T, V, NV, CK, FOLD, SILU>;
+  template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
+    return gn_bwd_solo_kernel<T, V, NV, MODE, CK, FOLD, SILU>;
   }
   template <class T, int V, bool CK, bool FOLD, bool SILU> static constexpr auto staged() {
     return gn_bwd_staged_kernel<T, V, CK, FOLD, SILU>;
   }
 };
 
-// the plan gives NV 2, 4 (forward: 8) to full vectors of one group each, 2 to full vectors that
-// straddle groups (their constants take the registers), 4 to narrower ones
-template <class D, class T, int VMAX, int MOST, bool CK, bool SILU>
+// the plan gives NV 2, 4, 8 to full vectors of one group each, 2 to vectors of 8 that straddle groups
+// (their constants take the registers), 4 to narrower ones
+template <class D, class T, int VMAX, bool CK, bool SILU>
 void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)p.wgs), dim3(p.TH), lds, st, a); };
   const bool full = p.V == VMAX, fold = full && p.g.cg % VMAX == 0;
@@ -934,13 +980,18 @@ void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st
     else go(D::template staged<T, 1, CK, false, SILU>());
     return;
   }
-  if (fold && p.NV == 2) go(D::template solo<T, VMAX, 2, CK, true, SILU>());
-  else if (fold && p.NV == 4) go(D::template solo<T, VMAX, 4, CK, true, SILU>());
-  else if (fold) go(D::template solo<T, VMAX, MOST, CK, true, SILU>());
-  else if (full) go(D::template solo<T, VMAX, 2, CK, false, SILU>());
-  else if (VMAX == 8 && p.V == 4) go(D::template solo<T, 4, 4, CK, false, SILU>());
-  else if (p.V == 2) go(D::template solo<T, 2, 4, CK, false, SILU>());
-  else go(D::template solo<T, 1, 4, CK, false, SILU>());
+  auto solo = [&](auto mode) {
+    constexpr int M = decltype(mode)::value;
+    if (fold && p.NV == 2) go(D::template solo<T, VMAX, 2, M, CK, true, SILU>());
+    else if (fold && p.NV == 4) go(D::template solo<T, VMAX, 4, M, CK, true, SILU>());
+    else if (fold) go(D::template solo<T, VMAX, 8, M, CK, true, SILU>());
+    else if (full) go(D::template solo<T, VMAX, VMAX == 4 ? 4 : 2, M, CK, false, SILU>());
+    else if (VMAX == 8 && p.V == 4) go(D::template solo<T, 4, 4, M, CK, false, SILU>());
+    else if (p.V == 2) go(D::template solo<T, 2, 4, M, CK, false, SILU>());
+    else go(D::template solo<T, 1, 4, M, CK, false, SILU>());
+  };
+  if (p.mode == SOLO) solo(std::integral_constant<int, SOLO>());
+  else solo(std::integral_constant<int, HELD>());
 }
 
 // one translation unit per direction and type

@@ -162,6 +162,7 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
+constexpr int kHeld = 480;    // tiles that wait for one another: two of 512 threads are resident on each of 256 CUs
 constexpr int kTiles = 512;   // tiles wanted before tiles grow (2048: gn_bwd 96 x 784 x 192 98 us, not 43)
 constexpr int kRounds = 6;    // rounds of a tile at most (2, 4, 8, 16: gn_bwd 128 x 12544 x 96 360, 260, 265, 314 us)
 // sums workgroups ahead of the use workgroups at least: half of what is resident (128, 256, 384, 1024:
@@ -194,7 +195,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   const int elt = dt == 2 ? 4 : 2;
   const int V = gcd_pow2(C, 16 / elt);
   p.V = V;
-  const int only = V * elt < 16 ? 4 : g.cg % V ? 2 : 0;   // NV of the kinds of vector that have one
+  const int only = V * elt < 16 ? 4 : g.cg % V ? (elt == 4 ? 4 : 2) : 0;   // NV of the kinds of vector that have one
   const int Q = ck && !bwd ? kMxBlock / V : 1;   // lanes of a checkpoint block
   // a slab is made of whole groups, vectors and (where they are written) checkpoint blocks
   long long L = std::lcm<long long>(g.cg, V);
@@ -237,13 +238,32 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     }
   }
   // whole rows where they fit a workgroup, the fewest slabs otherwise
-  p.TH = bwd ? 256 : 512;
-  for (long long slabs = 1;; ++slabs) {
-    cs = ((C + slabs - 1) / slabs + L - 1) / L * L;
-    shape(cs);
-    if (g.CVp <= p.TH || cs == L) break;
+  auto slabs = [&](int th) {
+    p.TH = th;
+    for (long long n = 1;; ++n) {
+      cs = ((C + n - 1) / n + L - 1) / L * L;
+      shape(cs);
+      if (g.CVp <= th || cs == L) break;
+    }
+    g.R = th / std::max(g.CVp, 1);
+    return g.CVp <= th && gn_lds(p, bwd) <= 65536;
+  };
+  // held: the fewest rows a thread with which all tiles are resident together
+  if (slabs(512)) {
+    for (int nv : nvs) {
+      if (only && nv != only) continue;
+      const long long rows = (long long)g.R * nv, k = (S + rows - 1) / rows;
+      if (B * g.nslab * k > kHeld) continue;
+      p.NV = nv;
+      g.rows = (int)rows;
+      g.k = (int)k;
+      p.mode = HELD;
+      p.wgs = B * g.nslab * k;
+      check(k);
+      return p;
+    }
   }
-  if (g.CVp > p.TH || gn_lds(p, bwd) > 65536) {
+  if (!slabs(bwd ? 256 : 512)) {
     p.mode = WIDE;
     g.k = 1;
     g.nslab = G;   // sums per (image, group)
@@ -251,7 +271,6 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     p.wgs = B * G;
     return p;
   }
-  g.R = p.TH / g.CVp;
   // tiles of up to kRounds rounds, fewer while the tiles do not fill the chip several times
   const long long round = (long long)g.R * (bwd ? 2 : 4), all = (S + round - 1) / round;
   const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, kRounds);
@@ -289,7 +308,7 @@ Ws gn_ws(const Plan &p, bool bwd) {
 }
 
 void gn_none(const Plan &p, unsigned long long *part, hipStream_t st) {
-  if (p.mode != STAGED) return;
+  if (p.mode != STAGED && p.mode != HELD) return;
   const long long n = p.g.B * p.g.nslab * p.g.k * p.g.gs;
   hipLaunchKernelGGL(gn_none_kernel, dim3((unsigned)std::min<long long>((n + 255) / 256, 2048)), dim3(256), 0, st, part, n);
 }

@@ -208,7 +208,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     g.CVp = (g.cs / V + Q - 1) / Q * Q;
   };
   auto check = [&](long long k) {   // grid and in-tile offsets
-    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)std::max(g.rows, g.R * p.NV) * C * elt > 0x7fffffff)
+    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)std::max(g.turn, g.R * p.NV) * C * elt > 0x7fffffff)
       throw std::invalid_argument("group norm: sizes past the kernels' 32-bit grid and tile offsets");
   };
   const int most = bwd ? 512 : 1024;
@@ -276,7 +276,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, kRounds);
   const long long k = (all + it - 1) / it;
   p.NV = 1;
-  g.rows = (int)(round * it);
+  g.turn = (int)round;
   g.k = (int)k;
   p.mode = STAGED;
   g.tiles = (int)std::min<long long>(B * g.nslab * k, 0x7fffffff);

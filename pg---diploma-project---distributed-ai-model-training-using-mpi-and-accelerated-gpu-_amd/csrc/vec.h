@@ -91,7 +91,7 @@ template <class T, int V> PG_DEVICE float block_amax(const typename Vec<T, V>::r
 #pragma unroll
     for (int j = 0; j < V; ++j) m = max(m, a.w[j] & 0x7fffffffu);
   }
-  if (m >= inf) {
+  if (__ballot(m >= inf)) {   // one branch for the wave
     m = 0;
     float f[V];
     Vec<T, V>::unpack(raw, f);

@@ -264,6 +264,13 @@ template <int ACT> PG_DEVICE float gn_act(float z) {
   else return z;
 }
 
+// a store through a buffer descriptor: offset kOOB drops it, without a branch around it
+PG_DEVICE void buf_store(rsrc_t r, uint32_t o, const uint4 &v) { bst16(r, o, v); }
+PG_DEVICE void buf_store(rsrc_t r, uint32_t o, const uint2 &v) { bst8(r, o, v); }
+PG_DEVICE void buf_store(rsrc_t r, uint32_t o, uint32_t v) { __builtin_amdgcn_raw_buffer_store_b32(v, r, (int)o, 0, 0); }
+PG_DEVICE void buf_store(rsrc_t r, uint32_t o, uint16_t v) { __builtin_amdgcn_raw_buffer_store_b16(v, r, (int)o, 0, 0); }
+PG_DEVICE void buf_store(rsrc_t r, uint32_t o, uint8_t v) { __builtin_amdgcn_raw_buffer_store_b8(v, r, (int)o, 0, 0); }
+
 // Where a tile's or round's checkpoint goes: rows r0 .. r0 + rows, through buffer descriptors, which drop
 // the masked lanes' stores without a branch.
 struct CkRows {
@@ -284,11 +291,8 @@ PG_DEVICE void gn_checkpoint(const FwdArgs &a, const Place &p, const typename Ve
   const typename Codes<V>::raw c = Codes<V>::encode(f, mx8_inv_scale(e));
   const uint32_t o = ok ? (uint32_t)r * a.g.C + p.c : kOOB;
   const uint32_t os = ok && p.c % kMxBlock == 0 ? (uint32_t)r * ((a.g.C + kMxBlock - 1) / kMxBlock) + p.c / kMxBlock : kOOB;
-  if constexpr (V == 8) bst8(k.q, o, c);
-  else if constexpr (V == 4) __builtin_amdgcn_raw_buffer_store_b32(c, k.q, (int)o, 0, 0);
-  else if constexpr (V == 2) __builtin_amdgcn_raw_buffer_store_b16(c, k.q, (int)o, 0, 0);
-  else __builtin_amdgcn_raw_buffer_store_b8(c, k.q, (int)o, 0, 0);
-  __builtin_amdgcn_raw_buffer_store_b8((uint8_t)e, k.qs, (int)os, 0, 0);
+  buf_store(k.q, o, c);
+  buf_store(k.qs, os, (uint8_t)e);
 }
 
 // y of one row's V channels
@@ -574,9 +578,8 @@ __global__ __launch_bounds__(512, 4) void gn_fwd_staged_kernel(const FwdArgs a) 
   fwd_constants<V, VG>(gi, gm, gr, mu, sc);
   with_act(a.act, [&](auto act) {
     stream([&](const typename X::raw &raw, long long r0, int r, int nr, uint32_t off) {
-      if (r < nr)
-        at<typename X::raw>(static_cast<T *>(a.y) + r0 * g.C, off) =
-            gn_y<T, V, VG, decltype(act)::value>(raw, mu, sc, be);
+      const rsrc_t y = make_rsrc(static_cast<T *>(a.y) + r0 * g.C, (uint32_t)nr * g.C * (uint32_t)sizeof(T));
+      buf_store(y, r < nr ? off : kOOB, gn_y<T, V, VG, decltype(act)::value>(raw, mu, sc, be));
     });
   });
 }
@@ -933,11 +936,9 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
       const int nr = rd.rows(i);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (p.row + u * g.R < nr) {
-          float df[V], dz[V];
-          th.template row<false>(v[u], df, dz);
-          f(df, dz, r0, first + u * hop);
-        }
+        float df[V], dz[V];
+        th.template row<false>(v[u], df, dz);
+        f(df, dz, r0, nr, p.row + u * g.R, first + u * hop);
       }
     };
 #pragma unroll 1
@@ -954,11 +955,13 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
     float s0[V], s1[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s0[j] = s1[j] = 0.f;
-    stream([&](const float (&df)[V], const float (&dz)[V], long long, uint32_t) {
+    stream([&](const float (&df)[V], const float (&dz)[V], long long, int nr, int r, uint32_t) {
+      if (r < nr) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        s1[j] = fmaf(dz[j], df[j], s1[j]);
-        s0[j] += dz[j];
+        for (int j = 0; j < V; ++j) {
+          s1[j] = fmaf(dz[j], df[j], s1[j]);
+          s0[j] += dz[j];
+        }
       }
     });
     bwd_sums<V>(a, p, rstd, s1, s0, m);
@@ -970,8 +973,9 @@ __global__ __launch_bounds__(256, SILU || !FOLD ? 3 : 4) void gn_bwd_staged_kern
   if (!p.on) return;
   float al[V], k1[Th::VG], k2[Th::VG];
   bwd_constants<V, Th::VG>(g, p, th.rs, th.gi, m, al, k1, k2);
-  stream([&](const float (&df)[V], const float (&dz)[V], long long r0, uint32_t o) {
-    at<typename X::raw>(static_cast<T *>(a.dx) + r0 * g.C, o * (uint32_t)sizeof(T)) = gn_dx<T, V, Th::VG>(df, dz, al, k1, k2);
+  stream([&](const float (&df)[V], const float (&dz)[V], long long r0, int nr, int r, uint32_t o) {
+    const rsrc_t dx = make_rsrc(static_cast<T *>(a.dx) + r0 * g.C, (uint32_t)nr * g.C * (uint32_t)sizeof(T));
+    buf_store(dx, r < nr ? o * (uint32_t)sizeof(T) : kOOB, gn_dx<T, V, Th::VG>(df, dz, al, k1, k2));
   });
 }
 

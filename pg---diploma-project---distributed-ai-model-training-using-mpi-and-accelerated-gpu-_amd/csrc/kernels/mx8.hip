@@ -108,18 +108,22 @@ __global__ __launch_bounds__(kThreads) void mx8_unpack_kernel(const uint8_t *__r
 // are read from shared memory transposed (ds_read_tr16_b64: 4 rows of a column a lane).  The codes'
 // scales change with the row, so they are decoded on their way into shared memory: to bf16 exactly
 // (4 significant bits), 2 an instruction.
-//   tile     TN x TK outputs, 4 waves of QN x QK; 64 rows a step, two buffers: the next step's rows
-//            are in registers while this one's are multiplied
-//   rows     of the tile in shared memory are 32 bytes longer than the data: the 4 rows of a
-//            16-lane group of a transposed read then lie in different banks
-//   split    the M rows are cut into `splits` so that two workgroups a CU have work; each writes a
+//   tile     W x W outputs, 4 waves of a quarter each; 64 rows a step, two buffers in shared memory and
+//            two steps in registers or on their way (25088 x 1024 x 1024: kernel 83 us; 100 with one, and
+//            with four the registers' moves cost more than is gained; 91 with 256 x 256 and 8 waves)
+//   rows     of the tile in shared memory keep their 32-byte pieces in an order that depends on the
+//            row (wg_swz), so that transposed reads meet no bank twice
+//   split    the M rows are cut into `splits` so that every CU has two workgroups; each writes a
 //            partial [N * K + N] and a second kernel adds them in order
+// Measured with the join: 25088 x 1024 x 1024 92 us, 570 TFLOP/s (a step's reads, decoding, products and
+// barrier follow one another, and two workgroups a CU hide half of it); 401408 x 144 x 24 31 us, 4.1 TB/s;
+// 128 x 1000 x 2048 8 us, most of it the launch and the first loads' latency.
 // ---------------------------------------------------------------------------
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-constexpr int kMK = 64;
+constexpr int kMK = 64, kAhead = 2;
 
 struct WgradArgs {
   const void *dy;
@@ -137,6 +141,26 @@ template <> PG_DEVICE f32x4_t wg_mfma<bf16_t>(s16x8_t a, s16x8_t b, f32x4_t c) {
 template <> PG_DEVICE f32x4_t wg_mfma<_Float16>(s16x8_t a, s16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
+
+// what a thread holds of a chunk: in one piece, or value by value where rows are not aligned
+template <bool ALN> struct WgRaw {
+  typedef uint4 a;
+  typedef uint2 b;
+  static PG_DEVICE uint4 pack(const uint4 &v) { return v; }
+  static PG_DEVICE uint2 pack(const uint2 &v) { return v; }
+};
+template <> struct WgRaw<false> {
+  struct a { uint16_t v[8]; };
+  struct b { uint8_t v[8]; };
+  static PG_DEVICE uint4 pack(const a &x) {
+    return make_uint4(x.v[0] | (uint32_t)x.v[1] << 16, x.v[2] | (uint32_t)x.v[3] << 16, x.v[4] | (uint32_t)x.v[5] << 16,
+                      x.v[6] | (uint32_t)x.v[7] << 16);
+  }
+  static PG_DEVICE uint2 pack(const b &x) {
+    return make_uint2(x.v[0] | (uint32_t)x.v[1] << 8 | (uint32_t)x.v[2] << 16 | (uint32_t)x.v[3] << 24,
+                      x.v[4] | (uint32_t)x.v[5] << 8 | (uint32_t)x.v[6] << 16 | (uint32_t)x.v[7] << 24);
+  }
+};
 
 // 8 codes of one block -> 8 values of T
 template <class T> PG_DEVICE uint4 wg_decode(uint2 c, uint8_t e) {
@@ -157,160 +181,179 @@ template <class T> PG_DEVICE uint4 wg_decode(uint2 c, uint8_t e) {
   return r;
 }
 
+// Where row r of a shared tile of W columns keeps its 32-byte pieces: byte offset ^ this. A transposed
+// read takes one piece of each of rows 0..3 and 8..11 (or 4 on, or 16 on) at once: they fall into
+// different eighths of the 64 banks, without padding.
+template <int W> PG_DEVICE int wg_swz(int r) {
+  if constexpr (W == 64) return ((r >> 1 & 1) | (r >> 3 & 1) << 1) * 32;
+  else return ((r & 3) | (r >> 3 & 1) << 2) * 32;
+}
+
 // ALN: rows of dY and of the codes begin at multiples of 8 values
-template <class T, int TN, int TK, int WN, int WK, bool ALN>
+template <class T, int W, bool ALN>
 __global__ __launch_bounds__(256) void mx8_wgrad_kernel(const WgradArgs a) {
-  static_assert(WN * WK == 4, "4 waves");
-  constexpr int QN = TN / WN, QK = TK / WK, RN = QN / 16, RK = QK / 16;
-  constexpr int PA = TN * 2 + 32, PB = TK * 2 + 32;             // row pitches in bytes
-  constexpr int CA = TN / 8, CB = TK / 8;                       // 8-value chunks of a row
-  constexpr int NA = kMK * CA / 256, NB = (kMK * CB + 255) / 256;   // chunks a thread
-  __shared__ __attribute__((aligned(16))) char smem[2][kMK * (PA + PB)];
+  constexpr int TH = 256;                                       // threads
+  constexpr int Q = W / 2, R = Q / 16;                          // a wave's part, 16 x 16 blocks of it
+  constexpr int P = W * 2;                                      // row pitch in bytes
+  constexpr int CH = W / 8, RS = TH / CH;                       // 8-value chunks of a row, rows at a time
+  constexpr int NC = kMK / RS;                                     // chunks a thread
+  constexpr int D = kAhead;                           // steps on their way in registers
+  __shared__ __attribute__((aligned(16))) char smem[2][kMK * 2 * P];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   // neighbouring tiles of one row split on one XCD, whose L2 holds the rows they share
   const int total = a.tn * a.tk * a.splits, per = total / 8;
   int id = blockIdx.x;
   if (id < per * 8) id = (id & 7) * per + (id >> 3);
   const int split = id / (a.tn * a.tk), tile = id % (a.tn * a.tk);
-  const int n0 = (tile / a.tk) * TN, k0 = (tile % a.tk) * TK;
-  const int mb = split * a.rows, me = min(a.M, mb + a.rows);
-  const T *dy = static_cast<const T *>(a.dy);
+  const int n0 = (tile / a.tk) * W, k0 = (tile % a.tk) * W;
+  const int mb = split * a.rows, rows = min(a.M - mb, a.rows);
+  // The split's rows through buffer descriptors: rows past its end, and columns past N or K (offset
+  // kOOB), read as zeros, without a branch or a select that would wait for the load.
+  const rsrc_t ry = make_rsrc(static_cast<const T *>(a.dy) + (long long)mb * a.N, (uint32_t)rows * a.N * 2u);
+  const rsrc_t rq = make_rsrc(a.q + (long long)mb * a.K, (uint32_t)rows * a.K);
+  const rsrc_t rs = make_rsrc(a.qs + (long long)mb * a.nb, (uint32_t)rows * a.nb);
 
-  uint4 ra[NA];
-  uint2 rb[NB];
-  uint8_t re[NB];
-  // chunk i of this thread: row, first column
-  auto load = [&](int m0) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int s = t + i * 256, m = m0 + s / CA, n = n0 + s % CA * 8;
-      if constexpr (ALN) {
-        const bool ok = m < me && n < a.N;
-        const uint4 v = *reinterpret_cast<const uint4 *>(dy + (ok ? (long long)m * a.N + n : 0));
-        ra[i] = ok ? v : make_uint4(0, 0, 0, 0);
-      } else {
-        struct alignas(16) { T v[8]; } w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool ok = m < me && n + j < a.N;
-          const T v = dy[ok ? (long long)m * a.N + n + j : 0];
-          w.v[j] = ok ? v : (T)0;
-        }
-        ra[i] = __builtin_bit_cast(uint4, w);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int s = t + i * 256, m = m0 + s / CB, k = k0 + s % CB * 8;
-      const bool row = m < me && s < kMK * CB;
-      if constexpr (ALN) {
-        const bool ok = row && k < a.K;
-        const uint2 v = *reinterpret_cast<const uint2 *>(a.q + (ok ? (long long)m * a.K + k : 0));
-        rb[i] = ok ? v : make_uint2(0, 0);
-        re[i] = a.qs[ok ? (long long)m * a.nb + k / kMxBlock : 0];
-      } else {
-        struct alignas(8) { uint8_t v[8]; } w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool ok = row && k + j < a.K;
-          const uint8_t v = a.q[ok ? (long long)m * a.K + k + j : 0];
-          w.v[j] = ok ? v : 0;
-        }
-        rb[i] = __builtin_bit_cast(uint2, w);
-        re[i] = a.qs[row && k < a.K ? (long long)m * a.nb + k / kMxBlock : 0];
-      }
-    }
+  struct Stage {
+    typename WgRaw<ALN>::a a[NC];
+    typename WgRaw<ALN>::b b[NC];
+    uint8_t e[NC];
   };
-  float sum[8] = {};   // db: this thread's columns (a thread's chunks of dY are one column's, 256 % CA == 0)
-  const bool bias = a.db && k0 == 0;
-  auto put = [&](int buf) {
+  // Chunk i of this thread: row t / CH + i * RS of the step, column t % CH * 8 (codes alike). Its
+  // offsets for the next load; from kOOB on they stay outside, a split spans less than 2^31 bytes.
+  const int na = n0 + t % CH * 8, kb = k0 + t % CH * 8;
+  constexpr int JA = ALN ? 1 : 8;
+  uint32_t oa[JA], ob[JA], oe = kb < a.K ? (uint32_t)(t / CH) * a.nb + kb / kMxBlock : kOOB;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int s = t + i * 256;
-      *reinterpret_cast<uint4 *>(smem[buf] + s / CA * PA + s % CA * 16) = ra[i];
-      if (bias) {
+  for (int j = 0; j < JA; ++j) {
+    oa[j] = na + j < a.N ? ((uint32_t)(t / CH) * a.N + na + j) * 2u : kOOB;
+    ob[j] = kb + j < a.K ? (uint32_t)(t / CH) * a.K + kb + j : kOOB;
+  }
+  auto load = [&](Stage &g) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const uint32_t d = (uint32_t)(i * RS) * a.N * 2u;
+      if constexpr (ALN) {
+        g.a[i] = bld16(ry, oa[0] + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g.a[i].v[j] = __builtin_amdgcn_raw_buffer_load_b16(ry, (int)(oa[j] + d), 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const uint32_t m = i * RS, d = m * a.K;
+      if constexpr (ALN) {
+        g.b[i] = bld8(rq, ob[0] + d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g.b[i].v[j] = __builtin_amdgcn_raw_buffer_load_b8(rq, (int)(ob[j] + d), 0, 0);
+      }
+      g.e[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(oe + m * a.nb), 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < JA; ++j) {
+      oa[j] += kMK * 2u * a.N;
+      ob[j] += (uint32_t)kMK * a.K;
+    }
+    oe += (uint32_t)kMK * a.nb;
+  };
+  float sum[8] = {};   // db: this thread's columns (a thread's chunks of dY are one column's, TH % CH == 0)
+  const bool bias = a.db && k0 == 0;
+  auto put = [&](const Stage &g, int buf) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = t / CH + i * RS;
+      *reinterpret_cast<uint4 *>(smem[buf] + r * P + (t % CH * 16 ^ wg_swz<W>(r))) = WgRaw<ALN>::pack(g.a[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = t / CH + i * RS;
+      *reinterpret_cast<uint4 *>(smem[buf] + kMK * P + r * P + (t % CH * 16 ^ wg_swz<W>(r))) =
+          wg_decode<T>(WgRaw<ALN>::pack(g.b[i]), g.e[i]);
+    }
+    if (bias)
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
         float v[8];
-        Vec<T, 8>::unpack(ra[i], v);
+        Vec<T, 8>::unpack(WgRaw<ALN>::pack(g.a[i]), v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += v[j];
       }
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int s = t + i * 256;
-      if (kMK * CB % 256 == 0 || s < kMK * CB)
-        *reinterpret_cast<uint4 *>(smem[buf] + kMK * PA + s / CB * PB + s % CB * 16) = wg_decode<T>(rb[i], re[i]);
-    }
   };
 
-  f32x4_t acc[RN][RK];
+  f32x4_t acc[R][R];
 #pragma unroll
-  for (int i = 0; i < RN; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < RK; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int wn = wave / WK * QN, wk = wave % WK * QK;
+    for (int j = 0; j < R; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int wn = wave / 2 * Q, wk = wave % 2 * Q;
   // transposed reads: lane (g = lane / 16, i = lane % 16) asks for row 8 g + i / 4 (then + 4), 8-byte
   // piece i % 4 of a 16-column block, and receives those rows of column i
   const int trow = 8 * (lane >> 4) + ((lane & 15) >> 2), tc = (lane & 3) * 8;
   auto mma = [&](int buf) {
-    const char *A = smem[buf], *B = smem[buf] + kMK * PA;
+    const char *A = smem[buf], *B = smem[buf] + kMK * P;
 #pragma unroll
     for (int sub = 0; sub < kMK / 32; ++sub) {
-      s16x8_t fa[RN], fb[RK];
+      s16x8_t fa[R], fb[R];
 #pragma unroll
-      for (int i = 0; i < RN; ++i) {
-        const char *p = A + (sub * 32 + trow) * PA + (wn + i * 16) * 2 + tc;
+      for (int i = 0; i < R; ++i) {
+        const char *p = A + (sub * 32 + trow) * P + ((wn + i * 16) * 2 ^ wg_swz<W>(trow)) + tc;
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * PA));
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * P));
         fa[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       }
 #pragma unroll
-      for (int j = 0; j < RK; ++j) {
-        const char *p = B + (sub * 32 + trow) * PB + (wk + j * 16) * 2 + tc;
+      for (int j = 0; j < R; ++j) {
+        const char *p = B + (sub * 32 + trow) * P + ((wk + j * 16) * 2 ^ wg_swz<W>(trow)) + tc;
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)p);
-        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * PB));
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t *)(p + 4 * P));
         fb[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       }
 #pragma unroll
-      for (int i = 0; i < RN; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < RK; ++j) acc[i][j] = wg_mfma<T>(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < R; ++j) acc[i][j] = wg_mfma<T>(fa[i], fb[j], acc[i][j]);
     }
   };
 
-  if (mb < me) {
-    load(mb);
-    put(0);
-    __syncthreads();
-    int buf = 0;
-    for (int m0 = mb; m0 < me; m0 += kMK, buf ^= 1) {
-      const bool more = m0 + kMK < me;
-      if (more) load(m0 + kMK);
-      mma(buf);
-      if (more) put(buf ^ 1);
+  // Steps x + 1 to x + D are in registers or on their way while step x is multiplied; a turn is D
+  // steps (rows past the end are zeros).
+  Stage g[D];
+#pragma unroll
+  for (int j = 0; j < D; ++j) load(g[j]);
+  put(g[0], 0);
+  __syncthreads();
+  const int turns = (rows + kMK * D - 1) / (kMK * D);
+#pragma unroll 1
+  for (int s = 0; s < turns; ++s) {
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      load(g[j]);
+      mma(j & 1);
+      put(g[(j + 1) % D], (j + 1) & 1);
       __syncthreads();
     }
   }
   float *out = a.out + (a.splits > 1 ? split * a.pitch : 0);
 #pragma unroll
-  for (int i = 0; i < RN; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < RK; ++j)
+    for (int j = 0; j < R; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int n = n0 + wn + i * 16 + 4 * (lane >> 4) + r, k = k0 + wk + j * 16 + (lane & 15);
         if (n < a.N && k < a.K) out[(long long)n * a.K + k] = acc[i][j][r];
       }
   if (!bias) return;
-  // the 256 / CA threads of a column chunk, in order
+  // the RS threads of a column chunk, in order
   float *sh = reinterpret_cast<float *>(smem[0]);
 #pragma unroll
   for (int j = 0; j < 8; ++j) sh[t * 8 + j] = sum[j];
   __syncthreads();
   float *db = a.splits > 1 ? out + (long long)a.N * a.K : a.db;
-  if (t < TN && n0 + t < a.N) {
+  if (t < W && n0 + t < a.N) {
     float s = 0.f;
-    for (int r = 0; r < 256 / CA; ++r) s += sh[(r * CA + t / 8) * 8 + t % 8];
+    for (int r = 0; r < RS; ++r) s += sh[(r * CH + t / 8) * 8 + t % 8];
     db[n0 + t] = s;
   }
 }
@@ -354,25 +397,32 @@ __global__ __launch_bounds__(1024) void mx8_join_kernel(const float *__restrict_
 }
 
 struct WgradPlan {
-  int kind;   // 0: 128 x 128, 1: 256 x 32, 2: 32 x 256, 3: 64 x 64
-  int tn, tk, splits, rows;
+  int W, tn, tk, splits, rows;
   long long pitch;
 };
-const int kTileN[4] = {128, 256, 32, 64}, kTileK[4] = {128, 32, 256, 64};
 
+// Tiles of 64 x 64 until there is work for larger ones: four workgroups of them fit a CU, and the odd
+// widths of narrow layers pad less.  Measured, 128 and 64 (us): 25088 x 1024 x 1024 81 and 113, 6272 x
+// 2048 x 1024 51 and 56, 100352 x 512 x 256 51 and 60; 25088 x 512 x 512 32 and 34, 100352 x 256 x 256
+// 35 and 35; 1568 x 2048 x 1000 30 and 18, 401408 x 144 x 24 49 and 31, 100352 x 192 x 192 33 and 27.
+// 128 x 128 take as long as 64 x 64 where they pad to a third more.
 WgradPlan wgrad_plan(int M, int N, int K) {
   WgradPlan p{};
-  auto tiles = [&](int i) { return (long long)((N + kTileN[i] - 1) / kTileN[i]) * ((K + kTileK[i] - 1) / kTileK[i]); };
-  // Narrow weights take the tile that reads the wide operand once; others the square of which less is
-  // padding.
-  p.kind = K <= 32 ? 1 : N <= 32 ? 2 : tiles(3) * 64 * 64 * 3 < tiles(0) * 128 * 128 * 2 ? 3 : 0;
-  p.tn = (N + kTileN[p.kind] - 1) / kTileN[p.kind];
-  p.tk = (K + kTileK[p.kind] - 1) / kTileK[p.kind];
-  const long long t = (long long)p.tn * p.tk;
+  auto up = [](int n, int w) { return (long long)((n + w - 1) / w); };
+  const bool large = (double)M * N * K >= 8e9 && up(N, 128) * up(K, 128) * 4 * 3 <= up(N, 64) * up(K, 64) * 4;
+  p.W = large ? 128 : 64;
+  const long long t = up(N, p.W) * up(K, p.W);
   if (t > 0x7fffffff) throw std::invalid_argument("mx8_wgrad: N * K is too large");
+  p.tn = (int)up(N, p.W);
+  p.tk = (int)up(K, p.W);
   const int steps = (M + kMK - 1) / kMK;
+  // 512 workgroups (256: up to a fifth slower, 768 and 1024: no faster)
   long long s = std::max<long long>(1, std::min<long long>(512 / t, steps / 4));
-  p.rows = (int)((steps + s - 1) / s) * kMK;
+  // whole turns; a split's rows, and as many steps on as are loaded, span less than 2^31 bytes
+  long long turns = (steps + s * kAhead - 1) / (s * kAhead);
+  turns = std::min<long long>(turns, 0x7fffffffll / (2ll * std::max(N, K) * kMK * kAhead) - 1);
+  if (turns < 1) throw std::invalid_argument("mx8_wgrad: N or K is too large");
+  p.rows = (int)(turns * kAhead * kMK);
   p.splits = (int)(((long long)M + p.rows - 1) / p.rows);
   p.pitch = ((long long)N * K + N + 3) / 4 * 4;
   return p;
@@ -380,10 +430,8 @@ WgradPlan wgrad_plan(int M, int N, int K) {
 
 template <class T, bool ALN> void wgrad_go(const WgradPlan &p, const WgradArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)(p.tn * p.tk * p.splits));
-  if (p.kind == 0) hipLaunchKernelGGL((mx8_wgrad_kernel<T, 128, 128, 2, 2, ALN>), grid, dim3(256), 0, st, a);
-  else if (p.kind == 1) hipLaunchKernelGGL((mx8_wgrad_kernel<T, 256, 32, 4, 1, ALN>), grid, dim3(256), 0, st, a);
-  else if (p.kind == 2) hipLaunchKernelGGL((mx8_wgrad_kernel<T, 32, 256, 1, 4, ALN>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((mx8_wgrad_kernel<T, 64, 64, 2, 2, ALN>), grid, dim3(256), 0, st, a);
+  if (p.W == 128) hipLaunchKernelGGL((mx8_wgrad_kernel<T, 128, ALN>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((mx8_wgrad_kernel<T, 64, ALN>), grid, dim3(256), 0, st, a);
 }
 
 unsigned slot_grid(long long M, long long slots) {

@@ -9,11 +9,11 @@
 //   solo     a workgroup holds all S rows of a slab of whole groups in registers: one read
 //   held     the S rows are k tiles, and all tiles of the tensor are so few that their workgroups run
 //            together: each keeps its tile in registers, publishes its sums, waits for the k - 1
-//            others of its image and goes on.  One read.  (With more tiles than fit, a workgroup's
-//            chain load - sum - publish - wait - join - store is not hidden behind others':
-//            128 x 12544 x 96 backward took 1129 us.)
+//            others of its image and goes on.  One read.  (96 x 784 x 192 with checkpoint, backward: kernel 22.5
+//            us, 28.0 staged.  With more tiles than fit, a workgroup's chain load - sum - publish - wait -
+//            join - store is not hidden behind others': 128 x 12544 x 96 backward 1129 us.)
 //   staged   longer maps: the S rows are k tiles.  One launch holds a sums and a use workgroup for
-//            every tile; the use of an image's tiles is queued `lead` images behind its sums, so
+//            every tile; the use of an image's tiles is queued `lead` tiles behind its sums, so
 //            that it hardly ever waits for them and finds the tile in the memory-side cache
 //            (256 MB).  HBM sees every value once.
 //   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
@@ -213,8 +213,8 @@ PG_DEVICE bool pairs(const unsigned long long *src, int k, int l, int W, int pol
       const unsigned long long who = __ballot(none);
       if (!who) break;
       // One lane looks for its first missing pair until it comes, then all look again: with every lane
-      // looking, the waiting waves' reads held up those that were waited for (7 x 3249 x 100: 19 us,
-      // not 13).
+      // looking, the waiting waves' reads held up those that were waited for (7 x 3249 x 100
+      // forward 18.8 us, not 17.7).
       if ((int)(threadIdx.x & 63) == __ffsll((long long)who) - 1) {
         const int u = v[0] == kNone ? 0 : v[1] == kNone ? 1 : v[2] == kNone ? 2 : 3, ch = c0 + u * W + l;
         for (; i < polls && pair_load(src + (ch < k ? ch : l < k ? l : 0)) == kNone; ++i) __builtin_amdgcn_s_sleep(16);
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
 }
 
 // The rounds of a staged tile.  The tiles of a unit take turns, so that at any time the chip reads few
-// and compact stretches of memory (tiles in one piece: 128 x 3136 x 144 forward 91 us, not 7x).
+// and compact stretches of memory (128 x 12544 x 96 backward 235 us; 245 with tiles in one piece).
 struct Rounds {
   long long S;
   int turn, k, c, n;
@@ -560,8 +560,8 @@ __global__ __launch_bounds__(512, 4) void gn_fwd_staged_kernel(const FwdArgs a) 
     for (int j = 0; j < V; ++j) {
       const int k = FOLD ? 0 : j;
       const float df = fmaf(s1[k], rn, K[k]) - gm[gi[k]] * cn;
-      acc[j] = FOLD && j ? 0.f : fmaxf(fmaf(-s1[k] * rn, s1[k], s2[k]), 0.f) + n * df * df;
-      if (s1[k] != s1[k]) acc[j] = s1[k];   // fmaxf drops a NaN
+      const float own = fmaf(-s1[k] * rn, s1[k], s2[k]);   // a NaN stays
+      acc[j] = FOLD && j ? 0.f : (own < 0.f ? 0.f : own) + n * df * df;
     }
     __syncthreads();
     group_sums<V, FOLD>(g, p, acc, red, gr);

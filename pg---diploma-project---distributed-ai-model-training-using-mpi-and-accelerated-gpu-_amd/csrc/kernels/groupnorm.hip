@@ -162,14 +162,18 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 }
 
 // ---- host: geometry ----------------------------------------------------------------------------
-constexpr int kHeld = 480;    // tiles that wait for one another: two of 512 threads are resident on each of 256 CUs
+// Held: all tiles at most (two of 512 threads are resident on each of 256 CUs), and tiles of a unit.  Units
+// start in order, so at any time one unit of a launch is there in part and waits, and launches on the 4
+// hardware queues together never fill the chip with tiles that wait for one another.
+constexpr int kHeld = 480, kHeldUnit = 96;
 constexpr int kTiles = 512;   // tiles wanted before tiles grow (2048: gn_bwd 96 x 784 x 192 98 us, not 43)
 constexpr int kRounds = 6;    // rounds of a tile at most (2, 4, 8, 16: gn_bwd 128 x 12544 x 96 360, 260, 265, 314 us)
 // sums workgroups ahead of the use workgroups at least: half of what is resident (128, 256, 384, 1024:
 // gn_bwd 128 x 12544 x 96 +23%, +6%, -2%, +8%; gn_fwd 128 x 3136 x 144 +15%, +4%, +3%, 0%)
 constexpr int kLead = 512;
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
-int g_wait = 1 << 24;
+// looks (about a microsecond each) after which a waiting workgroup does without its peers
+int g_wait = 1 << 16;
 
 int gcd_pow2(long long c, int most) {
   int v = most;
@@ -184,6 +188,7 @@ size_t gn_lds(const Plan &p, bool bwd) {
 }
 
 Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {
+  if (C > 0x3fffffff) throw std::invalid_argument("group norm: C is too large");
   Plan p{};
   Geo &g = p.g;
   g.B = B;
@@ -253,7 +258,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     for (int nv : nvs) {
       if (only && nv != only) continue;
       const long long rows = (long long)g.R * nv, k = (S + rows - 1) / rows;
-      if (B * g.nslab * k > kHeld) continue;
+      if (k > kHeldUnit || B * g.nslab * k > kHeld) continue;
       p.NV = nv;
       g.rows = (int)rows;
       g.k = (int)k;
@@ -316,7 +321,7 @@ void gn_none(const Plan &p, unsigned long long *part, hipStream_t st) {
 
 void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M, int C, hipStream_t st);
 
-// looks of a staged wait, about a microsecond each (tests: -1, what has come is not looked at)
+// tests: -1, what has come is not looked at
 void gn_set_wait(int polls) { g_wait = polls; }
 
 // dt: 0 bf16, 1 fp16, 2 fp32.  Forward and backward, with and without a checkpoint: the largest.

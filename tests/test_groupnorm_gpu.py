@@ -335,6 +335,35 @@ def test_two_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(alone[k], out))
 
 
+@pytest.mark.parametrize("S", [12200, 30000])
+def test_one_long_image_on_four_streams(S):
+    """Launches whose workgroups wait for one another share the chip: each comes out as it does alone."""
+    B, C, G = 1, 128, 16
+    x, gamma, beta, dy = make(B, S, C, torch.bfloat16, 50)
+    y, mean, rstd, q, qs = call_fwd(x, gamma, beta, B, S, C, G, 2, True)
+    alone = (y, mean, rstd, *call_bwd(dy, None, gamma, beta, mean, rstd, B, S, C, G, 2, q, qs))
+    torch.cuda.synchronize()
+    got = []
+    for st in [torch.cuda.Stream() for _ in range(4)] * 5:
+        with torch.cuda.stream(st):
+            y, mean, rstd, q, qs = call_fwd(x, gamma, beta, B, S, C, G, 2, True)
+            got.append((y, mean, rstd, *call_bwd(dy, None, gamma, beta, mean, rstd, B, S, C, G, 2, q, qs)))
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(torch.equal(a, b) for a, b in zip(alone, out))
+
+
+def test_squares_past_the_range_are_not_taken_for_zeros():
+    """Values whose squares pass fp32's range have no finite variance there: rstd is 0 or NaN. Their signs
+    are such that every thread's own sum is 0."""
+    B, S, C, G = 1, 25600, 128, 16
+    sign = 1 - 2 * (torch.arange(S, device="cuda") // 32 % 2)
+    x = (1e25 * sign).to(torch.bfloat16).view(1, S, 1).expand(B, S, C).contiguous()
+    one = torch.ones(C, device="cuda")
+    rstd = call_fwd(x, one, one, B, S, C, G, 0, False)[2]
+    assert ((rstd == 0) | rstd.isnan()).all()
+
+
 def test_offsets_past_32_bits():
     """2.15e9 values (4.3 GB): the last image comes out as it does alone."""
     B, S, C, G = 5, 419431, 1024, 128

@@ -166,10 +166,15 @@ __global__ __launch_bounds__(256) void gn_none_kernel(unsigned long long *__rest
 // start in order, so at any time one unit of a launch is there in part and waits, and launches on the 4
 // hardware queues together never fill the chip with tiles that wait for one another.
 constexpr int kHeld = 480, kHeldUnit = 96;
-constexpr int kTiles = 512;   // tiles wanted before tiles grow (2048: gn_bwd 96 x 784 x 192 98 us, not 43)
-constexpr int kRounds = 6;    // rounds of a tile at most (2, 4, 8, 16: gn_bwd 128 x 12544 x 96 360, 260, 265, 314 us)
-// sums workgroups ahead of the use workgroups at least: half of what is resident (128, 256, 384, 1024:
-// gn_bwd 128 x 12544 x 96 +23%, +6%, -2%, +8%; gn_fwd 128 x 3136 x 144 +15%, +4%, +3%, 0%)
+// Staged: tiles wanted before tiles grow (256, 512, 1024, 2048: gn_bwd 96 x 784 x 192, were it not held, 33, 33,
+// 40, 70 us)
+constexpr int kTiles = 512;
+// rounds of a tile at most, forward and backward (1, 2, 4, 6, 8, 16: gn_fwd 128 x 3136 x 144 with checkpoint 142,
+// 89, 77, 82, 89, 89 us; gn_bwd 128 x 12544 x 96 675, 340, 253, 232, 236, 305): a workgroup costs some 12 us of
+// latency however little it does, and with long ones the last tiles run alone
+constexpr int kRounds[2] = {4, 6};
+// sums workgroups ahead of the use workgroups at least: half of what is resident (128, 256, 512, 768, 1024: gn_bwd
+// 128 x 12544 x 96 297, 282, 232, 233, 260 us; gn_fwd 128 x 3136 x 144 within 5%)
 constexpr int kLead = 512;
 constexpr int kSplitRows = 64;     // row splits of a long dgamma / dbeta sum
 // looks (about a microsecond each) after which a waiting workgroup does without its peers
@@ -278,7 +283,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   }
   // tiles of up to kRounds rounds, fewer while the tiles do not fill the chip several times
   const long long round = (long long)g.R * (bwd ? 2 : 4), all = (S + round - 1) / round;
-  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, kRounds);
+  const long long it = std::clamp<long long>(B * g.nslab * all / kTiles, 1, kRounds[bwd]);
   const long long k = (all + it - 1) / it;
   p.NV = 1;
   g.turn = (int)round;

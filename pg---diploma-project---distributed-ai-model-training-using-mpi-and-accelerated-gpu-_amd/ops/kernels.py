@@ -1083,7 +1083,13 @@ def _apart(what, outs, ins):
                     raise ValueError(f"{what}: {na} overlaps {nb_}")
 
 
-def _workspace(what, ws, need, dev):
+def _not_recorded(what):
+    """Empty operands are dealt with by torch, which a launch plan does not record."""
+    if plan_recording():
+        raise ValueError(f"{what}: empty operands cannot be recorded into a launch plan")
+
+
+def _workspace(what, ws, need, dev, operands):
     """The caller's workspace, checked, or one from the allocator for this call alone."""
     if ws is None:
         if not need:
@@ -1094,6 +1100,7 @@ def _workspace(what, ws, need, dev):
     if ws.dtype != F32 or not ws.is_contiguous() or ws.numel() < need or ws.data_ptr() & 15:
         raise ValueError(f"{what}: ws must be {need} contiguous, 16-byte aligned floats")
     _device_of(what, ws)
+    _apart(what, [("ws", ws.data_ptr(), 4 * need)], operands)
     return ws
 
 
@@ -1102,17 +1109,24 @@ def mx8_blocks(C):
     return -(-C // MX8_BLOCK)
 
 
+def _gn_sizes(what, B, S, C, G):
+    if B < 0 or S < 0 or not 1 <= C < 1 << 30 or G < 1 or C % G:
+        raise ValueError(f"{what}: B={B} S={S} C={C} G={G}: G must divide C, B and S be 0 at least, C below 2^30")
+
+
 def _gn_check(what, t, B, S, C, G, act):
     if t.dtype not in _DT:
         raise TypeError(f"{what}: bf16, fp16 or fp32 activations, got {t.dtype}")
-    if B < 0 or S < 0 or C < 1 or G < 1 or C % G:
-        raise ValueError(f"{what}: B={B} S={S} C={C} G={G}: G must divide C, B and S be 0 at least")
+    _gn_sizes(what, B, S, C, G)
     if act not in (GN_NONE, GN_RELU, GN_RELU6, GN_SILU):
         raise ValueError(f"{what}: unknown activation {act}")
 
 
 def gn_workspace(B, S, C, G, dtype, bwd=False):
     """Floats of workspace that gn_fwd / gn_bwd of these sizes take as ``ws``."""
+    if dtype not in _DT:
+        raise TypeError(f"gn_workspace: bf16, fp16 or fp32 activations, got {dtype}")
+    _gn_sizes("gn_workspace", B, S, C, G)
     return int(lib().gn_workspace_floats(_DT[dtype], B, S, C, G, int(bwd)))
 
 
@@ -1124,8 +1138,8 @@ def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=N
     ``ws``: :func:`gn_workspace` floats for this call alone; None takes them from the allocator.
     No output may overlap another operand.  S = 0 gives mean 0, rstd 1/sqrt(eps)."""
     _gn_check("gn_fwd", x, B, S, C, G, act)
-    if not eps > 0:
-        raise ValueError(f"gn_fwd: eps={eps} must be positive")
+    if not 2.0 ** -126 <= eps < float("inf"):
+        raise ValueError(f"gn_fwd: eps={eps} must be a positive normal fp32 number")
     if (q is None) != (qs is None):
         raise ValueError("gn_fwd: q and qs both or neither")
     n, ns, e = B * S * C, B * S * mx8_blocks(C), x.element_size()
@@ -1133,14 +1147,16 @@ def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=N
     pg, pb = _operand(gamma, "gamma", F32, C), _operand(beta, "beta", F32, C)
     pm, pr = _operand(mean, "mean", F32, B * G), _operand(rstd, "rstd", F32, B * G)
     pq, ps = _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
-    _apart("gn_fwd", [("y", py, n * e), ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G), ("q", pq, n), ("qs", ps, ns)],
-           [("x", px, n * e), ("gamma", pg, 4 * C), ("beta", pb, 4 * C)])
+    outs = [("y", py, n * e), ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G), ("q", pq, n), ("qs", ps, ns)]
+    ins = [("x", px, n * e), ("gamma", pg, 4 * C), ("beta", pb, 4 * C)]
+    _apart("gn_fwd", outs, ins)
     dev = _device_of("gn_fwd", x, y, gamma, beta, mean, rstd, q, qs)
     if n == 0:
+        _not_recorded("gn_fwd")
         mean.zero_()
         rstd.fill_(eps ** -0.5)
         return
-    ws = _workspace("gn_fwd", ws, gn_workspace(B, S, C, G, x.dtype), dev)
+    ws = _workspace("gn_fwd", ws, gn_workspace(B, S, C, G, x.dtype), dev, outs + ins)
     lib().gn_fwd(_DT[x.dtype], px, pg, pb, py, pm, pr, pq, ps, 0 if ws is None else ws.data_ptr(), B, S, C, G,
                  float(eps), act, _raw_stream(dev))
 
@@ -1160,15 +1176,17 @@ def gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=GN_NONE, q=N
     pm, pr = _operand(mean, "mean", F32, B * G), _operand(rstd, "rstd", F32, B * G)
     pq, ps = _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
     pw = _operand(dgb, "dgb", F32, 2 * C)
-    _apart("gn_bwd", [("dx", po, n * e), ("dgb", pw, 8 * C)],
-           [("dy", pd, n * e), ("x", px, n * e), ("q", pq, n), ("qs", ps, ns), ("gamma", pg, 4 * C), ("beta", pb, 4 * C),
-            ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G)])
+    outs = [("dx", po, n * e), ("dgb", pw, 8 * C)]
+    ins = [("dy", pd, n * e), ("x", px, n * e), ("q", pq, n), ("qs", ps, ns), ("gamma", pg, 4 * C), ("beta", pb, 4 * C),
+           ("mean", pm, 4 * B * G), ("rstd", pr, 4 * B * G)]
+    _apart("gn_bwd", outs, ins)
     dev = _device_of("gn_bwd", dy, x, gamma, beta, mean, rstd, dx, dgb, q, qs)
     if n == 0:
+        _not_recorded("gn_bwd")
         if dgb is not None:
             dgb.zero_()
         return
-    ws = _workspace("gn_bwd", ws, gn_workspace(B, S, C, G, dy.dtype, True), dev)
+    ws = _workspace("gn_bwd", ws, gn_workspace(B, S, C, G, dy.dtype, True), dev, outs + ins)
     lib().gn_bwd(_DT[dy.dtype], pd, px, pq, ps, pg, pb, pm, pr, po, pw, 0 if ws is None else ws.data_ptr(), B, S, C, G,
                  act, _raw_stream(dev))
 
@@ -1207,8 +1225,14 @@ def mx8_unpack(q, qs, x, M, C):
         lib().mx8_unpack(_DT[x.dtype], pq, ps, px, M, C, _raw_stream(dev))
 
 
+def _wgrad_sizes(what, M, N, K):
+    if not 0 <= M <= _I31 or not 1 <= N <= _I31 or not 1 <= K <= _I31:
+        raise ValueError(f"{what}: M={M} N={N} K={K}: N and K must be positive, M 0 at least, each below 2^31")
+
+
 def mx8_wgrad_workspace(M, N, K):
     """Floats of workspace that mx8_wgrad of these sizes takes as ``ws``."""
+    _wgrad_sizes("mx8_wgrad_workspace", M, N, K)
     return int(lib().mx8_wgrad_workspace_floats(M, N, K))
 
 
@@ -1220,19 +1244,20 @@ def mx8_wgrad(dy, q, qs, grad, M, N, K, db=None, ws=None):
     :func:`mx8_wgrad_workspace` floats for this call alone; None takes them from the allocator."""
     if dy.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"mx8_wgrad: dy bf16 or fp16, got {dy.dtype}")
-    if not 0 <= M <= _I31 or not 1 <= N <= _I31 or not 1 <= K <= _I31:
-        raise ValueError(f"mx8_wgrad: M={M} N={N} K={K}: N and K must be positive, M 0 at least, each below 2^31")
+    _wgrad_sizes("mx8_wgrad", M, N, K)
     nq, ns = M * K, M * mx8_blocks(K)
     pd, pq, ps = _operand(dy, "dy", dy.dtype, M * N), _operand(q, "q", torch.uint8, nq), _operand(qs, "qs", torch.uint8, ns)
     pw, pb = _operand(grad, "grad", F32, N * K), _operand(db, "db", F32, N)
-    _apart("mx8_wgrad", [("grad", pw, 4 * N * K), ("db", pb, 4 * N)], [("dy", pd, 2 * M * N), ("q", pq, nq), ("qs", ps, ns)])
+    outs, ins = [("grad", pw, 4 * N * K), ("db", pb, 4 * N)], [("dy", pd, 2 * M * N), ("q", pq, nq), ("qs", ps, ns)]
+    _apart("mx8_wgrad", outs, ins)
     dev = _device_of("mx8_wgrad", dy, q, qs, grad, db)
     if M == 0:
+        _not_recorded("mx8_wgrad")
         grad.zero_()
         if db is not None:
             db.zero_()
         return
-    ws = _workspace("mx8_wgrad", ws, mx8_wgrad_workspace(M, N, K), dev)
+    ws = _workspace("mx8_wgrad", ws, mx8_wgrad_workspace(M, N, K), dev, outs + ins)
     lib().mx8_wgrad(_DT[dy.dtype], pd, pq, ps, pw, pb, 0 if ws is None else ws.data_ptr(), M, N, K, _raw_stream(dev))
 
 

@@ -50,8 +50,8 @@ class _GroupNormAct(torch.autograd.Function):
             S = xl.numel() // (B * C) if B else 0
             w, b = _vec(weight), _vec(bias)
             y = torch.empty_like(xl)
-            mean = torch.empty(B, groups, device=x.device)
-            rstd = torch.empty(B, groups, device=x.device)
+            mean = torch.empty(B, groups, dtype=torch.float32, device=x.device)
+            rstd = torch.empty_like(mean)
             keep = ckpt8 and any(ctx.needs_input_grad[:3])
             q, qs = _codes(B * S, C, x.device) if keep else (None, None)
             K.gn_fwd(xl, w, b, y, mean, rstd, B, S, C, groups, eps=eps, act=act, q=q, qs=qs)
@@ -69,7 +69,7 @@ class _GroupNormAct(torch.autograd.Function):
         with _on(dy):
             dyl = _rows(dy)
             dx = torch.empty_like(dyl)
-            dgb = torch.empty(2, C, device=dy.device) if params else None
+            dgb = torch.empty(2, C, dtype=torch.float32, device=dy.device) if params else None
             K.gn_bwd(dyl, xl, w, b, mean, rstd, dx, dgb, B, S, C, groups, act=act, q=q, qs=qs)
         dw = dgb[0].to(ctx.dtypes[0]) if ctx.needs_input_grad[1] else None
         db = dgb[1].to(ctx.dtypes[1]) if ctx.needs_input_grad[2] else None
@@ -85,7 +85,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt
     if x.dim() < 2:
         raise ValueError("group_norm_act: x must be [B, C, ...]")
     C = x.shape[1]
-    if groups < 1 or C % groups:
+    if C < 1 or groups < 1 or C % groups:
         raise ValueError(f"group_norm_act: {groups} groups do not divide {C} channels")
     for t, nm in ((weight, "weight"), (bias, "bias")):
         if t is not None and (t.numel() != C or t.device != x.device):
@@ -100,7 +100,7 @@ class GroupNormAct(nn.Module):
 
     def __init__(self, num_groups: int, num_channels: int, act: str = "none", eps: float = 1e-5, ckpt8: bool = False):
         super().__init__()
-        if num_groups < 1 or num_channels % num_groups:
+        if num_channels < 1 or num_groups < 1 or num_channels % num_groups:
             raise ValueError(f"GroupNormAct: {num_groups} groups do not divide {num_channels} channels")
         if act not in ACTS:
             raise ValueError(f"GroupNormAct: unknown activation {act!r}; available: {sorted(ACTS)}")
@@ -145,8 +145,8 @@ class _Conv1x1(torch.autograd.Function):
             if ctx.needs_input_grad[0]:
                 dx = (dyl.view(M, N) @ w).view(*dyl.shape[:-1], C).movedim(-1, 1).to(xdt)
             if ctx.needs_input_grad[1]:
-                dw = torch.empty(N, C, device=dy.device)
-                db = torch.empty(N, device=dy.device) if ctx.needs_input_grad[2] else None
+                dw = torch.empty(N, C, dtype=torch.float32, device=dy.device)
+                db = torch.empty(N, dtype=torch.float32, device=dy.device) if ctx.needs_input_grad[2] else None
                 K.mx8_wgrad(dyl, q, qs, dw, M, N, C, db=db)
                 dw = dw.view(wshape).to(wdt)
             elif ctx.needs_input_grad[2]:

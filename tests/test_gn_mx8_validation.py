@@ -100,5 +100,31 @@ def test_mx8_wgrad_refuses():
         K.mx8_wgrad(**{**a, "db": a["grad"].view(-1)[:8]})
 
 
+def test_sizes_of_workspaces_are_checked():
+    for args, error in (((-1, 4, 32, 4, BF), ValueError), ((1, 4, 0, 1, BF), ValueError), ((1, 4, 32, 0, BF), ValueError),
+                        ((1, 4, 32, 5, BF), ValueError), ((1, 4, 1 << 30, 4, BF), ValueError),
+                        ((1, 4, 32, 4, torch.float64), TypeError)):
+        with pytest.raises(error):
+            K.gn_workspace(*args)
+    for args in ((4, 0, 40), (4, 8, 0), (-1, 8, 40), (4, 1 << 31, 40)):
+        with pytest.raises(ValueError):
+            K.mx8_wgrad_workspace(*args)
+    assert K.gn_workspace(0, 4, 32, 4, BF) == 0 and K.mx8_wgrad_workspace(0, 8, 40) == 0
+
+
+@pytest.mark.parametrize("eps", [1e-45, float("inf")])
+def test_gn_fwd_refuses_an_eps_that_fp32_does_not_hold(eps):
+    with pytest.raises(ValueError, match="eps"):
+        K.gn_fwd(**{**fwd_args(), "eps": eps})
+
+
+def test_modules_refuse_no_channels():
+    from pgdist.ops import nn as N
+    with pytest.raises(ValueError):
+        N.GroupNormAct(1, 0)
+    with pytest.raises(ValueError):
+        N.group_norm_act(torch.zeros(2, 0, 3, 3), 1)
+
+
 def test_blocks():
     assert [K.mx8_blocks(c) for c in (1, 32, 33, 144)] == [1, 1, 2, 5]

@@ -133,6 +133,56 @@ def test_on_another_stream():
     assert all(torch.equal(a, b) for o in got for a, b in zip(o, want))
 
 
+def test_under_another_default_type():
+    x, w, b, dy = inputs((2, 32, 6, 6), torch.bfloat16, 6)
+    conv = (0.1 * torch.randn(16, 32, 1, 1, device="cuda")).bfloat16().requires_grad_()
+
+    def once():
+        xs = x.detach().requires_grad_()
+        y = N.conv1x1(N.group_norm_act(xs, 4, w.requires_grad_(), b.requires_grad_(), act="relu", ckpt8=True), conv)
+        return torch.autograd.grad(y.float().square().sum(), (xs, w, b, conv))
+
+    want = once()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = once()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_a_captured_training_step_replays():
+    m = torch.nn.Sequential(N.Conv1x1Ckpt8(24, 64), N.GroupNormAct(8, 64, "relu6", ckpt8=True), N.Conv1x1Ckpt8(64, 16),
+                            N.GroupNormAct(2, 16, "silu")).cuda().bfloat16().to(memory_format=torch.channels_last)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    data = [torch.randn(4, 24, 40, 40, generator=g, device="cuda").bfloat16().contiguous(memory_format=torch.channels_last)
+            for _ in range(4)]
+    x = data[0].clone(memory_format=torch.preserve_format)
+    dy = torch.randn(4, 16, 40, 40, generator=g, device="cuda").bfloat16()
+    params = list(m.parameters())
+
+    def step():
+        return torch.autograd.grad(m(x), params, dy)
+
+    want = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for d in data:
+            x.copy_(d)
+            want.append([t.clone() for t in step()])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in (1, 2, 3, 0, 2):
+        x.copy_(data[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+        _ = torch.randn(1 << 20, device="cuda").sum().item()   # the program's own work between replays
+
+
 def test_empty_batches():
     m = N.GroupNormAct(4, 32, "relu", ckpt8=True).cuda()
     x = torch.zeros(0, 32, 5, 5, device="cuda", dtype=torch.bfloat16, requires_grad=True)

@@ -314,6 +314,30 @@ def test_recorded_plan_replays():
     plan.free()
 
 
+def test_a_workspace_over_an_operand_and_empty_recordings_are_refused():
+    B, S, C, G = 2, 6001, 96, 12
+    x, gamma, beta, dy = make(B, S, C, torch.float32, 31)
+    need = K.gn_workspace(B, S, C, G, torch.float32, True)
+    y, mean, rstd = torch.empty_like(x), *(torch.empty(B, G, device="cuda") for _ in range(2))
+    assert y.numel() >= need > 0
+    with pytest.raises(ValueError, match="ws overlaps y"):
+        K.gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, ws=y.view(-1))
+    dw, q, qs = torch.empty(64, 96, device="cuda"), *zero_codes(4096, 96)
+    d = torch.zeros(4096, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="ws overlaps dy"):
+        K.mx8_wgrad(d, q, qs, dw, 4096, 64, 96, ws=d.view(torch.float32).view(-1))
+    none = torch.empty(0, 96, device="cuda")
+    plan = K.LaunchPlan()
+    with pytest.raises(ValueError, match="recorded"):
+        plan.record(lambda: K.gn_bwd(none, none, None, None, none, none, none, torch.empty(2, 96, device="cuda"), 0, 5,
+                                     96, 12))
+
+
+def zero_codes(M, C):
+    return (torch.zeros(M, C, dtype=torch.uint8, device="cuda"),
+            torch.full((M, K.mx8_blocks(C)), 127, dtype=torch.uint8, device="cuda"))
+
+
 def test_two_streams_at_once():
     B, S, C, G = 8, 6001, 96, 12
     data = [make(B, S, C, torch.bfloat16, 30 + k) for k in range(2)]

@@ -32,6 +32,10 @@ struct BnFin {
   float *coef, *dgamma, *dbeta;         // backward outputs (coef [3][C])
 };
 
+// A running statistic's step, with its roundings written out: left to the compiler, either product may be
+// the fused one, and the finalize kernels would differ in the last bit.
+PG_DEVICE float bn_running(float momentum, float old, float now) { return fmaf(momentum, now, (1.f - momentum) * old); }
+
 // forward: totals (sum, sum of squares) of channel c -> mean, rstd, scale, shift, running stats
 PG_DEVICE void bn_fwd_channel(int c, double s0, double s1, double n, const float *gamma, const float *beta,
                               float eps, float momentum, float *rmean, float *rvar, float *mean_out,
@@ -47,8 +51,8 @@ PG_DEVICE void bn_fwd_channel(int c, double s0, double s1, double n, const float
   shift_out[c] = b - (float)mean * g * rstd;
   if (rmean) {
     const double unbiased = n > 1.0 ? var * n / (n - 1.0) : var;
-    rmean[c] = (1.f - momentum) * rmean[c] + momentum * (float)mean;
-    rvar[c] = (1.f - momentum) * rvar[c] + momentum * (float)unbiased;
+    rmean[c] = bn_running(momentum, rmean[c], (float)mean);
+    rvar[c] = bn_running(momentum, rvar[c], (float)unbiased);
   }
 }
 

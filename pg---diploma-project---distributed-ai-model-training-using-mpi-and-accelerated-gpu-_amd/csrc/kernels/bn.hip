@@ -154,8 +154,8 @@ __global__ __launch_bounds__(128) void bn_finalize_small_kernel(
       shift[c] = b - (float)m * g * r;
       if (rmean) {
         const double unbiased = n > 1.0 ? var * n / (n - 1.0) : var;
-        rmean[c] = (1.f - momentum) * rm0 + momentum * (float)m;
-        rvar[c] = (1.f - momentum) * rv0 + momentum * (float)unbiased;
+        rmean[c] = bn_running(momentum, rm0, (float)m);
+        rvar[c] = bn_running(momentum, rv0, (float)unbiased);
       }
     }
   }

@@ -106,7 +106,7 @@ def test_wgrad(mnk, dtype):
     want, mag = d.t().contiguous() @ x, d.abs().t().contiguous() @ x.abs()
     # every product is exact in fp32 (12 significant bits); at most M + 64 additions, each u off
     O.within(dw, want, (M + 64) * O.U * mag)
-    O.within(db, d.sum(0), (M + 64) * O.U * d.abs().sum(0))
+    O.within(db, O.sums(d), (M + 64) * O.U * O.sums(d.abs()))
     # roundings are as often up as down: over the matrix they add as a random walk, u sqrt(M / 6) of the norm
     assert (dw.double() - want).norm() <= 4 * O.U * (M + 1) ** 0.5 * want.norm() + 1e-30
     again = torch.empty_like(dw)

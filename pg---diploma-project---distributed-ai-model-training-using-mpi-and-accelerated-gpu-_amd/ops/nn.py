@@ -150,7 +150,10 @@ class _Conv1x1(torch.autograd.Function):
                 K.mx8_wgrad(dyl, q, qs, dw, M, N, C, db=db)
                 dw = dw.view(wshape).to(wdt)
             elif ctx.needs_input_grad[2]:
-                db = dyl.view(M, N).float().sum(0)
+                db = torch.empty(N, dtype=torch.float32, device=dy.device)
+                z = torch.zeros(M, 8, dtype=torch.uint8, device=dy.device)   # no input was kept: beside a product with zeros
+                K.mx8_wgrad(dyl, z, z.view(-1)[:M].view(M, 1), torch.empty(N, 8, dtype=torch.float32, device=dy.device),
+                            M, N, 8, db=db)
         return dx, dw, None if db is None else db.to(bdt), None
 
 

@@ -87,6 +87,18 @@ def test_conv1x1(dtype, stride):
     assert ((dx.movedim(1, -1).double() - full).abs() <= 2 * h * full.abs() + 2 * h * full.abs().mean()).all()
 
 
+def test_conv1x1_with_a_frozen_weight():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(3, 24, 37, 41, generator=g, device="cuda").bfloat16().contiguous(memory_format=torch.channels_last)
+    w = torch.randn(20, 24, 1, 1, generator=g, device="cuda").bfloat16()
+    b = torch.zeros(20, device="cuda", requires_grad=True)
+    y = N.conv1x1(x, w, b)
+    dy = torch.randn(y.shape, generator=g, device="cuda").bfloat16()
+    db, = torch.autograd.grad(y, b, dy)
+    d = dy.movedim(1, -1).reshape(-1, 20).double()
+    O.within(db, O.sums(d), (d.shape[0] + 64) * O.U * O.sums(d.abs()))
+
+
 def test_under_autocast_parameters_keep_their_type():
     m = torch.nn.Sequential(N.Conv1x1Ckpt8(16, 32), N.GroupNormAct(4, 32, "relu6", ckpt8=True),
                             N.Conv1x1Ckpt8(32, 8)).cuda()

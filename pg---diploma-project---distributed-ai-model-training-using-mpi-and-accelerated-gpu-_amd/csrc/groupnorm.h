@@ -403,8 +403,11 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
     d[i] = at<typename X::raw>(src, (r * g.C + p.c) * (uint32_t)sizeof(T));
   }
   float acc[V], mu[VG], sc[V], be[V];
-  channel_values(a.gamma, a.mean, p.c, 1.f, sc);
-  channel_values(a.beta, a.mean, p.c, 0.f, be);
+  auto affine = [&] {
+    channel_values(a.gamma, a.mean, p.c, 1.f, sc);
+    channel_values(a.beta, a.mean, p.c, 0.f, be);
+  };
+  if constexpr (MODE == SOLO) affine();
 #pragma unroll
   for (int j = 0; j < V; ++j) acc[j] = 0.f;
 #pragma unroll
@@ -445,6 +448,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_solo_kernel(const FwdArgs a) {
     unsigned long long *out = a.part + p.unit * g.k * g.gs + p.chunk, pv[4];
     for (int i = threadIdx.x; i < p.ng; i += blockDim.x) pair_store(out + (long long)i * g.k, gm[i], gr[i]);
     __syncthreads();   // gm and gr have been read
+    affine();
     jl.ahead(g, p, pv);
     fwd_join<T, MODE>(a, p, jl, pv, gm, gr);
   } else {
@@ -988,6 +992,8 @@ struct Plan {
 
 struct Fwd {
   typedef FwdArgs Args;
+  template <int MODE, bool SILU> static constexpr int most = 8;   // NV at most
+  template <bool CK> static constexpr bool held = !CK;
   template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
     return gn_fwd_solo_kernel<T, V, NV, MODE, CK, FOLD>;
   }
@@ -997,6 +1003,8 @@ struct Fwd {
 };
 struct Bwd {
   typedef BwdArgs Args;
+  template <int MODE, bool SILU> static constexpr int most = MODE == SOLO || SILU ? 4 : 8;
+  template <bool CK> static constexpr bool held = true;
   template <class T, int V, int NV, int MODE, bool CK, bool FOLD, bool SILU> static constexpr auto solo() {
     return gn_bwd_solo_kernel<T, V, NV, MODE, CK, FOLD, SILU>;
   }
@@ -1005,7 +1013,7 @@ struct Bwd {
   }
 };
 
-// the plan gives NV 2, 4, 8 to full vectors of one group each, 2 to vectors of 8 that straddle groups
+// the plan gives NV 2, 4 and (up to `most`) 8 to full vectors of one group each, 2 to vectors of 8 that straddle groups
 // (their constants take the registers), 4 to narrower ones
 template <class D, class T, int VMAX, bool CK, bool SILU>
 void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st) {
@@ -1021,16 +1029,17 @@ void launch(const Plan &p, size_t lds, const typename D::Args &a, hipStream_t st
   }
   auto solo = [&](auto mode) {
     constexpr int M = decltype(mode)::value;
+    constexpr int most = D::template most<M, SILU>;
     if (fold && p.NV == 2) go(D::template solo<T, VMAX, 2, M, CK, true, SILU>());
-    else if (fold && p.NV == 4) go(D::template solo<T, VMAX, 4, M, CK, true, SILU>());
-    else if (fold) go(D::template solo<T, VMAX, 8, M, CK, true, SILU>());
+    else if (fold && p.NV == most) go(D::template solo<T, VMAX, most, M, CK, true, SILU>());
+    else if (fold) go(D::template solo<T, VMAX, 4, M, CK, true, SILU>());
     else if (full) go(D::template solo<T, VMAX, VMAX == 4 ? 4 : 2, M, CK, false, SILU>());
     else if (VMAX == 8 && p.V == 4) go(D::template solo<T, 4, 4, M, CK, false, SILU>());
     else if (p.V == 2) go(D::template solo<T, 2, 4, M, CK, false, SILU>());
     else go(D::template solo<T, 1, 4, M, CK, false, SILU>());
   };
   if (p.mode == SOLO) solo(std::integral_constant<int, SOLO>());
-  else solo(std::integral_constant<int, HELD>());
+  else if constexpr (D::template held<CK>) solo(std::integral_constant<int, HELD>());
 }
 
 // one translation unit per direction and type

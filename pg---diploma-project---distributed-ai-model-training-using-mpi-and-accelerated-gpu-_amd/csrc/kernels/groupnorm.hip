@@ -192,7 +192,8 @@ size_t gn_lds(const Plan &p, bool bwd) {
   return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 : 1) * (size_t)p.g.cs + red);
 }
 
-Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) {
+// ck: with a checkpoint to write (forward); silu: backward through it
+Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd, bool silu) {
   if (C > 0x3fffffff) throw std::invalid_argument("group norm: C is too large");
   Plan p{};
   Geo &g = p.g;
@@ -223,7 +224,7 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
   };
   const int most = bwd ? 512 : 1024;
   const int nvs[3] = {2, 4, 8};
-  const int nv_most = bwd ? 4 : 8;
+  const int nv_most = bwd ? Bwd::most<SOLO, false> : Fwd::most<SOLO, false>;
   // solo: rows of 128 bytes at least, more while the tile is small and the chip stays full
   long long cs = (128 / elt + L - 1) / L * L;
   while (cs < C && S * cs * elt < 16384 && B * ((C + 2 * cs - 1) / (2 * cs)) >= 1024) cs *= 2;
@@ -258,10 +259,14 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd) 
     g.R = th / std::max(g.CVp, 1);
     return g.CVp <= th && gn_lds(p, bwd) <= 65536;
   };
-  // held: the fewest rows a thread with which all tiles are resident together
-  if (slabs(512)) {
+  // Held: the fewest rows a thread with which all tiles are resident together.  Calls of 96 x 784 x 192, 32 x
+  // 3136 x 96 and 16 x 3136 x 144, held and staged (us): forward 23, 21, 19 and 38, 24, 23; backward from a
+  // checkpoint 27, 25, 23 and 33, 29, 29, from x 30, 27, 23 and 33, 27, 27.  Where a checkpoint is written held
+  // is no faster with few rows (16 and 16) and has not the registers for 8 (35, 30, 25 and 40, 25, 22); silu's
+  // backward neither (52, 48 and 43, 33 with 8).
+  if (!(ck && !bwd) && slabs(512)) {
     for (int nv : nvs) {
-      if (only && nv != only) continue;
+      if ((only && nv != only) || (bwd && silu && nv > Bwd::most<HELD, true>)) continue;
       const long long rows = (long long)g.R * nv, k = (S + rows - 1) / rows;
       if (k > kHeldUnit || B * g.nslab * k > kHeld) continue;
       p.NV = nv;
@@ -329,17 +334,17 @@ void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M
 // tests: -1, what has come is not looked at
 void gn_set_wait(int polls) { g_wait = polls; }
 
-// dt: 0 bf16, 1 fp16, 2 fp32.  Forward and backward, with and without a checkpoint: the largest.
+// dt: 0 bf16, 1 fp16, 2 fp32.  With and without a checkpoint (forward) or silu (backward): the largest.
 long long gn_workspace_floats(int dt, long long B, long long S, int C, int G, int bwd) {
   if (B * S <= 0) return 0;
-  return std::max(gn_ws(gn_plan(dt, B, S, C, G, false, bwd), bwd).total,
-                  gn_ws(gn_plan(dt, B, S, C, G, true, bwd), bwd).total);
+  return std::max(gn_ws(gn_plan(dt, B, S, C, G, false, bwd, false), bwd).total,
+                  gn_ws(gn_plan(dt, B, S, C, G, true, bwd, true), bwd).total);
 }
 
 void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                    uint8_t *q, uint8_t *qs, float *ws, long long B, long long S, int C, int G, float eps, int act,
                    hipStream_t st) {
-  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, false);
+  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, false, false);
   const Ws w = gn_ws(p, false);
   const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<unsigned long long *>(ws + w.part), eps, act};
   gn_none(p, a.part, st);
@@ -356,7 +361,7 @@ void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta,
 void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, const uint8_t *qs, const float *gamma,
                    const float *beta, const float *mean, const float *rstd, void *dx, float *dgb, float *ws,
                    long long B, long long S, int C, int G, int act, hipStream_t st) {
-  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, true);
+  const Plan p = gn_plan(dt, B, S, C, G, false, true, act == GN_SILU);
   const Ws w = gn_ws(p, true);
   const BwdArgs a{p.g, dy, x, q, qs, gamma, beta, mean, rstd, dx, reinterpret_cast<unsigned long long *>(ws + w.part),
                   dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act};

@@ -9,13 +9,15 @@
 //   solo     a workgroup holds all S rows of a slab of whole groups in registers: one read
 //   held     the S rows are k tiles, and all tiles of the tensor are so few that their workgroups run
 //            together: each keeps its tile in registers, publishes its sums, waits for the k - 1
-//            others of its image and goes on.  One read.  (96 x 784 x 192 with checkpoint, backward: kernel 22.5
-//            us, 28.0 staged.  With more tiles than fit, a workgroup's chain load - sum - publish - wait -
-//            join - store is not hidden behind others': 128 x 12544 x 96 backward 1129 us.)
+//            others of its image and goes on.  One read.  (96 x 784 x 192 from a checkpoint, backward: 27
+//            us a call, 33 staged.  With more tiles than fit, a workgroup's chain load - sum - publish -
+//            wait - join - store is not hidden behind others': 128 x 12544 x 96 backward 1129 us.)
 //   staged   longer maps: the S rows are k tiles.  One launch holds a sums and a use workgroup for
 //            every tile; the use of an image's tiles is queued `lead` tiles behind its sums, so
 //            that it hardly ever waits for them and finds the tile in the memory-side cache
-//            (256 MB).  HBM sees every value once.
+//            (256 MB).  HBM sees every value once: 128 x 12544 x 96 backward reads 607 MB and
+//            writes 308 in 226 us, 4.1 TB/s; 128 x 3136 x 144 forward with checkpoint 289 MB in 75 us,
+//            3.8 TB/s.  What is left of a copy's 5.1 TB/s goes to a workgroup's latencies.
 //   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
 //            one workgroup per (image, group), then one value a thread.
 // A thread owns one vector of V channels (16 bytes where C allows) and every R-th row of the tile.

@@ -143,23 +143,23 @@ template <> PG_DEVICE f32x4_t wg_mfma<_Float16>(s16x8_t a, s16x8_t b, f32x4_t c)
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
 }
 
-// what a thread holds of a chunk: in one piece, or value by value where rows are not aligned
+// What a thread holds of a chunk: itself or, where rows are not aligned, the aligned words that it lies in,
+// `shift` bytes into the first.
 template <bool ALN> struct WgRaw {
   typedef uint4 a;
   typedef uint2 b;
-  static PG_DEVICE uint4 pack(const uint4 &v) { return v; }
-  static PG_DEVICE uint2 pack(const uint2 &v) { return v; }
+  static PG_DEVICE uint4 pack(const uint4 &v, uint32_t) { return v; }
+  static PG_DEVICE uint2 pack(const uint2 &v, uint32_t) { return v; }
 };
 template <> struct WgRaw<false> {
-  struct a { uint16_t v[8]; };
-  struct b { uint8_t v[8]; };
-  static PG_DEVICE uint4 pack(const a &x) {
-    return make_uint4(x.v[0] | (uint32_t)x.v[1] << 16, x.v[2] | (uint32_t)x.v[3] << 16, x.v[4] | (uint32_t)x.v[5] << 16,
-                      x.v[6] | (uint32_t)x.v[7] << 16);
+  struct a { uint4 v; uint32_t more; };
+  struct b { uint2 v; uint32_t more; };
+  static PG_DEVICE uint4 pack(const a &x, uint32_t shift) {
+    return make_uint4(__builtin_amdgcn_alignbyte(x.v.y, x.v.x, shift), __builtin_amdgcn_alignbyte(x.v.z, x.v.y, shift),
+                      __builtin_amdgcn_alignbyte(x.v.w, x.v.z, shift), __builtin_amdgcn_alignbyte(x.more, x.v.w, shift));
   }
-  static PG_DEVICE uint2 pack(const b &x) {
-    return make_uint2(x.v[0] | (uint32_t)x.v[1] << 8 | (uint32_t)x.v[2] << 16 | (uint32_t)x.v[3] << 24,
-                      x.v[4] | (uint32_t)x.v[5] << 8 | (uint32_t)x.v[6] << 16 | (uint32_t)x.v[7] << 24);
+  static PG_DEVICE uint2 pack(const b &x, uint32_t shift) {
+    return make_uint2(__builtin_amdgcn_alignbyte(x.v.y, x.v.x, shift), __builtin_amdgcn_alignbyte(x.more, x.v.y, shift));
   }
 };
 
@@ -210,8 +210,12 @@ __global__ __launch_bounds__(256) void mx8_wgrad_kernel(const WgradArgs a) {
   const int mb = split * a.rows, rows = min(a.M - mb, a.rows);
   // The split's rows through buffer descriptors: rows past its end, and columns past N or K (offset
   // kOOB), read as zeros, without a branch or a select that would wait for the load.
-  const rsrc_t ry = make_rsrc(static_cast<const T *>(a.dy) + (long long)mb * a.N, (uint32_t)rows * a.N * 2u);
-  const rsrc_t rq = make_rsrc(a.q + (long long)mb * a.K, (uint32_t)rows * a.K);
+  // (Unaligned rows are read in whole words: the last one may reach past the end, but not into another
+  // page, and a chunk's columns past N or K are another row's values, which reach only results that are
+  // not written. Rows past the split's end are masked there.)
+  auto bytes = [](uint32_t n) { return ALN ? n : (n + 3) & ~3u; };
+  const rsrc_t ry = make_rsrc(static_cast<const T *>(a.dy) + (long long)mb * a.N, bytes((uint32_t)rows * a.N * 2u));
+  const rsrc_t rq = make_rsrc(a.q + (long long)mb * a.K, bytes((uint32_t)rows * a.K));
   const rsrc_t rs = make_rsrc(a.qs + (long long)mb * a.nb, (uint32_t)rows * a.nb);
 
   struct Stage {
@@ -222,41 +226,32 @@ __global__ __launch_bounds__(256) void mx8_wgrad_kernel(const WgradArgs a) {
   // Chunk i of this thread: row t / CH + i * RS of the step, column t % CH * 8 (codes alike). Its
   // offsets for the next load; from kOOB on they stay outside, a split spans less than 2^31 bytes.
   const int na = n0 + t % CH * 8, kb = k0 + t % CH * 8;
-  constexpr int JA = ALN ? 1 : 8;
-  uint32_t oa[JA], ob[JA], oe = kb < a.K ? (uint32_t)(t / CH) * a.nb + kb / kMxBlock : kOOB;
-#pragma unroll
-  for (int j = 0; j < JA; ++j) {
-    oa[j] = na + j < a.N ? ((uint32_t)(t / CH) * a.N + na + j) * 2u : kOOB;
-    ob[j] = kb + j < a.K ? (uint32_t)(t / CH) * a.K + kb + j : kOOB;
-  }
+  uint32_t row = t / CH, oa = na < a.N ? (row * a.N + na) * 2u : kOOB, ob = kb < a.K ? row * a.K + kb : kOOB;
+  uint32_t oe = kb < a.K ? row * a.nb + kb / kMxBlock : kOOB;
+  const uint32_t sa = oa & 3u, sb = ob & 3u;   // of every chunk of this thread: RS and kMK are multiples of 4
+  oa -= sa;
+  ob -= sb;
   auto load = [&](Stage &g) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const uint32_t d = (uint32_t)(i * RS) * a.N * 2u;
+      const uint32_t m = i * RS, da = oa + m * a.N * 2u, db = ob + m * a.K;
       if constexpr (ALN) {
-        g.a[i] = bld16(ry, oa[0] + d);
+        g.a[i] = bld16(ry, da);
+        g.b[i] = bld8(rq, db);
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g.a[i].v[j] = __builtin_amdgcn_raw_buffer_load_b16(ry, (int)(oa[j] + d), 0, 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const uint32_t m = i * RS, d = m * a.K;
-      if constexpr (ALN) {
-        g.b[i] = bld8(rq, ob[0] + d);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) g.b[i].v[j] = __builtin_amdgcn_raw_buffer_load_b8(rq, (int)(ob[j] + d), 0, 0);
+        const bool in = row + m < (uint32_t)rows;
+        const uint32_t ia = in ? da : kOOB, ib = in ? db : kOOB;
+        g.a[i].v = bld16(ry, ia);
+        g.a[i].more = __builtin_amdgcn_raw_buffer_load_b32(ry, (int)(ia + 16), 0, 0);
+        g.b[i].v = bld8(rq, ib);
+        g.b[i].more = __builtin_amdgcn_raw_buffer_load_b32(rq, (int)(ib + 8), 0, 0);
       }
       g.e[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, (int)(oe + m * a.nb), 0, 0);
     }
-#pragma unroll
-    for (int j = 0; j < JA; ++j) {
-      oa[j] += kMK * 2u * a.N;
-      ob[j] += (uint32_t)kMK * a.K;
-    }
+    oa += kMK * 2u * a.N;
+    ob += (uint32_t)kMK * a.K;
     oe += (uint32_t)kMK * a.nb;
+    row += kMK;
   };
   float sum[8] = {};   // db: this thread's columns (a thread's chunks of dY are one column's, TH % CH == 0)
   const bool bias = a.db && k0 == 0;
@@ -264,19 +259,19 @@ __global__ __launch_bounds__(256) void mx8_wgrad_kernel(const WgradArgs a) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int r = t / CH + i * RS;
-      *reinterpret_cast<uint4 *>(smem[buf] + r * P + (t % CH * 16 ^ wg_swz<W>(r))) = WgRaw<ALN>::pack(g.a[i]);
+      *reinterpret_cast<uint4 *>(smem[buf] + r * P + (t % CH * 16 ^ wg_swz<W>(r))) = WgRaw<ALN>::pack(g.a[i], sa);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int r = t / CH + i * RS;
       *reinterpret_cast<uint4 *>(smem[buf] + kMK * P + r * P + (t % CH * 16 ^ wg_swz<W>(r))) =
-          wg_decode<T>(WgRaw<ALN>::pack(g.b[i]), g.e[i]);
+          wg_decode<T>(WgRaw<ALN>::pack(g.b[i], sb), g.e[i]);
     }
     if (bias)
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
         float v[8];
-        Vec<T, 8>::unpack(WgRaw<ALN>::pack(g.a[i]), v);
+        Vec<T, 8>::unpack(WgRaw<ALN>::pack(g.a[i], sa), v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += v[j];
       }

@@ -94,6 +94,27 @@ WG = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (31, 16, 33), (128, 1000, 2048), (100, 10
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("mnk", [(1, 1, 1), (3, 5, 7), (129, 33, 31), (1025, 65, 127), (641, 257, 3), (30001, 129, 65)])
+def test_wgrad_takes_nothing_from_behind_its_operands(mnk, dtype):
+    """Rows of odd lengths end inside a word: NaN in its other half, and after it, stays outside."""
+    M, N, Kd = mnk
+    dy, q, qs = wgrad_case(M, N, Kd, DT[dtype], M + 1)
+
+    def inside(t, fill):
+        big = torch.full((t.numel() + 4096,), fill, dtype=t.dtype, device="cuda")
+        big[:t.numel()] = t.reshape(-1)
+        return big[:t.numel()].view(t.shape)
+
+    out = []
+    for d, c, e in ((dy, q, qs), (inside(dy, float("nan")), inside(q, 127), inside(qs, 254))):
+        dw, db = torch.full((N, Kd), float("nan"), device="cuda"), torch.full((N,), float("nan"), device="cuda")
+        K.mx8_wgrad(d, c, e, dw, M, N, Kd, db=db)
+        out.append((dw, db))
+    assert torch.isfinite(out[0][0]).all() and torch.isfinite(out[0][1]).all()
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("mnk", WG)
 def test_wgrad(mnk, dtype):
     M, N, Kd = mnk

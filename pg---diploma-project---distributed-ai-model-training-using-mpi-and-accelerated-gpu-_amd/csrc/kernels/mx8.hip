@@ -5,11 +5,12 @@
 
 #include <algorithm>
 #include <stdexcept>
+#include <type_traits>
 
 namespace {
 constexpr int kHalfMax = 65504;
 
-// i / d by a multiplication while i * d < 2^32 (i is below d + 1024 here); m = ceil(2^32 / d)
+// i / d by a multiplication while i * d < 2^32 (i is below d + 8192 here); m = ceil(2^32 / d)
 struct FastDiv {
   uint32_t d, m;
   explicit FastDiv(uint32_t n) : d(n), m(n > 1 ? (uint32_t)(((1ull << 32) + n - 1) / n) : 0) {}
@@ -18,7 +19,9 @@ struct FastDiv {
 
 // Pack and unpack stream the matrix: V channels a thread, U of them in flight, neighbouring threads on
 // neighbouring vectors of a row.  Bound by memory: pack 401408 x 144 bf16 33 us, 5.3 TB/s; unpack 100352 x 960
-// bf16 50 us, 5.8 TB/s (a copy of 1 GiB: 5.1).  24999 x 75 fp16, value by value, 5.3 us: the launch.
+// bf16 50 us, 5.8 TB/s (a copy of 1 GiB: 5.1).
+// ANY: rows begin anywhere, and a row's last vector may be cut short: it is read from C - V on and shifted,
+// and its codes are written one by one.
 constexpr int kU = 4, kThreads = 256;
 
 // a workgroup's U * 256 slots of a [M][slots] grid: row and slot of the u-th of this thread
@@ -37,8 +40,37 @@ struct Slots {
   }
 };
 
+// what V values of a row have in memory at p, at any alignment of theirs, without the first `cut` values
+template <class R, class P> PG_DEVICE R load_cut(const P *p, int cut) {
+  R r;
+  __builtin_memcpy(&r, p, sizeof(R));
+  const uint32_t s = cut * (uint32_t)sizeof(P) * 8;
+  if constexpr (sizeof(R) == 16) {
+    const uint64_t lo = r.x | (uint64_t)r.y << 32, hi = r.z | (uint64_t)r.w << 32, t = s & 63;
+    const uint64_t l = s < 64 ? lo >> t | (t ? hi << (64 - t) : 0) : hi >> t, h = s < 64 ? hi >> t : 0;
+    return make_uint4((uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32));
+  } else if constexpr (sizeof(R) == 8) {
+    const uint64_t v = (r.x | (uint64_t)r.y << 32) >> s;
+    return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+  } else {
+    return r >> s;
+  }
+}
+// the first n of V values, at any alignment of theirs
+template <int V, class R, class P> PG_DEVICE void store_cut(P *p, const R &r, int n) {
+  if (n >= V) {
+    __builtin_memcpy(p, &r, sizeof(R));
+  } else {
+    struct alignas(sizeof(R)) Parts { P v[V]; };
+    const Parts a = __builtin_bit_cast(Parts, r);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < n) p[j] = a.v[j];
+  }
+}
+
 // slots of a row: its blocks' 32 / V vectors each (the last block's may lie past C)
-template <class T, int V>
+template <class T, int V, bool ANY>
 __global__ __launch_bounds__(kThreads) void mx8_pack_kernel(const T *__restrict__ x, uint8_t *__restrict__ q,
                                                             uint8_t *__restrict__ qs, long long M, int C, int nb,
                                                             FastDiv f) {
@@ -51,7 +83,12 @@ __global__ __launch_bounds__(kThreads) void mx8_pack_kernel(const T *__restrict_
     uint32_t slot;
     s.at(u, f, row, slot);
     const bool ok = row < M && slot * V < (uint32_t)C;
-    d[u] = *reinterpret_cast<const typename X::raw *>(x + (ok ? row * C + slot * V : 0));
+    if constexpr (ANY) {
+      const int cut = ok ? max(0, (int)(slot * V) + V - C) : 0;
+      d[u] = load_cut<typename X::raw>(x + (ok ? row * C + slot * V - cut : 0), cut);
+    } else {
+      d[u] = *reinterpret_cast<const typename X::raw *>(x + (ok ? row * C + slot * V : 0));
+    }
   }
 #pragma unroll
   for (int u = 0; u < kU; ++u) {
@@ -63,7 +100,9 @@ __global__ __launch_bounds__(kThreads) void mx8_pack_kernel(const T *__restrict_
     X::unpack(d[u], v);
     const int e = mx8_exp(block_amax<T, V>(d[u], ok));
     if (ok) {
-      *reinterpret_cast<typename Codes<V>::raw *>(q + row * C + slot * V) = Codes<V>::encode(v, mx8_inv_scale(e));
+      const typename Codes<V>::raw c = Codes<V>::encode(v, mx8_inv_scale(e));
+      if constexpr (ANY) store_cut<V>(q + row * C + slot * V, c, C - (int)(slot * V));
+      else *reinterpret_cast<typename Codes<V>::raw *>(q + row * C + slot * V) = c;
       if (slot % (kMxBlock / V) == 0) qs[row * nb + slot / (kMxBlock / V)] = (uint8_t)e;
     }
   }
@@ -101,6 +140,42 @@ __global__ __launch_bounds__(kThreads) void mx8_unpack_kernel(const uint8_t *__r
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = mx8_hold<T>(v[j]);
     if (row < M) *reinterpret_cast<typename Vec<T, V>::raw *>(x + row * C + slot * V) = Vec<T, V>::pack(v);
+  }
+}
+
+// Rows that begin anywhere: the matrix as one run of vectors, so that codes and values are aligned.
+// V neighbouring values lie in three blocks at most, whose scales are neighbours too.
+template <class T, int V>
+__global__ __launch_bounds__(kThreads) void mx8_unpack_run_kernel(const uint8_t *__restrict__ q,
+                                                                  const uint8_t *__restrict__ qs, T *__restrict__ x,
+                                                                  long long M, int C, int nb, FastDiv f) {
+  const unsigned long long first = (unsigned long long)blockIdx.x * (kU * kThreads * V);
+  const long long total = M * C, row0 = (long long)(first / (uint32_t)C), last = M * nb - 1;
+  const uint32_t rem = (uint32_t)(first % (uint32_t)C);
+  typename Codes<V>::raw d[kU];
+  uint8_t e[kU][3];
+  int n0[kU], n1[kU];   // values of the first and of the second block
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint32_t at = (u * kThreads + threadIdx.x) * V, local = rem + at, r = f.div(local), c = local - r * C;
+    const long long i = (long long)first + at, k = (row0 + r) * nb + c / kMxBlock;
+    const int cut = (int)min((long long)V, max(0ll, i + V - total));   // V: nothing left, the last vector is read
+    d[u] = load_cut<typename Codes<V>::raw>(q + min(i, total - V), cut % V);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) e[u][j] = qs[min(k + j, last)];
+    n0[u] = min(kMxBlock - (int)(c % kMxBlock), C - (int)c);
+    const int c1 = (int)c + n0[u];
+    n1[u] = n0[u] + min(kMxBlock, c1 < C ? C - c1 : C);
+  }
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const long long i = (long long)first + (u * kThreads + threadIdx.x) * V;
+    float v[V];
+    Codes<V>::decode(d[u], 1.f, v);
+    const float s0 = mx8_scale(e[u][0]), s1 = mx8_scale(e[u][1]), s2 = mx8_scale(e[u][2]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = mx8_hold<T>(v[j] * (j < n0[u] ? s0 : j < n1[u] ? s1 : s2));
+    if (i < total) store_cut<V>(x + i, Vec<T, V>::pack(v), (int)min((long long)V, total - i));
   }
 }
 
@@ -435,45 +510,56 @@ unsigned slot_grid(long long M, long long slots) {
   if (n > 0x7fffffff) throw std::invalid_argument("mx8: M * C is too large");
   return (unsigned)n;
 }
-int vec_of(int C, int most) {
-  while (C % most) most >>= 1;
-  return most;
+// Values a thread (16 bytes of them, or 8 where rows are a multiple of that only), and whether rows begin
+// anywhere. 400000 rows of 140, 142, 143 and 144 bf16: pack 37, 52, 55, 34 us (one and two values a thread
+// took 65 for 142 and 126 for 143), unpack 32 each (45 and 78); of 142 fp32 in twos 61 and 55 (as if at
+// any alignment: 69 and 71). Matrices narrower than 16 bytes go value by value.
+struct Lanes {
+  int V;
+  bool any;
+  Lanes(int C, int full) : V(C % full == full / 2 ? full / 2 : C % full == 0 || C >= full ? full : 1),
+                           any(V == full && C % full != 0) {}
+};
+template <int FULL, class F> void with_lanes(const Lanes &l, F f) {
+  typedef std::integral_constant<int, FULL> Full;
+  if (l.V == 1) f(std::integral_constant<int, 1>(), std::false_type());
+  else if (l.V == FULL / 2) f(std::integral_constant<int, FULL / 2>(), std::false_type());
+  else if (l.any) f(Full(), std::true_type());
+  else f(Full(), std::false_type());
 }
 }  // namespace
+
+template <class T> static void pack_go(const void *x, uint8_t *q, uint8_t *qs, long long M, int C, hipStream_t st) {
+  const int nb = (C + kMxBlock - 1) / kMxBlock, full = 16 / (int)sizeof(T);
+  const Lanes l(C, full);
+  const FastDiv f((uint32_t)nb * (kMxBlock / l.V));
+  const dim3 grid(slot_grid(M, f.d));
+  with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
+    hipLaunchKernelGGL((mx8_pack_kernel<T, decltype(v)::value, decltype(any)::value>), grid, dim3(kThreads), 0, st,
+                       (const T *)x, q, qs, M, C, nb, f);
+  });
+}
+template <class T> static void unpack_go(const uint8_t *q, const uint8_t *qs, void *x, long long M, int C, hipStream_t st) {
+  const int nb = (C + kMxBlock - 1) / kMxBlock;
+  const Lanes l(C, 16 / (int)sizeof(T));
+  const FastDiv f((uint32_t)(l.any ? C : C / l.V));
+  const dim3 grid(l.any ? slot_grid(1, M * C / l.V + 1) : slot_grid(M, f.d));
+  with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
+    constexpr int V = decltype(v)::value;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, q, qs, (T *)x, M, C, nb, f); };
+    if constexpr (decltype(any)::value) go(mx8_unpack_run_kernel<T, V>);
+    else go(mx8_unpack_kernel<T, V>);
+  });
+}
 
 // dt: 0 bf16, 1 fp16, 2 fp32
 void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M, int C, hipStream_t st) {
   if (M <= 0) return;
-  const int nb = (C + kMxBlock - 1) / kMxBlock, V = vec_of(C, dt == 2 ? 4 : 8);
-  const FastDiv f((uint32_t)nb * (kMxBlock / V));
-  const dim3 grid(slot_grid(M, f.d));
-#define PACK(T, N) hipLaunchKernelGGL((mx8_pack_kernel<T, N>), grid, dim3(kThreads), 0, st, (const T *)x, q, qs, M, C, nb, f)
-#define PACK_V(T)             \
-  if (V == 4) PACK(T, 4);     \
-  else if (V == 2) PACK(T, 2); \
-  else PACK(T, 1)
-  if (dt == 2) { PACK_V(float); }
-  else if (dt == 0) { if (V == 8) PACK(bf16_t, 8); else PACK_V(bf16_t); }
-  else { if (V == 8) PACK(_Float16, 8); else PACK_V(_Float16); }
-#undef PACK_V
-#undef PACK
+  (dt == 0 ? pack_go<bf16_t> : dt == 1 ? pack_go<_Float16> : pack_go<float>)(x, q, qs, M, C, st);
 }
-
 void launch_mx8_unpack(int dt, const uint8_t *q, const uint8_t *qs, void *x, long long M, int C, hipStream_t st) {
   if (M <= 0) return;
-  const int nb = (C + kMxBlock - 1) / kMxBlock, V = vec_of(C, dt == 2 ? 4 : 8);
-  const FastDiv f((uint32_t)(C / V));
-  const dim3 grid(slot_grid(M, f.d));
-#define UNPACK(T, N) hipLaunchKernelGGL((mx8_unpack_kernel<T, N>), grid, dim3(kThreads), 0, st, q, qs, (T *)x, M, C, nb, f)
-#define UNPACK_V(T)              \
-  if (V == 4) UNPACK(T, 4);      \
-  else if (V == 2) UNPACK(T, 2); \
-  else UNPACK(T, 1)
-  if (dt == 2) { UNPACK_V(float); }
-  else if (dt == 0) { if (V == 8) UNPACK(bf16_t, 8); else UNPACK_V(bf16_t); }
-  else { if (V == 8) UNPACK(_Float16, 8); else UNPACK_V(_Float16); }
-#undef UNPACK_V
-#undef UNPACK
+  (dt == 0 ? unpack_go<bf16_t> : dt == 1 ? unpack_go<_Float16> : unpack_go<float>)(q, qs, x, M, C, st);
 }
 
 long long mx8_wgrad_workspace_floats(int M, int N, int K) {

@@ -93,6 +93,24 @@ WG = [(1, 1, 1), (1, 8, 8), (3, 5, 7), (31, 16, 33), (128, 1000, 2048), (100, 10
       (513, 65, 129), (64, 256, 256), (2000, 96, 576), (20000, 17, 19), (9000, 320, 40), (33, 300, 257), (4097, 128, 128)]
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("C", [1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 15, 17, 31, 33, 34, 36, 39, 41, 63, 65, 95, 97, 129, 1001])
+def test_every_row_length_and_nothing_behind(C, dtype):
+    """Rows that begin at any alignment, matrices that end inside a vector, and the bytes behind them."""
+    for M in (1, 2, 5, 700):
+        g = torch.Generator(device="cuda").manual_seed(C * M)
+        x = (torch.randn(M, C, generator=g, device="cuda") * 2.0 ** torch.randint(-9, 9, (M, 1), generator=g, device="cuda")).to(DT[dtype])
+        q = torch.full((M * C + 64,), 77, dtype=torch.uint8, device="cuda")
+        qs = torch.full((M * K.mx8_blocks(C) + 64,), 77, dtype=torch.uint8, device="cuda")
+        K.mx8_pack(x, q[:M * C].view(M, C), qs[:-64].view(M, -1), M, C)
+        wq, ws = O.pack(x)
+        assert torch.equal(q[:M * C].view(M, C), wq) and torch.equal(qs[:-64].view(M, -1), ws)
+        y = torch.full((M * C + 64,), 77.0, dtype=DT[dtype], device="cuda")
+        K.mx8_unpack(wq, ws, y[:M * C].view(M, C), M, C)
+        assert torch.equal(y[:M * C].view(M, C), O.unpack(wq, ws).to(DT[dtype]))
+        assert (q[M * C:] == 77).all() and (qs[-64:] == 77).all() and (y[M * C:] == 77).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("mnk", [(1, 1, 1), (3, 5, 7), (129, 33, 31), (1025, 65, 127), (641, 257, 3), (30001, 129, 65)])
 def test_wgrad_takes_nothing_from_behind_its_operands(mnk, dtype):

@@ -23,6 +23,18 @@ def _rows(x):
     return x.clone() if x.data_ptr() % 16 else x
 
 
+def _like_rows(rows, C):
+    """An output of C channels for channels-last rows [B, ..., n]: ([B, C, ...], its [B, ..., C] alias). The first is
+    the tensor itself and the alias a view of it: autograd refuses in-place code behind an operator that returns a
+    view of its own making."""
+    shape, stride, n = (*rows.shape[:-1], C), [], 1
+    for d in reversed(shape):
+        stride.insert(0, n)
+        n *= max(d, 1)
+    y = torch.empty_strided((shape[0], C, *shape[1:-1]), (stride[0], 1, *stride[1:-1]), dtype=rows.dtype, device=rows.device)
+    return y, y.movedim(1, -1)
+
+
 def _vec(t):
     """A per-channel parameter as the kernels take it: fp32, contiguous, aligned."""
     if t is None:
@@ -49,16 +61,16 @@ class _GroupNormAct(torch.autograd.Function):
             B, C = xl.shape[0], xl.shape[-1]
             S = xl.numel() // (B * C) if B else 0
             w, b = _vec(weight), _vec(bias)
-            y = torch.empty_like(xl)
+            y, yl = _like_rows(xl, C)
             mean = torch.empty(B, groups, dtype=torch.float32, device=x.device)
             rstd = torch.empty_like(mean)
             keep = ckpt8 and any(ctx.needs_input_grad[:3])
             q, qs = _codes(B * S, C, x.device) if keep else (None, None)
-            K.gn_fwd(xl, w, b, y, mean, rstd, B, S, C, groups, eps=eps, act=act, q=q, qs=qs)
+            K.gn_fwd(xl, w, b, yl, mean, rstd, B, S, C, groups, eps=eps, act=act, q=q, qs=qs)
         ctx.save_for_backward(None if keep else xl, q, qs, w, b, mean, rstd)
         ctx.sizes = (B, S, C, groups, act)
         ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        return y.movedim(-1, 1)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -123,16 +135,17 @@ class _Conv1x1(torch.autograd.Function):
             N, C = weight.shape[:2]
             M = xl.numel() // C
             w = weight.detach().reshape(N, C).to(dtype)
-            y = xl.view(M, C) @ w.t()
+            y, yl = _like_rows(xl, N)
+            torch.mm(xl.view(M, C), w.t(), out=yl.view(M, N))
             if bias is not None:
-                y += bias.detach().to(dtype)
+                yl += bias.detach().to(dtype)
             q = qs = None
             if ctx.needs_input_grad[1]:
                 q, qs = _codes(M, C, x.device)
                 K.mx8_pack(xl, q, qs, M, C)
         ctx.save_for_backward(w if ctx.needs_input_grad[0] else None, q, qs)
         ctx.sizes = (M, N, C, x.dtype, weight.shape, weight.dtype, None if bias is None else bias.dtype)
-        return y.view(*xl.shape[:-1], N).movedim(-1, 1)
+        return y
 
     @staticmethod
     @once_differentiable

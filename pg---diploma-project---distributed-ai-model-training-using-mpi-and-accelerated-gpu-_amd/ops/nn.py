@@ -104,7 +104,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt
             raise ValueError(f"group_norm_act: {nm} must hold {C} values on {x.device}")
     if not x.is_cuda:
         return _PLAIN[act](F.group_norm(x, groups, weight, bias, eps))
-    return _GroupNormAct.apply(x, weight, bias, groups, eps, ACTS[act], ckpt8)
+    # needs_input_grad does not know of no_grad, and gradients are off within forward
+    return _GroupNormAct.apply(x, weight, bias, groups, eps, ACTS[act], ckpt8 and torch.is_grad_enabled())
 
 
 class GroupNormAct(nn.Module):
@@ -129,7 +130,7 @@ class GroupNormAct(nn.Module):
 
 class _Conv1x1(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, dtype):
+    def forward(ctx, x, weight, bias, dtype, grad):
         with _on(x):
             xl = _rows(x.to(dtype))
             N, C = weight.shape[:2]
@@ -140,7 +141,7 @@ class _Conv1x1(torch.autograd.Function):
             if bias is not None:
                 yl += bias.detach().to(dtype)
             q = qs = None
-            if ctx.needs_input_grad[1]:
+            if grad and ctx.needs_input_grad[1]:
                 q, qs = _codes(M, C, x.device)
                 K.mx8_pack(xl, q, qs, M, C)
         ctx.save_for_backward(w if ctx.needs_input_grad[0] else None, q, qs)
@@ -167,7 +168,7 @@ class _Conv1x1(torch.autograd.Function):
                 z = torch.zeros(M, 8, dtype=torch.uint8, device=dy.device)   # no input was kept: beside a product with zeros
                 K.mx8_wgrad(dyl, z, z.view(-1)[:M].view(M, 1), torch.empty(N, 8, dtype=torch.float32, device=dy.device),
                             M, N, 8, db=db)
-        return dx, dw, None if db is None else db.to(bdt), None
+        return dx, dw, None if db is None else db.to(bdt), None, None
 
 
 def conv1x1(x, weight, bias=None, stride=1):
@@ -181,7 +182,7 @@ def conv1x1(x, weight, bias=None, stride=1):
         return F.conv2d(x, weight, bias, stride)
     if stride != 1:
         x = x[:, :, ::stride, ::stride]
-    return _Conv1x1.apply(x, weight, bias, dtype)
+    return _Conv1x1.apply(x, weight, bias, dtype, torch.is_grad_enabled())
 
 
 class Conv1x1Ckpt8(nn.Conv2d):

@@ -39,3 +39,19 @@ def test_in_place_code_behind_an_output(op, layout):
 
     for plain, inside in ((torch.relu, torch.relu_), (lambda y: y + x, lambda y: y.add_(x))):
         assert all(torch.equal(a, c) for a, c in zip(run(inside), run(plain)))
+
+
+def test_no_checkpoint_is_made_where_no_gradient_is_wanted(monkeypatch):
+    made = []
+    fwd, pack = K.gn_fwd, K.mx8_pack
+    monkeypatch.setattr(K, "gn_fwd", lambda *a, **k: (made.append(("gn_fwd", k["q"] is not None)), fwd(*a, **k)))
+    monkeypatch.setattr(K, "mx8_pack", lambda *a, **k: (made.append(("mx8_pack", True)), pack(*a, **k)))
+    m = torch.nn.Sequential(N.Conv1x1Ckpt8(32, 64), N.GroupNormAct(8, 64, "relu", ckpt8=True)).cuda().to(BF)
+    x = randn(2, 32, 8, 8).to(BF)
+    want = m(x)
+    assert made == [("mx8_pack", True), ("gn_fwd", True)] and want.requires_grad
+    for off in (torch.no_grad, torch.inference_mode):
+        made.clear()
+        with off():
+            got = m(x)
+        assert made == [("gn_fwd", False)] and torch.equal(got, want)

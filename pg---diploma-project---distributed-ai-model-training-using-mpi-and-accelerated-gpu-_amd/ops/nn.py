@@ -5,6 +5,7 @@ first in shape) and hand channels-last operands to the kernels; a ``channels_las
 copied.  On a CPU tensor they are the plain torch operations, with exact gradients.
 """
 import contextlib
+from typing import Tuple, Union
 
 import torch
 import torch.nn.functional as F
@@ -172,24 +173,29 @@ class _Conv1x1(torch.autograd.Function):
 
 
 def conv1x1(x, weight, bias=None, stride=1):
-    """1x1 convolution of [B, C, H, W] (weight [N, C, 1, 1]) whose backward pass keeps its input as the
-    8-bit checkpoint (kernels.mx8_pack): dW and db come from kernels.mx8_wgrad.  On the GPU in bf16
-    or fp16 (the input's type, or autocast's); any other call is the plain convolution."""
+    """1x1 convolution of [B, C, H, W] (weight [N, C, 1, 1]; stride one number or one a direction) whose
+    backward pass keeps its input as the 8-bit checkpoint (kernels.mx8_pack): dW and db come from
+    kernels.mx8_wgrad.  On the GPU in bf16 or fp16 (the input's type, or autocast's); any other call is
+    the plain convolution."""
+    stride = tuple(stride) if isinstance(stride, (tuple, list)) else (stride,)
+    stride = stride * 2 if len(stride) == 1 else stride
+    if len(stride) != 2 or min(stride) < 1:
+        raise ValueError(f"conv1x1: stride {stride} must be a positive number or two")
     if x.dim() != 4 or weight.dim() != 4 or tuple(weight.shape[2:]) != (1, 1) or weight.shape[1] != x.shape[1]:
         raise ValueError(f"conv1x1: x [B, C, H, W] and weight [N, C, 1, 1], got {tuple(x.shape)}, {tuple(weight.shape)}")
     dtype = torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else x.dtype
     if not x.is_cuda or dtype not in (torch.bfloat16, torch.float16) or x.numel() == 0:
         return F.conv2d(x, weight, bias, stride)
-    if stride != 1:
-        x = x[:, :, ::stride, ::stride]
+    if stride != (1, 1):
+        x = x[:, :, ::stride[0], ::stride[1]]
     return _Conv1x1.apply(x, weight, bias, dtype, torch.is_grad_enabled())
 
 
 class Conv1x1Ckpt8(nn.Conv2d):
     """nn.Conv2d of kernel size 1 (no padding, no groups) through :func:`conv1x1`."""
 
-    def __init__(self, cin: int, cout: int, stride: int = 1, bias: bool = False):
+    def __init__(self, cin: int, cout: int, stride: Union[int, Tuple[int, int]] = 1, bias: bool = False):
         super().__init__(cin, cout, 1, stride, bias=bias)
 
     def forward(self, x):
-        return conv1x1(x, self.weight, self.bias, self.stride[0])
+        return conv1x1(x, self.weight, self.bias, self.stride)

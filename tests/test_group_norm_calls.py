@@ -1,0 +1,22 @@
+"""Group norm and 8-bit checkpoints as programs call them, without a GPU: arguments, checkpoints of models, plans."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from pgdist.ops import nn as N
+
+
+@pytest.mark.parametrize("stride", [1, 3, (2,), (1, 1), (2, 1), (1, 3), [3, 2]])
+def test_conv1x1_takes_a_stride_of_each_direction(stride):
+    x, w, b = torch.randn(2, 4, 11, 10), torch.randn(3, 4, 1, 1), torch.randn(3)
+    want = F.conv2d(x, w, b, stride)
+    assert torch.equal(N.conv1x1(x, w, b, stride), want)
+    m = N.Conv1x1Ckpt8(4, 3, stride, bias=True)
+    m.load_state_dict(dict(weight=w, bias=b))
+    assert torch.equal(m(x), want)
+
+
+@pytest.mark.parametrize("stride", [0, -1, (2, 0), (1, 2, 3), ()])
+def test_conv1x1_refuses_other_strides(stride):
+    with pytest.raises(ValueError, match="stride"):
+        N.conv1x1(torch.zeros(2, 4, 5, 5), torch.zeros(3, 4, 1, 1), stride=stride)

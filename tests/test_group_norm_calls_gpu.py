@@ -55,3 +55,30 @@ def test_no_checkpoint_is_made_where_no_gradient_is_wanted(monkeypatch):
         with off():
             got = m(x)
         assert made == [("gn_fwd", False)] and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("stride", [(1, 1), (2, 1), (1, 3), (2, 2), [3, 2]])
+def test_conv1x1_takes_a_stride_of_each_direction(stride):
+    x, w = randn(2, 16, 11, 10).to(BF), (0.2 * randn(24, 16, 1, 1, seed=1)).to(BF)
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = N.conv1x1(xs, ws, stride=stride)
+    sh, sw = stride
+    rows = x[:, :, ::sh, ::sw].movedim(1, -1)
+    want = rows.double() @ w.view(24, 16).double().t()
+    mag = rows.double().abs() @ w.view(24, 16).double().abs().t()
+    assert y.shape == (2, 24, -(-11 // sh), -(-10 // sw))
+    # one rounding of the product and its sums in fp32
+    assert ((y.movedim(1, -1).double() - want).abs() <= O.half(BF) * want.abs() + 32 * O.U * mag).all()
+    c = N.Conv1x1Ckpt8(16, 24, stride if isinstance(stride, tuple) else tuple(stride)).cuda().to(BF)
+    with torch.no_grad():
+        c.weight.copy_(w)
+        assert torch.equal(c(x), y)
+    dy = randn(*y.shape, seed=2).to(BF)
+    dx, dw = torch.autograd.grad(y, (xs, ws), dy)
+    d = dy.movedim(1, -1).reshape(-1, 24).double()
+    X = O.unpack(*O.pack(rows.reshape(-1, 16)))
+    want, mag = d.t().contiguous() @ X, d.abs().t().contiguous() @ X.abs()
+    assert ((dw.view(24, 16).double() - want).abs() <= O.half(BF) * want.abs() + 400 * O.U * mag).all()
+    hit = torch.zeros(11, 10, dtype=torch.bool, device="cuda")
+    hit[::sh, ::sw] = True
+    assert (dx[:, :, ~hit] == 0).all() and (dx[:, :, hit] != 0).any(1).all()

@@ -101,8 +101,8 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt
     if C < 1 or groups < 1 or C % groups:
         raise ValueError(f"group_norm_act: {groups} groups do not divide {C} channels")
     for t, nm in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.numel() != C or t.device != x.device):
-            raise ValueError(f"group_norm_act: {nm} must hold {C} values on {x.device}")
+        if t is not None and (t.shape != (C,) or t.device != x.device):
+            raise ValueError(f"group_norm_act: {nm} must be [{C}] on {x.device}, got {list(t.shape)} on {t.device}")
     if not x.is_cuda:
         return _PLAIN[act](F.group_norm(x, groups, weight, bias, eps))
     # needs_input_grad does not know of no_grad, and gradients are off within forward
@@ -183,6 +183,8 @@ def conv1x1(x, weight, bias=None, stride=1):
         raise ValueError(f"conv1x1: stride {stride} must be a positive number or two")
     if x.dim() != 4 or weight.dim() != 4 or tuple(weight.shape[2:]) != (1, 1) or weight.shape[1] != x.shape[1]:
         raise ValueError(f"conv1x1: x [B, C, H, W] and weight [N, C, 1, 1], got {tuple(x.shape)}, {tuple(weight.shape)}")
+    if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device):
+        raise ValueError(f"conv1x1: bias must be [{weight.shape[0]}] on {x.device}, got {list(bias.shape)} on {bias.device}")
     dtype = torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else x.dtype
     if not x.is_cuda or dtype not in (torch.bfloat16, torch.float16) or x.numel() == 0:
         return F.conv2d(x, weight, bias, stride)

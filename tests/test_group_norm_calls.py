@@ -20,3 +20,15 @@ def test_conv1x1_takes_a_stride_of_each_direction(stride):
 def test_conv1x1_refuses_other_strides(stride):
     with pytest.raises(ValueError, match="stride"):
         N.conv1x1(torch.zeros(2, 4, 5, 5), torch.zeros(3, 4, 1, 1), stride=stride)
+
+
+@pytest.mark.parametrize("shape", [(2, 2), (4, 1), (1, 4), (1,), (5,), ()])
+def test_parameters_of_other_shapes_are_refused(shape):
+    """Not only of other counts: their gradients would have another shape than they have."""
+    x, bad = torch.zeros(2, 4, 5, 5), torch.ones(shape)
+    for kw in (dict(weight=bad), dict(bias=bad)):
+        with pytest.raises(ValueError, match="must be"):
+            N.group_norm_act(x, 2, **kw)
+    for dt in (torch.float32, torch.bfloat16):
+        with pytest.raises(ValueError, match="must be"):
+            N.conv1x1(x.to(dt), torch.zeros(4, 4, 1, 1, dtype=dt), bad.to(dt))

@@ -82,3 +82,13 @@ def test_conv1x1_takes_a_stride_of_each_direction(stride):
     hit = torch.zeros(11, 10, dtype=torch.bool, device="cuda")
     hit[::sh, ::sw] = True
     assert (dx[:, :, ~hit] == 0).all() and (dx[:, :, hit] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 2), (4, 1), (1, 4), (1,), (5,), ()])
+def test_parameters_of_other_shapes_are_refused(shape):
+    x, bad = torch.zeros(2, 4, 5, 5, device="cuda"), torch.ones(shape, device="cuda")
+    for kw in (dict(weight=bad), dict(bias=bad)):
+        with pytest.raises(ValueError, match="must be"):
+            N.group_norm_act(x, 2, **kw)
+    with pytest.raises(ValueError, match="must be"):
+        N.conv1x1(x.to(BF), torch.zeros(4, 4, 1, 1, dtype=BF, device="cuda"), bad.to(BF))

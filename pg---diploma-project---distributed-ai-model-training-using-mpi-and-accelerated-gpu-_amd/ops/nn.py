@@ -185,7 +185,8 @@ def conv1x1(x, weight, bias=None, stride=1):
         raise ValueError(f"conv1x1: x [B, C, H, W] and weight [N, C, 1, 1], got {tuple(x.shape)}, {tuple(weight.shape)}")
     if bias is not None and (bias.shape != weight.shape[:1] or bias.device != x.device):
         raise ValueError(f"conv1x1: bias must be [{weight.shape[0]}] on {x.device}, got {list(bias.shape)} on {bias.device}")
-    dtype = torch.get_autocast_dtype("cuda") if x.is_cuda and torch.is_autocast_enabled("cuda") else x.dtype
+    cast = x.is_cuda and x.dtype != torch.float64 and torch.is_autocast_enabled("cuda")   # autocast leaves fp64 alone
+    dtype = torch.get_autocast_dtype("cuda") if cast else x.dtype
     if not x.is_cuda or dtype not in (torch.bfloat16, torch.float16) or x.numel() == 0:
         return F.conv2d(x, weight, bias, stride)
     if stride != (1, 1):

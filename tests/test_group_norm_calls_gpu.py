@@ -92,3 +92,12 @@ def test_parameters_of_other_shapes_are_refused(shape):
             N.group_norm_act(x, 2, **kw)
     with pytest.raises(ValueError, match="must be"):
         N.conv1x1(x.to(BF), torch.zeros(4, 4, 1, 1, dtype=BF, device="cuda"), bad.to(BF))
+
+
+def test_conv1x1_of_doubles_stays_double_under_autocast():
+    """Autocast leaves fp64 alone."""
+    x, w = randn(2, 16, 5, 5).double(), randn(8, 16, 1, 1, seed=1).double()
+    with torch.autocast("cuda", dtype=BF):
+        y = N.conv1x1(x, w)
+    want = (x.movedim(1, -1).cpu() @ w.view(8, 16).t().cpu()).movedim(-1, 1)
+    assert y.dtype == torch.float64 and (y.cpu() - want).abs().max() <= 1e-13 * 16 * want.abs().max()

@@ -112,7 +112,7 @@ void launch_reduce_metrics(const float *, const float *, int, double *, hipStrea
 long long gn_workspace_floats(int, long long, long long, int, int, int);
 void gn_set_wait(int);
 void launch_gn_fwd(int, const void *, const float *, const float *, void *, float *, float *, uint8_t *, uint8_t *,
-                   float *, long long, long long, int, int, float, int, hipStream_t);
+                   float *, long long, long long, int, int, float, int, int, hipStream_t);
 void launch_gn_bwd(int, const void *, const void *, const uint8_t *, const uint8_t *, const float *, const float *,
                    const float *, const float *, void *, float *, float *, long long, long long, int, int, int,
                    hipStream_t);
@@ -215,10 +215,11 @@ PYBIND11_MODULE(_pgdist_C, m) {
   m.def("gn_workspace_floats", &gn_workspace_floats);
   m.def("gn_set_wait", &gn_set_wait);
   m.def("gn_fwd", [](int dt, P x, P gamma, P beta, P y, P mean, P rstd, P q, P qs, P ws, long long B, long long S_,
-                     int C, int G, float eps, int act, P s) {
+                     int C, int G, float eps, int act, int as_ckpt8, P s) {
     pgdist_rt::run_op([=] {
       launch_gn_fwd(dt, ptr<void>(x), ptr<float>(gamma), ptr<float>(beta), ptr<void>(y), ptr<float>(mean),
-                    ptr<float>(rstd), ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<float>(ws), B, S_, C, G, eps, act, S(s));
+                    ptr<float>(rstd), ptr<uint8_t>(q), ptr<uint8_t>(qs), ptr<float>(ws), B, S_, C, G, eps, act, as_ckpt8,
+                    S(s));
       launched("gn_fwd");
     });
   });

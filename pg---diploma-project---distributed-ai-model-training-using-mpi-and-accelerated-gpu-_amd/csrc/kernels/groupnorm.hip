@@ -192,7 +192,7 @@ size_t gn_lds(const Plan &p, bool bwd) {
   return sizeof(float) * (2 * (size_t)p.g.gs + (bwd ? 6 : 1) * (size_t)p.g.cs + red);
 }
 
-// ck: with a checkpoint to write (forward); silu: backward through it
+// ck: with a checkpoint to write (forward), or as if there were; silu: backward through it
 Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd, bool silu) {
   if (C > 0x3fffffff) throw std::invalid_argument("group norm: C is too large");
   Plan p{};
@@ -343,8 +343,8 @@ long long gn_workspace_floats(int dt, long long B, long long S, int C, int G, in
 
 void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
                    uint8_t *q, uint8_t *qs, float *ws, long long B, long long S, int C, int G, float eps, int act,
-                   hipStream_t st) {
-  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr, false, false);
+                   int as_ckpt8, hipStream_t st) {
+  const Plan p = gn_plan(dt, B, S, C, G, q != nullptr || as_ckpt8, false, false);
   const Ws w = gn_ws(p, false);
   const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<unsigned long long *>(ws + w.part), eps, act};
   gn_none(p, a.part, st);

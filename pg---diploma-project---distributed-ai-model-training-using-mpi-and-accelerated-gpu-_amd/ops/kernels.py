@@ -1130,11 +1130,13 @@ def gn_workspace(B, S, C, G, dtype, bwd=False):
     return int(lib().gn_workspace_floats(_DT[dtype], B, S, C, G, int(bwd)))
 
 
-def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=None, qs=None, ws=None):
+def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=None, qs=None, ws=None,
+           as_ckpt8=False):
     """Group norm + activation of a channels-last [B, S, C] tensor (bf16, fp16 or fp32):
     y = act((x - mean) * rstd * gamma + beta), mean / rstd over the S * C/G values of each (image,
     group) and written as well (fp32 [B, G]; :func:`gn_bwd` reads them).  gamma / beta: fp32 [C] or
     None.  With q, qs the 8-bit checkpoint of x (:func:`mx8_pack` of [B*S, C]) is also written.
+    ``as_ckpt8`` without them: sums in the order of a call with them, so that y, mean and rstd have its bits.
     ``ws``: :func:`gn_workspace` floats for this call alone; None takes them from the allocator.
     No output may overlap another operand.  S = 0 gives mean 0, rstd 1/sqrt(eps)."""
     _gn_check("gn_fwd", x, B, S, C, G, act)
@@ -1158,7 +1160,7 @@ def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=N
         return
     ws = _workspace("gn_fwd", ws, gn_workspace(B, S, C, G, x.dtype), dev, outs + ins)
     lib().gn_fwd(_DT[x.dtype], px, pg, pb, py, pm, pr, pq, ps, 0 if ws is None else ws.data_ptr(), B, S, C, G,
-                 float(eps), act, _raw_stream(dev))
+                 float(eps), act, int(as_ckpt8), _raw_stream(dev))
 
 
 def gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=GN_NONE, q=None, qs=None, ws=None):

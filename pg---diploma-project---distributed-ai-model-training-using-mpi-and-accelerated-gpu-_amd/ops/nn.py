@@ -56,7 +56,7 @@ def _codes(M, C, device):
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, ckpt8):
+    def forward(ctx, x, weight, bias, groups, eps, act, ckpt8, grad):
         with _on(x):
             xl = _rows(x)
             B, C = xl.shape[0], xl.shape[-1]
@@ -65,9 +65,9 @@ class _GroupNormAct(torch.autograd.Function):
             y, yl = _like_rows(xl, C)
             mean = torch.empty(B, groups, dtype=torch.float32, device=x.device)
             rstd = torch.empty_like(mean)
-            keep = ckpt8 and any(ctx.needs_input_grad[:3])
+            keep = ckpt8 and grad and any(ctx.needs_input_grad[:3])
             q, qs = _codes(B * S, C, x.device) if keep else (None, None)
-            K.gn_fwd(xl, w, b, yl, mean, rstd, B, S, C, groups, eps=eps, act=act, q=q, qs=qs)
+            K.gn_fwd(xl, w, b, yl, mean, rstd, B, S, C, groups, eps=eps, act=act, q=q, qs=qs, as_ckpt8=ckpt8)
         ctx.save_for_backward(None if keep else xl, q, qs, w, b, mean, rstd)
         ctx.sizes = (B, S, C, groups, act)
         ctx.dtypes = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
@@ -86,13 +86,14 @@ class _GroupNormAct(torch.autograd.Function):
             K.gn_bwd(dyl, xl, w, b, mean, rstd, dx, dgb, B, S, C, groups, act=act, q=q, qs=qs)
         dw = dgb[0].to(ctx.dtypes[0]) if ctx.needs_input_grad[1] else None
         db = dgb[1].to(ctx.dtypes[1]) if ctx.needs_input_grad[2] else None
-        return dx.movedim(-1, 1) if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None
+        return dx.movedim(-1, 1) if ctx.needs_input_grad[0] else None, dw, db, None, None, None, None, None
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt8=False):
     """act(group_norm(x)) of [B, C, ...] with its gradients.  act: none, relu, relu6 or silu.
     ``ckpt8``: the backward pass keeps x as its 8-bit checkpoint (kernels.mx8_pack) instead of as it
-    is, and its gradients are those of the values that stands for."""
+    is, and its gradients are those of the values that stands for.  Without gradients none is made, and
+    the result has the same bits."""
     if act not in ACTS:
         raise ValueError(f"group_norm_act: unknown activation {act!r}; available: {sorted(ACTS)}")
     if x.dim() < 2:
@@ -106,7 +107,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt
     if not x.is_cuda:
         return _PLAIN[act](F.group_norm(x, groups, weight, bias, eps))
     # needs_input_grad does not know of no_grad, and gradients are off within forward
-    return _GroupNormAct.apply(x, weight, bias, groups, eps, ACTS[act], ckpt8 and torch.is_grad_enabled())
+    return _GroupNormAct.apply(x, weight, bias, groups, eps, ACTS[act], ckpt8, torch.is_grad_enabled())
 
 
 class GroupNormAct(nn.Module):

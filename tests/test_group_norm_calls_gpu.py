@@ -101,3 +101,35 @@ def test_conv1x1_of_doubles_stays_double_under_autocast():
         y = N.conv1x1(x, w)
     want = (x.movedim(1, -1).cpu() @ w.view(8, 16).t().cpu()).movedim(-1, 1)
     assert y.dtype == torch.float64 and (y.cpu() - want).abs().max() <= 1e-13 * 16 * want.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32])
+@pytest.mark.parametrize("size", [(2, 49, 24, 3), (3, 7, 30, 5), (1, 196, 576, 72), (8, 1024, 64, 8), (2, 3136, 144, 18),
+                                  (7, 3249, 100, 10), (64, 3136, 32, 4), (1, 60001, 96, 12), (8, 784, 625, 25),
+                                  (2, 9, 2049, 1), (3, 333, 264, 11)])
+def test_the_bits_of_a_call_with_a_checkpoint_without_one(size, dtype):
+    B, S, C, G = size
+    x, gamma, beta = randn(B, S, C).to(dtype), 1 + 0.1 * randn(C, seed=1), randn(C, seed=2)
+    outs = []
+    for ck in (True, False):
+        y, mean, rstd = torch.empty_like(x), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+        q = torch.empty(B * S, C, dtype=torch.uint8, device="cuda") if ck else None
+        qs = torch.empty(B * S, K.mx8_blocks(C), dtype=torch.uint8, device="cuda") if ck else None
+        K.gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, act=K.GN_SILU, q=q, qs=qs, as_ckpt8=True)
+        outs.append((y, mean, rstd))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("grad", ["no_grad", "inference_mode", "frozen"])
+def test_evaluation_has_the_bits_of_training(grad):
+    m = N.GroupNormAct(8, 64, "relu", ckpt8=True).cuda()
+    for seed in range(8):
+        x = randn(8, 64, 32, 32, seed=seed).to(BF).contiguous(memory_format=torch.channels_last)
+        want = m(x).detach()
+        if grad == "frozen":
+            got = m.requires_grad_(False)(x)
+            m.requires_grad_(True)
+        else:
+            with getattr(torch, grad)():
+                got = m(x)
+        assert torch.equal(got, want)

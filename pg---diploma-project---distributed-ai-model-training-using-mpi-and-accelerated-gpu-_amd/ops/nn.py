@@ -139,9 +139,10 @@ class _Conv1x1(torch.autograd.Function):
             M = xl.numel() // C
             w = weight.detach().reshape(N, C).to(dtype)
             y, yl = _like_rows(xl, N)
-            torch.mm(xl.view(M, C), w.t(), out=yl.view(M, N))
-            if bias is not None:
-                yl += bias.detach().to(dtype)
+            if bias is None:
+                torch.mm(xl.view(M, C), w.t(), out=yl.view(M, N))
+            else:   # the bias joins the product's fp32 sums: one rounding
+                torch.addmm(bias.detach().to(dtype), xl.view(M, C), w.t(), out=yl.view(M, N))
             q = qs = None
             if grad and ctx.needs_input_grad[1]:
                 q, qs = _codes(M, C, x.device)

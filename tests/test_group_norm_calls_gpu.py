@@ -133,3 +133,14 @@ def test_evaluation_has_the_bits_of_training(grad):
             with getattr(torch, grad)():
                 got = m(x)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,last", [(BF, 8), (torch.float16, 11)])
+def test_conv1x1_rounds_product_and_bias_once(dtype, last):
+    """2^last + 1 takes a bit more than the type has, so rounded by itself it loses the 1; with a bias of 1 the sum
+    2^last + 2 is held exactly."""
+    x = torch.ones(1, 8, 2, 2, dtype=dtype, device="cuda")
+    w = torch.zeros(8, 8, 1, 1, dtype=dtype, device="cuda")
+    w[:, 0], w[:, 1] = 2.0 ** last, 1.0
+    b = torch.ones(8, dtype=dtype, device="cuda")
+    assert (N.conv1x1(x, w, b) == 2 ** last + 2).all()

@@ -605,14 +605,14 @@ struct BwdArgs {
 // Which values of a channel relu and relu6 pass: lo < x < hi.  0 < z (and z < 6) is a condition on x
 // itself, x > mean - beta / (rstd gamma) or < where gamma < 0.  The border is found in 64 bits, once a
 // channel, and rounded away from the side that passes, so the comparison of x, which is exact in
-// fp32, with it tells what z in 64 bits would: no rounding of z takes part.
+// fp32, with it tells what z in 64 bits would: no rounding of z takes part.  A border that is not there is
+// NaN: nothing, infinities among them, lies behind it (a NaN z, of a group with infinite values, passes).
 PG_DEVICE void gn_border(int act, float mean, float rstd, float gamma, float beta, float &lo, float &hi) {
   const double k = (double)rstd * (double)gamma, b = beta;
-  lo = -INFINITY;
-  hi = INFINITY;
+  lo = hi = NAN;
   if (act != GN_RELU && act != GN_RELU6) return;
   if (k == 0.0) {   // z is beta everywhere
-    if (!(beta > 0.f) || (act == GN_RELU6 && !(beta < 6.f))) lo = INFINITY;
+    if (beta <= 0.f || (act == GN_RELU6 && beta >= 6.f)) lo = INFINITY;
     return;
   }
   const double r = 1.0 / k, t0 = fma(-b, r, (double)mean), t6 = fma(6.0 - b, r, (double)mean);

@@ -144,3 +144,26 @@ def test_conv1x1_rounds_product_and_bias_once(dtype, last):
     w[:, 0], w[:, 1] = 2.0 ** last, 1.0
     b = torch.ones(8, dtype=dtype, device="cuda")
     assert (N.conv1x1(x, w, b) == 2 ** last + 2).all()
+
+
+@pytest.mark.parametrize("size", [(2, 60, 64, 8), (2, 3001, 96, 12), (2, 60001, 96, 12), (1, 9, 2049, 1)])
+@pytest.mark.parametrize("act", [0, 1, 2])
+def test_infinite_inputs_keep_their_term_of_dbeta(size, act):
+    """Without a border dz is dy whatever x is; where the statistics are NaN, z is, and NaN passes."""
+    B, S, C, G = size
+    x, dy = randn(B, S, C), randn(B, S, C, seed=1).round()   # whole numbers: dbeta is exact
+    x[0, S // 2, 3] = float("inf")
+    x[B - 1, S // 3, C - 1] = -float("inf")
+    dy[0, S // 2, 3] = dy[B - 1, S // 3, C - 1] = 2
+    one, zero = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    y, mean, rstd = torch.empty_like(x), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+    K.gn_fwd(x, one, zero, y, mean, rstd, B, S, C, G, act=act)
+    dx, dgb = torch.empty_like(x), torch.empty(2, C, device="cuda")
+    K.gn_bwd(dy, x, one, zero, mean, rstd, dx, dgb, B, S, C, G, act=act)
+    cg = C // G
+    z = ((x.view(B, S, G, cg).double() - mean.view(B, 1, G, 1)) * rstd.view(B, 1, G, 1).double()).view(B, S, C)
+    out = (z <= 0) if act else torch.zeros_like(z, dtype=torch.bool)
+    if act == 2:
+        out |= z >= 6
+    assert torch.isnan(z[0, :, 3]).all() and torch.isnan(z[B - 1, :, C - 1]).all()
+    assert torch.equal(dgb[1].double(), torch.where(out, 0.0, dy.double()).sum((0, 1)))

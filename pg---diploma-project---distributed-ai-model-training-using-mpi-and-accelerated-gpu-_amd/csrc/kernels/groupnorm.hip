@@ -9,8 +9,13 @@
 using namespace gn;
 
 namespace {
+// Work-items of a launch: the runtime takes 2^32 and more without a word and runs what is left modulo 2^32
+// (gn_bwd of 2050 x 2 x 8200 left most gradients unwritten).
+constexpr long long kMostItems = 0xffffffffll;
+constexpr long long kMostWgs = 65536;   // of kernels that loop: more than are resident, many times over
+
 // ---- wide groups: not tuned, every access one value -----------------------------------------------
-// A plain loop over memory: C / G of thousands of channels, or over a thousand of an odd number.
+// Plain loops over memory, with grids of kMostWgs workgroups at most: C / G of thousands of channels, or over a thousand of an odd number.
 PG_DEVICE float load_one(const void *x, int dt, long long i) {
   return dt == 0 ? bf2f(static_cast<const bf16_t *>(x)[i])
                  : dt == 1 ? (float)static_cast<const _Float16 *>(x)[i] : static_cast<const float *>(x)[i];
@@ -31,18 +36,21 @@ PG_DEVICE float block_sum(float v) {   // 256 threads
 
 __global__ __launch_bounds__(256) void gn_wide_stats_kernel(const FwdArgs a, int dt) {
   const Geo &g = a.g;
-  const long long n = g.S * g.cg, base = blockIdx.x / g.G * g.S * g.C + (long long)(blockIdx.x % g.G) * g.cg;
-  float s = 0.f, v = 0.f;
-  for (long long i = threadIdx.x; i < n; i += 256) s += load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg);
-  const float mu = block_sum(s) / (float)n;
-  for (long long i = threadIdx.x; i < n; i += 256) {
-    const float d = load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg) - mu;
-    v = fmaf(d, d, v);
-  }
-  v = block_sum(v);
-  if (threadIdx.x == 0) {
-    a.mean[blockIdx.x] = mu;
-    a.rstd[blockIdx.x] = 1.f / sqrtf(v / (float)n + a.eps);
+  const long long n = g.S * g.cg;
+  for (long long k = blockIdx.x; k < g.B * g.G; k += gridDim.x) {
+    const long long base = k / g.G * g.S * g.C + k % g.G * g.cg;
+    float s = 0.f, v = 0.f;
+    for (long long i = threadIdx.x; i < n; i += 256) s += load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg);
+    const float mu = block_sum(s) / (float)n;
+    for (long long i = threadIdx.x; i < n; i += 256) {
+      const float d = load_one(a.x, dt, base + i / g.cg * g.C + i % g.cg) - mu;
+      v = fmaf(d, d, v);
+    }
+    v = block_sum(v);
+    if (threadIdx.x == 0) {
+      a.mean[k] = mu;
+      a.rstd[k] = 1.f / sqrtf(v / (float)n + a.eps);
+    }
   }
 }
 __global__ __launch_bounds__(256) void gn_wide_apply_kernel(const FwdArgs a, int dt) {
@@ -75,39 +83,41 @@ PG_DEVICE void wide_dz(const BwdArgs &a, int dt, long long r, int c, float &df, 
     dz = gn_dz<false>(dy, x, df, lo, hi);
   }
 }
-// one workgroup per (image, channel) -> dpart [B][2][C]
+// a workgroup at a time per (image, channel) -> dpart [B][2][C]
 __global__ __launch_bounds__(256) void gn_wide_dsums_kernel(const BwdArgs a, int dt) {
   const Geo &g = a.g;
-  const long long b = blockIdx.x / g.C;
-  const int c = (int)(blockIdx.x % g.C);
-  float s0 = 0.f, s1 = 0.f, df, al, dz;
-  for (long long s = threadIdx.x; s < g.S; s += 256) {
-    wide_dz(a, dt, b * g.S + s, c, df, al, dz);
-    s0 += dz;
-    s1 = fmaf(dz, df, s1);
-  }
-  s0 = block_sum(s0);
-  s1 = block_sum(s1);
-  if (threadIdx.x == 0) {
-    a.dpart[b * 2 * g.C + c] = s1 * a.rstd[b * g.G + c / g.cg];
-    a.dpart[(b * 2 + 1) * g.C + c] = s0;
+  for (long long k = blockIdx.x; k < g.B * g.C; k += gridDim.x) {
+    const long long b = k / g.C;
+    const int c = (int)(k % g.C);
+    float s0 = 0.f, s1 = 0.f, df, al, dz;
+    for (long long s = threadIdx.x; s < g.S; s += 256) {
+      wide_dz(a, dt, b * g.S + s, c, df, al, dz);
+      s0 += dz;
+      s1 = fmaf(dz, df, s1);
+    }
+    s0 = block_sum(s0);
+    s1 = block_sum(s1);
+    if (threadIdx.x == 0) {
+      a.dpart[b * 2 * g.C + c] = s1 * a.rstd[b * g.G + c / g.cg];
+      a.dpart[(b * 2 + 1) * g.C + c] = s0;
+    }
   }
 }
-// one workgroup per (image, group) -> part [B * G][2]
+// a workgroup at a time per (image, group) -> part [B * G][2]
 __global__ __launch_bounds__(256) void gn_wide_gsums_kernel(const BwdArgs a) {
   const Geo &g = a.g;
-  const long long b = blockIdx.x / g.G;
-  const int c0 = (int)(blockIdx.x % g.G) * g.cg;
-  float u = 0.f, v = 0.f;
-  for (int c = c0 + threadIdx.x; c < c0 + g.cg; c += 256) {
-    const float ga = a.gamma ? a.gamma[c] : 1.f;
-    v = fmaf(ga, a.dpart[b * 2 * g.C + c], v);
-    u = fmaf(ga, a.dpart[(b * 2 + 1) * g.C + c], u);
-  }
-  u = block_sum(u);
-  v = block_sum(v);
-  if (threadIdx.x == 0) {
-    pair_store(a.part + blockIdx.x, u, v);
+  for (long long k = blockIdx.x; k < g.B * g.G; k += gridDim.x) {
+    const long long b = k / g.G;
+    const int c0 = (int)(k % g.G) * g.cg;
+    float u = 0.f, v = 0.f;
+    for (int c = c0 + threadIdx.x; c < c0 + g.cg; c += 256) {
+      const float ga = a.gamma ? a.gamma[c] : 1.f;
+      v = fmaf(ga, a.dpart[b * 2 * g.C + c], v);
+      u = fmaf(ga, a.dpart[(b * 2 + 1) * g.C + c], u);
+    }
+    u = block_sum(u);
+    v = block_sum(v);
+    if (threadIdx.x == 0) pair_store(a.part + k, u, v);
   }
 }
 __global__ __launch_bounds__(256) void gn_wide_dx_kernel(const BwdArgs a, int dt) {
@@ -131,28 +141,32 @@ __global__ __launch_bounds__(256) void gn_wide_dx_kernel(const BwdArgs a, int dt
 __global__ __launch_bounds__(1024) void gn_dparam_kernel(const float *__restrict__ part, float *__restrict__ dst,
                                                          long long rows, int n, int split) {
   __shared__ float sh[16][64];
-  const int col = threadIdx.x & 63, st = threadIdx.x >> 6, j = blockIdx.x * 64 + col;
+  const int col = threadIdx.x & 63, st = threadIdx.x >> 6;
   const long long r0 = (long long)blockIdx.y * split, r1 = min(rows, r0 + split);
-  float s = 0.f;
-  if (j < n) {   // eight rows in flight
-    float v[8] = {};
-    long long r = r0 + st;
-    for (; r + 7 * 16 < r1; r += 8 * 16) {
+#pragma unroll 1
+  for (long long j = blockIdx.x * 64ll + col; j - col < n; j += gridDim.x * 64ll) {
+    float s = 0.f;
+    if (j < n) {   // eight rows in flight
+      float v[8] = {};
+      long long r = r0 + st;
+      for (; r + 7 * 16 < r1; r += 8 * 16) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] += part[(r + u * 16) * n + j];
+        for (int u = 0; u < 8; ++u) v[u] += part[(r + u * 16) * n + j];
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[0] += r + u * 16 < r1 ? part[(r + u * 16) * n + j] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
     }
+    sh[st][col] = s;
+    __syncthreads();
+    if (st == 0 && j < n) {
+      s = 0.f;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[0] += r + u * 16 < r1 ? part[(r + u * 16) * n + j] : 0.f;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) s += v[u];
-  }
-  sh[st][col] = s;
-  __syncthreads();
-  if (st == 0 && j < n) {
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += sh[i][col];
-    dst[(size_t)blockIdx.y * n + j] = s;
+      for (int i = 0; i < 16; ++i) s += sh[i][col];
+      dst[(size_t)blockIdx.y * n + j] = s;
+    }
+    __syncthreads();   // sh has been read
   }
 }
 
@@ -219,7 +233,8 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd, 
     g.CVp = (g.cs / V + Q - 1) / Q * Q;
   };
   auto check = [&](long long k) {   // grid and in-tile offsets
-    if (k > 0x7fffffff || p.wgs > 0x7fffffff || (long long)std::max(g.turn, g.R * p.NV) * C * elt > 0x7fffffff)
+    const bool grid = p.mode == SOLO || p.wgs <= kMostItems / p.TH;   // solo: in as many launches as it takes
+    if (k > 0x7fffffff || !grid || (long long)std::max(g.turn, g.R * p.NV) * C * elt > 0x7fffffff)
       throw std::invalid_argument("group norm: sizes past the kernels' 32-bit grid and tile offsets");
   };
   const int most = bwd ? 512 : 1024;
@@ -283,7 +298,6 @@ Plan gn_plan(int dt, long long B, long long S, int C, int G, bool ck, bool bwd, 
     g.k = 1;
     g.nslab = G;   // sums per (image, group)
     g.gs = 1;
-    p.wgs = B * G;
     return p;
   }
   // tiles of up to kRounds rounds, fewer while the tiles do not fill the chip several times
@@ -322,6 +336,20 @@ Ws gn_ws(const Plan &p, bool bwd) {
   return w;
 }
 
+dim3 looped(long long wgs) { return dim3((unsigned)std::min(wgs, kMostWgs)); }
+
+// one launch, or (solo, whose images have nothing to do with one another) as many as the grid needs: f(plan of the
+// launch, its first image)
+template <class F> void launches(const Plan &p, F f) {
+  if (p.mode != SOLO) return f(p, 0);
+  const long long most = std::max<long long>(1, kMostItems / p.TH / p.g.nslab);
+  for (long long b = 0; b < p.g.B; b += most) {
+    Plan part = p;
+    part.wgs = std::min(most, p.g.B - b) * p.g.nslab;
+    f(part, b);
+  }
+}
+
 void gn_none(const Plan &p, unsigned long long *part, hipStream_t st) {
   if (p.mode != STAGED && p.mode != HELD) return;
   const long long n = p.g.B * p.g.nslab * p.g.k * p.g.gs;
@@ -349,13 +377,24 @@ void launch_gn_fwd(int dt, const void *x, const float *gamma, const float *beta,
   const FwdArgs a{p.g, x, gamma, beta, y, mean, rstd, q, qs, reinterpret_cast<unsigned long long *>(ws + w.part), eps, act};
   gn_none(p, a.part, st);
   if (p.mode == WIDE) {
-    const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));
-    hipLaunchKernelGGL(gn_wide_stats_kernel, dim3((unsigned)p.wgs), dim3(256), 0, st, a, dt);
-    hipLaunchKernelGGL(gn_wide_apply_kernel, grid, dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_stats_kernel, looped(B * G), dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_apply_kernel, looped((B * S * C + 255) / 256), dim3(256), 0, st, a, dt);
     if (q) launch_mx8_pack(dt, x, q, qs, B * S, C, st);
     return;
   }
-  (dt == 0 ? fwd_bf16 : dt == 1 ? fwd_fp16 : fwd_fp32)(p, gn_lds(p, false), a, st);
+  const long long e = dt == 2 ? 4 : 2, nb = (C + kMxBlock - 1) / kMxBlock;
+  launches(p, [&](const Plan &part, long long b) {
+    FwdArgs t = a;
+    t.x = static_cast<const char *>(x) + b * S * C * e;
+    t.y = static_cast<char *>(y) + b * S * C * e;
+    t.mean += b * G;
+    t.rstd += b * G;
+    if (q) {
+      t.q += b * S * C;
+      t.qs += b * S * nb;
+    }
+    (dt == 0 ? fwd_bf16 : dt == 1 ? fwd_fp16 : fwd_fp32)(part, gn_lds(p, false), t, st);
+  });
 }
 
 void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, const uint8_t *qs, const float *gamma,
@@ -367,17 +406,30 @@ void launch_gn_bwd(int dt, const void *dy, const void *x, const uint8_t *q, cons
                   dgb || p.mode == WIDE ? ws + w.dpart : nullptr, act};
   gn_none(p, a.part, st);
   if (p.mode == WIDE) {
-    if (B * C > 0x7fffffff) throw std::invalid_argument("gn_bwd: B * C is too large");
-    const dim3 grid((unsigned)std::min<long long>((B * S * C + 255) / 256, 65536));
-    hipLaunchKernelGGL(gn_wide_dsums_kernel, dim3((unsigned)(B * C)), dim3(256), 0, st, a, dt);
-    hipLaunchKernelGGL(gn_wide_gsums_kernel, dim3((unsigned)p.wgs), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(gn_wide_dx_kernel, grid, dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_dsums_kernel, looped(B * C), dim3(256), 0, st, a, dt);
+    hipLaunchKernelGGL(gn_wide_gsums_kernel, looped(B * G), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(gn_wide_dx_kernel, looped((B * S * C + 255) / 256), dim3(256), 0, st, a, dt);
   } else {
-    (dt == 0 ? bwd_bf16 : dt == 1 ? bwd_fp16 : bwd_fp32)(p, gn_lds(p, true), a, st);
+    const long long e = dt == 2 ? 4 : 2, nb = (C + kMxBlock - 1) / kMxBlock;
+    launches(p, [&](const Plan &part, long long b) {
+      BwdArgs t = a;
+      t.dy = static_cast<const char *>(dy) + b * S * C * e;
+      t.dx = static_cast<char *>(dx) + b * S * C * e;
+      if (q) {
+        t.q += b * S * C;
+        t.qs += b * S * nb;
+      } else {
+        t.x = static_cast<const char *>(x) + b * S * C * e;
+      }
+      t.mean += b * G;
+      t.rstd += b * G;
+      if (t.dpart) t.dpart += b * 2 * C;
+      (dt == 0 ? bwd_bf16 : dt == 1 ? bwd_fp16 : bwd_fp32)(part, gn_lds(p, true), t, st);
+    });
   }
   if (!dgb) return;
   const long long rows = B * p.g.k;
-  const unsigned nb = (2 * C + 63) / 64;
+  const unsigned nb = looped((2ll * C + 63) / 64).x;
   if (rows > 16 * kSplitRows) {
     const int split = (int)((rows + kSplitRows - 1) / kSplitRows), ns = (int)((rows + split - 1) / split);
     hipLaunchKernelGGL(gn_dparam_kernel, dim3(nb, ns), dim3(1024), 0, st, ws + w.dpart, ws + w.lvl, rows, 2 * C, split);

@@ -32,3 +32,12 @@ def test_parameters_of_other_shapes_are_refused(shape):
     for dt in (torch.float32, torch.bfloat16):
         with pytest.raises(ValueError, match="must be"):
             N.conv1x1(x.to(dt), torch.zeros(4, 4, 1, 1, dtype=dt), bad.to(dt))
+
+
+def test_sizes_past_the_grid_are_refused():
+    """Tiles that wait for one another come in one launch; the runtime would take 2^32 work-items and more for fewer."""
+    from pgdist.ops import kernels as K
+    for bwd in (False, True):
+        with pytest.raises(ValueError, match="32-bit grid"):
+            K.gn_workspace(1 << 24, 3136, 64, 8, torch.bfloat16, bwd)
+        assert K.gn_workspace(1 << 27, 1, 8, 1, torch.bfloat16, bwd) >= 0   # images of their own: several launches

@@ -167,3 +167,63 @@ def test_infinite_inputs_keep_their_term_of_dbeta(size, act):
         out |= z >= 6
     assert torch.isnan(z[0, :, 3]).all() and torch.isnan(z[B - 1, :, C - 1]).all()
     assert torch.equal(dgb[1].double(), torch.where(out, 0.0, dy.double()).sum((0, 1)))
+
+
+def test_many_images_of_wide_groups():
+    """More (image, channel) pairs than one launch has workgroups for."""
+    B, S, C, G = 2050, 2, 8200, 1
+    x, dy = randn(B, S, C).to(BF), randn(B, S, C, seed=1).to(BF)
+    gamma, beta = 1 + 0.1 * randn(C, seed=2), randn(C, seed=3)
+    y, mean, rstd = torch.empty_like(x), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+    K.gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, act=1)
+    want, bound = O.fwd(x, gamma, beta, B, S, C, G, 1e-5, 1)
+    for got, w, b in zip((y, mean, rstd), want, bound):
+        O.within(got, w, b)
+    dx, dgb = torch.full_like(x, float("nan")), torch.full((2, C), float("nan"), device="cuda")
+    K.gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=1)
+    want, bound = O.bwd(dy, x, gamma, beta, mean, rstd, B, S, C, G, 1)
+    for got, w, b in zip((dx, dgb[0], dgb[1]), want, bound):
+        O.within(got, w, b)
+
+
+@pytest.mark.parametrize("ck", [False, True])
+def test_more_images_than_one_launch_has_workgroups_for(ck):
+    """The images on both sides of the first launch's end, and the last, as they come out alone."""
+    B, S, C, G = (1 << 26) + 70, 1, 8, 1
+    x, dy = torch.ones(B, S, C, dtype=BF, device="cuda"), torch.zeros(B, S, C, dtype=BF, device="cuda")
+    parts = [slice(0, 64), slice((1 << 26) - 80, (1 << 26) + 6), slice(B - 64, B)]
+    for i, p in enumerate(parts):
+        n = p.stop - p.start
+        x[p], dy[p] = randn(n, S, C, seed=i).to(BF), randn(n, S, C, seed=9 + i).round().to(BF)
+    y, dx = torch.full_like(x, 7), torch.full_like(x, 7)
+    mean, rstd, dgb = torch.full((B, G), 7.0, device="cuda"), torch.full((B, G), 7.0, device="cuda"), torch.empty(2, C, device="cuda")
+    q = torch.zeros(B, C, dtype=torch.uint8, device="cuda") if ck else None
+    qs = torch.zeros(B, 1, dtype=torch.uint8, device="cuda") if ck else None
+    K.gn_fwd(x, None, None, y, mean, rstd, B, S, C, G, q=q, qs=qs)
+    K.gn_bwd(dy, None if ck else x, None, None, mean, rstd, dx, dgb, B, S, C, G, q=q, qs=qs)
+    for p in parts:
+        n = p.stop - p.start
+        want = [torch.empty_like(t[p]) for t in (y, mean, rstd)]
+        wq = [torch.empty_like(t[p]) for t in (q, qs)] if ck else [None, None]
+        K.gn_fwd(x[p].clone(), None, None, *want, n, S, C, G, q=wq[0], qs=wq[1])
+        wdx = torch.empty_like(x[p])
+        K.gn_bwd(dy[p].clone(), None if ck else x[p].clone(), None, None, *want[1:], wdx, None, n, S, C, G, q=wq[0], qs=wq[1])
+        assert all(torch.equal(t[p], w) for t, w in zip((y, mean, rstd, dx), (*want, wdx)))
+        assert not ck or (torch.equal(q[p], wq[0]) and torch.equal(qs[p], wq[1]))
+    assert bool((mean[64:parts[1].start] == 1).all()) and bool((dx[64:parts[1].start] == 0).all())
+    assert torch.equal(dgb[1].double(), sum(dy[p].double().sum((0, 1)) for p in parts))   # whole numbers
+
+
+def test_backward_of_the_most_channels():
+    """One row of 2^30 - 8 channels: the first and the last against the oracle."""
+    C = (1 << 30) - 8
+    G, n = C // 8, 1 << 14
+    x, dy = (torch.empty(1, 1, C, dtype=BF, device="cuda").normal_() for _ in range(2))
+    mean, rstd = torch.zeros(1, G, device="cuda"), torch.ones(1, G, device="cuda")   # any will do
+    dx, dgb = torch.full_like(x, float("nan")), torch.full((2, C), float("nan"), device="cuda")
+    K.gn_bwd(dy, x, None, None, mean, rstd, dx, dgb, 1, 1, C, G, act=1)
+    for p, g in ((slice(0, n), slice(0, n // 8)), (slice(C - n, C), slice(G - n // 8, G))):
+        want, bound = O.bwd(dy[..., p].contiguous(), x[..., p].contiguous(), None, None, mean[:, g], rstd[:, g], 1, 1, n, n // 8, 1)
+        for got, w, b in zip((dx[..., p], dgb[0, p], dgb[1, p]), want, bound):
+            O.within(got, w, b)
+    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dgb).all())

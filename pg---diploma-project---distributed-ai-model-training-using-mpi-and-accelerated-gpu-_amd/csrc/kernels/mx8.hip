@@ -505,11 +505,13 @@ template <class T, bool ALN> void wgrad_go(const WgradPlan &p, const WgradArgs &
   else hipLaunchKernelGGL((mx8_wgrad_kernel<T, 64, ALN>), grid, dim3(256), 0, st, a);
 }
 
-unsigned slot_grid(long long M, long long slots) {
-  const long long n = (M * slots + kU * kThreads - 1) / (kU * kThreads);
-  if (n > 0x7fffffff) throw std::invalid_argument("mx8: M * C is too large");
-  return (unsigned)n;
-}
+// workgroups of kThreads a launch: the runtime takes 2^32 work-items and more without a word and runs what is left
+// modulo 2^32
+constexpr long long kMostWgs = 0xffffffffll / kThreads;
+
+long long slot_wgs(long long M, long long slots) { return (M * slots + kU * kThreads - 1) / (kU * kThreads); }
+// rows a launch: a multiple of 16, so that the next one's begin as aligned as the first's
+long long slot_rows(long long slots) { return kMostWgs * (kU * kThreads) / slots / 16 * 16; }
 // Values a thread (16 bytes of them, or 8 where rows are a multiple of that only), and whether rows begin
 // anywhere. 400000 rows of 140, 142, 143 and 144 bf16: pack 37, 52, 55, 34 us (one and two values a thread
 // took 65 for 142 and 126 for 143), unpack 32 each (45 and 78); of 142 fp32 in twos 61 and 55 (as if at
@@ -533,23 +535,31 @@ template <class T> static void pack_go(const void *x, uint8_t *q, uint8_t *qs, l
   const int nb = (C + kMxBlock - 1) / kMxBlock, full = 16 / (int)sizeof(T);
   const Lanes l(C, full);
   const FastDiv f((uint32_t)nb * (kMxBlock / l.V));
-  const dim3 grid(slot_grid(M, f.d));
-  with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
-    hipLaunchKernelGGL((mx8_pack_kernel<T, decltype(v)::value, decltype(any)::value>), grid, dim3(kThreads), 0, st,
-                       (const T *)x, q, qs, M, C, nb, f);
-  });
+  for (long long r = 0, most = slot_rows(f.d); r < M; r += most) {
+    const long long rows = std::min(most, M - r);
+    const dim3 grid((unsigned)slot_wgs(rows, f.d));
+    with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
+      hipLaunchKernelGGL((mx8_pack_kernel<T, decltype(v)::value, decltype(any)::value>), grid, dim3(kThreads), 0, st,
+                         (const T *)x + r * C, q + r * C, qs + r * nb, rows, C, nb, f);
+    });
+  }
 }
 template <class T> static void unpack_go(const uint8_t *q, const uint8_t *qs, void *x, long long M, int C, hipStream_t st) {
   const int nb = (C + kMxBlock - 1) / kMxBlock;
   const Lanes l(C, 16 / (int)sizeof(T));
   const FastDiv f((uint32_t)(l.any ? C : C / l.V));
-  const dim3 grid(l.any ? slot_grid(1, M * C / l.V + 1) : slot_grid(M, f.d));
-  with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
-    constexpr int V = decltype(v)::value;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, q, qs, (T *)x, M, C, nb, f); };
-    if constexpr (decltype(any)::value) go(mx8_unpack_run_kernel<T, V>);
-    else go(mx8_unpack_kernel<T, V>);
-  });
+  for (long long r = 0, most = slot_rows(f.d); r < M; r += most) {
+    const long long rows = std::min(most, M - r);
+    const dim3 grid((unsigned)(l.any ? slot_wgs(1, rows * C / l.V + 1) : slot_wgs(rows, f.d)));
+    with_lanes<16 / sizeof(T)>(l, [&](auto v, auto any) {
+      constexpr int V = decltype(v)::value;
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, q + r * C, qs + r * nb, (T *)x + r * C, rows, C, nb, f);
+      };
+      if constexpr (decltype(any)::value) go(mx8_unpack_run_kernel<T, V>);
+      else go(mx8_unpack_kernel<T, V>);
+    });
+  }
 }
 
 // dt: 0 bf16, 1 fp16, 2 fp32

@@ -227,3 +227,14 @@ def test_backward_of_the_most_channels():
         for got, w, b in zip((dx[..., p], dgb[0, p], dgb[1, p]), want, bound):
             O.within(got, w, b)
     assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dgb).all())
+
+
+def test_pack_of_more_rows_than_one_launch_has_workgroups_for():
+    M = (1 << 29) + 37
+    x = torch.full((M, 1), 3.0, dtype=BF, device="cuda")
+    x[-64:, 0] = randn(64).to(BF)
+    q, qs = torch.zeros(M, 1, dtype=torch.uint8, device="cuda"), torch.zeros(M, 1, dtype=torch.uint8, device="cuda")
+    K.mx8_pack(x, q, qs, M, 1)
+    wq, ws = O.pack(x[-100:])
+    assert torch.equal(q[-100:], wq) and torch.equal(qs[-100:], ws)
+    assert bool((q[:-64] == wq[0]).all()) and bool((qs[:-64] == ws[0]).all())

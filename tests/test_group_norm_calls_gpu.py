@@ -226,7 +226,8 @@ def test_backward_of_the_most_channels():
         want, bound = O.bwd(dy[..., p].contiguous(), x[..., p].contiguous(), None, None, mean[:, g], rstd[:, g], 1, 1, n, n // 8, 1)
         for got, w, b in zip((dx[..., p], dgb[0, p], dgb[1, p]), want, bound):
             O.within(got, w, b)
-    assert bool(torch.isfinite(dx).all()) and bool(torch.isfinite(dgb).all())
+    for t in (*dx.view(-1).split(1 << 26), *dgb.view(-1).split(1 << 26)):
+        assert bool(torch.isfinite(t).all())
 
 
 def test_pack_of_more_rows_than_one_launch_has_workgroups_for():

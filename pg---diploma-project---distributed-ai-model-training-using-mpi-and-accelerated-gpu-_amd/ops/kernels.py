@@ -1196,8 +1196,8 @@ def gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=GN_NONE, q=N
 def _mx8_check(what, t, M, C):
     if t.dtype not in _DT:
         raise TypeError(f"{what}: bf16, fp16 or fp32 values, got {t.dtype}")
-    if M < 0 or not 1 <= C <= _I31:
-        raise ValueError(f"{what}: M={M} C={C}: C must be positive, M 0 at least")
+    if M < 0 or not 1 <= C < 1 << 30:
+        raise ValueError(f"{what}: M={M} C={C}: C must be positive and below 2^30, M 0 at least")
 
 
 def mx8_pack(x, q, qs, M, C):

@@ -41,3 +41,14 @@ def test_sizes_past_the_grid_are_refused():
         with pytest.raises(ValueError, match="32-bit grid"):
             K.gn_workspace(1 << 24, 3136, 64, 8, torch.bfloat16, bwd)
         assert K.gn_workspace(1 << 27, 1, 8, 1, torch.bfloat16, bwd) >= 0   # images of their own: several launches
+
+
+@pytest.mark.parametrize("C", [1 << 30, (1 << 31) - 1, 1 << 31])
+def test_checkpoints_of_2_30_channels_and_more_are_refused(C):
+    """Their block counts pass 32 bits from 2^31 - 31 on."""
+    from pgdist.ops import kernels as K
+    x, q = torch.empty(0, dtype=torch.bfloat16), torch.empty(0, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="below 2\\^30"):
+        K.mx8_pack(x, q, q, 0, C)
+    with pytest.raises(ValueError, match="below 2\\^30"):
+        K.mx8_unpack(q, q, x, 0, C)

@@ -486,7 +486,7 @@ WgradPlan wgrad_plan(int M, int N, int K) {
   if (t > 0x7fffffff) throw std::invalid_argument("mx8_wgrad: N * K is too large");
   p.tn = (int)up(N, p.W);
   p.tk = (int)up(K, p.W);
-  const int steps = (M + kMK - 1) / kMK;
+  const long long steps = ((long long)M + kMK - 1) / kMK;
   // 512 workgroups (256: up to a fifth slower, 768 and 1024: no faster)
   long long s = std::max<long long>(1, std::min<long long>(512 / t, steps / 4));
   // whole turns; a split's rows, and as many steps on as are loaded, span less than 2^31 bytes

@@ -52,3 +52,10 @@ def test_checkpoints_of_2_30_channels_and_more_are_refused(C):
         K.mx8_pack(x, q, q, 0, C)
     with pytest.raises(ValueError, match="below 2\\^30"):
         K.mx8_unpack(q, q, x, 0, C)
+
+
+def test_wgrad_plans_for_the_most_rows():
+    from pgdist.ops import kernels as K
+    for M in ((1 << 31) - 64, (1 << 31) - 63, (1 << 31) - 1):
+        # 512 splits of 2^22 rows, each of 8 x 8 products and 8 sums
+        assert K.mx8_wgrad_workspace(M, 8, 8) == 512 * (8 * 8 + 8)

@@ -239,3 +239,15 @@ def test_pack_of_more_rows_than_one_launch_has_workgroups_for():
     wq, ws = O.pack(x[-100:])
     assert torch.equal(q[-100:], wq) and torch.equal(qs[-100:], ws)
     assert bool((q[:-64] == wq[0]).all()) and bool((qs[:-64] == ws[0]).all())
+
+
+def test_wgrad_of_the_most_rows():
+    """2^31 - 1 rows, ones but for a few: every sum is a whole number below 2^24 until the splits are joined."""
+    M = (1 << 31) - 1
+    dy = torch.zeros(M, 1, dtype=BF, device="cuda")
+    q, qs = torch.full((M, 1), 0x38, dtype=torch.uint8, device="cuda"), torch.full((M, 1), 127, dtype=torch.uint8, device="cuda")
+    at = torch.tensor([0, 63, 64, 12345678, (1 << 30) + 5, M - 2, M - 1], device="cuda")   # 0x38 is 1.0
+    dy[at, 0] = torch.arange(1, 8, device="cuda").to(BF)
+    dw, db = torch.empty(1, 1, device="cuda"), torch.empty(1, device="cuda")
+    K.mx8_wgrad(dy, q, qs, dw, M, 1, 1, db=db)
+    assert dw.item() == 28 and db.item() == 28

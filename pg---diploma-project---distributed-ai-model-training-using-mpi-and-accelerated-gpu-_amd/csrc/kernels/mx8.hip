@@ -23,6 +23,8 @@ struct FastDiv {
 // ANY: rows begin anywhere, and a row's last vector may be cut short: it is read from C - V on and shifted,
 // and its codes are written one by one.
 constexpr int kU = 4, kThreads = 256;
+// Work-items of a launch: the runtime takes 2^32 and more without a word and runs what is left modulo 2^32
+constexpr long long kMostItems = 0xffffffffll, kMostWgs = kMostItems / kThreads;
 
 // a workgroup's U * 256 slots of a [M][slots] grid: row and slot of the u-th of this thread
 struct Slots {
@@ -479,11 +481,10 @@ struct WgradPlan {
 // 128 x 128 take as long as 64 x 64 where they pad to a third more.
 WgradPlan wgrad_plan(int M, int N, int K) {
   WgradPlan p{};
-  auto up = [](int n, int w) { return (long long)((n + w - 1) / w); };
+  auto up = [](long long n, int w) { return (n + w - 1) / w; };
   const bool large = (double)M * N * K >= 8e9 && up(N, 128) * up(K, 128) * 4 * 3 <= up(N, 64) * up(K, 64) * 4;
   p.W = large ? 128 : 64;
   const long long t = up(N, p.W) * up(K, p.W);
-  if (t > 0x7fffffff) throw std::invalid_argument("mx8_wgrad: N * K is too large");
   p.tn = (int)up(N, p.W);
   p.tk = (int)up(K, p.W);
   const long long steps = ((long long)M + kMK - 1) / kMK;
@@ -496,6 +497,9 @@ WgradPlan wgrad_plan(int M, int N, int K) {
   p.rows = (int)(turns * kAhead * kMK);
   p.splits = (int)(((long long)M + p.rows - 1) / p.rows);
   p.pitch = ((long long)N * K + N + 3) / 4 * 4;
+  // the product's grid, and the join's: a work-item for every sum, in whole workgroups of 1024
+  if (t * p.splits > kMostWgs || (p.splits > 1 && p.pitch > kMostItems - 1023))
+    throw std::invalid_argument("mx8_wgrad: N * K is too large");
   return p;
 }
 
@@ -504,10 +508,6 @@ template <class T, bool ALN> void wgrad_go(const WgradPlan &p, const WgradArgs &
   if (p.W == 128) hipLaunchKernelGGL((mx8_wgrad_kernel<T, 128, ALN>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((mx8_wgrad_kernel<T, 64, ALN>), grid, dim3(256), 0, st, a);
 }
-
-// workgroups of kThreads a launch: the runtime takes 2^32 work-items and more without a word and runs what is left
-// modulo 2^32
-constexpr long long kMostWgs = 0xffffffffll / kThreads;
 
 long long slot_wgs(long long M, long long slots) { return (M * slots + kU * kThreads - 1) / (kU * kThreads); }
 // rows a launch: a multiple of 16, so that the next one's begin as aligned as the first's

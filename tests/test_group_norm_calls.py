@@ -59,3 +59,11 @@ def test_wgrad_plans_for_the_most_rows():
     for M in ((1 << 31) - 64, (1 << 31) - 63, (1 << 31) - 1):
         # 512 splits of 2^22 rows, each of 8 x 8 products and 8 sums
         assert K.mx8_wgrad_workspace(M, 8, 8) == 512 * (8 * 8 + 8)
+
+
+@pytest.mark.parametrize("M,N,Kd", [(20000, 1 << 16, 1 << 16), (100, 1 << 19, 1 << 19), (1, (1 << 31) - 1, 1), (1, 1, (1 << 31) - 1),
+                                    (1, (1 << 31) - 1, (1 << 31) - 1)])
+def test_wgrad_refuses_grids_that_would_not_run_whole(M, N, Kd):
+    from pgdist.ops import kernels as K
+    with pytest.raises(ValueError, match="too large"):
+        K.mx8_wgrad_workspace(M, N, Kd)

@@ -96,7 +96,10 @@ def resnet50(num_classes: int = 1000, pretrained: Optional[str] = None, **kw) ->
         sd = torch.load(pretrained, map_location="cpu", weights_only=True)
         if sd["fc.weight"].shape[0] != num_classes:
             sd = {k: v for k, v in sd.items() if not k.startswith("fc.")}
-            model.load_state_dict(sd, strict=False)
+            missing, unexpected = model.load_state_dict(sd, strict=False)
+            # the norms' weights have the same names in both kinds, batch statistics only one has
+            if any(k.endswith("running_mean") for k in (*missing, *unexpected)):
+                raise ValueError(f"{pretrained} holds another kind of norm than norm={model.norm!r}")
         else:
             model.load_state_dict(sd)
     return model

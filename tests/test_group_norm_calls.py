@@ -67,3 +67,19 @@ def test_wgrad_refuses_grids_that_would_not_run_whole(M, N, Kd):
     from pgdist.ops import kernels as K
     with pytest.raises(ValueError, match="too large"):
         K.mx8_wgrad_workspace(M, N, Kd)
+
+
+def test_pretrained_weights_of_the_other_norm_are_refused(tmp_path):
+    """With another number of classes too, where the head's weights are left out."""
+    from pgdist.models import build_model
+    path = str(tmp_path / "w.pth")
+    for name in ("mobilenet_v2", "resnet50"):
+        for saved, wanted in (("batch", "group"), ("group", "batch")):
+            torch.save(build_model(name, 10, norm=saved).state_dict(), path)
+            for classes in (10, 7):
+                with pytest.raises((ValueError, RuntimeError)):
+                    build_model(name, classes, pretrained=path, norm=wanted)
+                m = build_model(name, classes, pretrained=path, norm=saved)
+                sd = torch.load(path, weights_only=True)
+                assert all(torch.equal(v, sd[k]) for k, v in m.state_dict().items() if sd[k].shape == v.shape
+                           and not k.startswith(("fc.", "classifier.")))

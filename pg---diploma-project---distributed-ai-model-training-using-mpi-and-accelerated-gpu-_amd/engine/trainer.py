@@ -68,6 +68,8 @@ class Trainer:
         if backend == "hip" and cfg.norm != "batch":
             raise NotImplementedError("the native executors are built for BatchNorm; norm='group' runs on the torch "
                                       "backend (with the HIP group-norm kernels on a GPU)")
+        if cfg.precision == "fp8" and cfg.norm != "batch":
+            raise NotImplementedError("precision='fp8' needs the native executors, which norm='group' does not run on")
         if backend == "hip" and self.device.type != "cuda":
             raise RuntimeError("backend 'hip' needs a GPU")
         self.backend = backend

@@ -83,3 +83,12 @@ def test_pretrained_weights_of_the_other_norm_are_refused(tmp_path):
                 sd = torch.load(path, weights_only=True)
                 assert all(torch.equal(v, sd[k]) for k, v in m.state_dict().items() if sd[k].shape == v.shape
                            and not k.startswith(("fc.", "classifier.")))
+
+
+def test_trainer_refuses_fp8_with_group_norm():
+    """It would train in fp32 on the torch backend without a word."""
+    from pgdist.config import TrainConfig
+    from pgdist.engine.trainer import Trainer
+    with pytest.raises(NotImplementedError, match="fp8"):
+        Trainer(TrainConfig(data="synthetic", synthetic_train_size=8, synthetic_test_size=8, batch_size=8, img_size=32,
+                            device="cpu", norm="group", precision="fp8"))

@@ -111,6 +111,7 @@ void launch_reduce_metrics(const float *, const float *, int, double *, hipStrea
 // ---- group norm, 8-bit activation checkpoints (groupnorm.hip, mx8.hip) ----
 long long gn_workspace_floats(int, long long, long long, int, int, int);
 void gn_set_wait(int);
+int gn_form(int, long long, long long, int, int, int, int, int);
 void launch_gn_fwd(int, const void *, const float *, const float *, void *, float *, float *, uint8_t *, uint8_t *,
                    float *, long long, long long, int, int, float, int, int, hipStream_t);
 void launch_gn_bwd(int, const void *, const void *, const uint8_t *, const uint8_t *, const float *, const float *,
@@ -214,6 +215,7 @@ PYBIND11_MODULE(_pgdist_C, m) {
   // ---- group norm, 8-bit activation checkpoints ----
   m.def("gn_workspace_floats", &gn_workspace_floats);
   m.def("gn_set_wait", &gn_set_wait);
+  m.def("gn_form", &gn_form);
   m.def("gn_fwd", [](int dt, P x, P gamma, P beta, P y, P mean, P rstd, P q, P qs, P ws, long long B, long long S_,
                      int C, int G, float eps, int act, int as_ckpt8, P s) {
     pgdist_rt::run_op([=] {

@@ -361,6 +361,10 @@ void launch_mx8_pack(int dt, const void *x, uint8_t *q, uint8_t *qs, long long M
 
 // tests: -1, what has come is not looked at
 void gn_set_wait(int polls) { g_wait = polls; }
+// tests: the form (GnMode) that a call of these sizes takes
+int gn_form(int dt, long long B, long long S, int C, int G, int ck, int bwd, int act) {
+  return gn_plan(dt, B, S, C, G, ck && !bwd, bwd, bwd && act == GN_SILU).mode;
+}
 
 // dt: 0 bf16, 1 fp16, 2 fp32.  With and without a checkpoint (forward) or silu (backward): the largest.
 long long gn_workspace_floats(int dt, long long B, long long S, int C, int G, int bwd) {

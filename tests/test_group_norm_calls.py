@@ -92,3 +92,13 @@ def test_trainer_refuses_fp8_with_group_norm():
     with pytest.raises(NotImplementedError, match="fp8"):
         Trainer(TrainConfig(data="synthetic", synthetic_train_size=8, synthetic_test_size=8, batch_size=8, img_size=32,
                             device="cpu", norm="group", precision="fp8"))
+
+
+def test_forms_of_group_norm():
+    """SOLO, HELD, STAGED, WIDE by size, type and direction (bf16, fp16, fp32 are 0, 1, 2)."""
+    from pgdist.ops import kernels as K
+    form = K.lib().gn_form
+    assert form(0, 1, 49, 1280, 160, False, False, 0) == form(0, 1, 49, 1280, 160, False, True, 0) == 0
+    assert form(2, 7, 3249, 100, 10, False, False, 0) == form(0, 96, 784, 192, 24, True, True, 0) == 1
+    assert form(0, 128, 3136, 144, 18, True, False, 0) == form(0, 128, 12544, 96, 12, False, True, 0) == 2
+    assert form(0, 2, 9, 2049, 1, False, False, 0) == form(0, 2050, 2, 8200, 1, False, True, 0) == 3

@@ -251,3 +251,57 @@ def test_wgrad_of_the_most_rows():
     dw, db = torch.empty(1, 1, device="cuda"), torch.empty(1, device="cuda")
     K.mx8_wgrad(dy, q, qs, dw, M, 1, 1, db=db)
     assert dw.item() == 28 and db.item() == 28
+
+
+SOLO, HELD, STAGED, WIDE = range(4)
+
+
+def both_passes(size, dtype, act, ck_fwd, seed=0):
+    """Forward, and backward from x and (ck_fwd) from the checkpoint, against the oracle."""
+    B, S, C, G = size
+    x, dy = randn(B, S, C, seed=seed).to(dtype), randn(B, S, C, seed=seed + 1).to(dtype)
+    gamma, beta = 1 + 0.2 * randn(C, seed=seed + 2), 0.3 * randn(C, seed=seed + 3)
+    y, mean, rstd = torch.full_like(x, float("nan")), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+    q = torch.zeros(B * S, C, dtype=torch.uint8, device="cuda") if ck_fwd else None
+    qs = torch.zeros(B * S, K.mx8_blocks(C), dtype=torch.uint8, device="cuda") if ck_fwd else None
+    K.gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, act=act, q=q, qs=qs)
+    want, bound = O.fwd(x, gamma, beta, B, S, C, G, 1e-5, act)
+    for got, w, b in zip((y, mean, rstd), want, bound):
+        O.within(got, w, b)
+    if ck_fwd:
+        wq, ws = O.pack(x.view(B * S, C))
+        assert torch.equal(q, wq) and torch.equal(qs, ws)
+    for ck in (False, True) if ck_fwd else (False,):
+        dx, dgb = torch.full_like(x, float("nan")), torch.full((2, C), float("nan"), device="cuda")
+        K.gn_bwd(dy, None if ck else x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=act, q=q if ck else None,
+                 qs=qs if ck else None)
+        want, bound = O.bwd(dy, O.unpack(q, qs) if ck else x, gamma, beta, mean, rstd, B, S, C, G, act)
+        for got, w, b in zip((dx, dgb[0], dgb[1]), want, bound):
+            O.within(got, w, b)
+
+
+@pytest.mark.parametrize("size,dtype,ck,forms", [
+    ((2, 6001, 96, 12), BF, False, (HELD, HELD)), ((7, 3249, 100, 10), torch.float32, False, (HELD, HELD)),
+    ((4, 40001, 96, 12), BF, True, (STAGED, STAGED)), ((3, 50001, 33, 3), torch.float32, False, (STAGED, STAGED)),
+    ((2, 60001, 24, 3), torch.float16, True, (STAGED, HELD))])
+@pytest.mark.parametrize("act", [2, 3])
+def test_a_wait_that_is_given_up_in_every_form(size, dtype, ck, forms, act):
+    """Sums that are not waited for are taken from the tensor, held and staged, forward and backward. A lane then adds
+    n / 2 values in a row at most; roundings are as often up as down, so they add as a random walk, to sqrt(n / 2) u / 3,
+    which the oracle's (n / 64 + 32) u is six times of at least."""
+    lib, dt = K.lib(), {BF: 0, torch.float16: 1, torch.float32: 2}[dtype]
+    assert (lib.gn_form(dt, *size, ck, False, act), lib.gn_form(dt, *size, ck, True, act)) == forms
+    try:
+        lib.gn_set_wait(-1)
+        both_passes(size, dtype, act, ck)
+    finally:
+        lib.gn_set_wait(1 << 16)
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32])
+@pytest.mark.parametrize("size,ck", [((3, 400, 2048, 32), True), ((2, 784, 1920, 240), True), ((2, 300, 4096, 32), True),
+                                     ((2, 784, 625, 25), True), ((2, 600, 663, 39), True), ((2, 600, 663, 39), False),
+                                     ((2, 784, 1280, 160), True)])
+def test_wide_rows_of_long_maps(size, ck, dtype):
+    """2048 channels in 32 groups, and rows whose checkpoint blocks or sums do not fit one workgroup."""
+    both_passes(size, dtype, 1, ck, seed=20)

@@ -2,6 +2,7 @@
 the ends of their ranges."""
 import pytest
 import torch
+import torch.nn.functional as F
 
 import gn_oracle as O
 from pgdist.ops import kernels as K
@@ -305,3 +306,57 @@ def test_a_wait_that_is_given_up_in_every_form(size, dtype, ck, forms, act):
 def test_wide_rows_of_long_maps(size, ck, dtype):
     """2048 channels in 32 groups, and rows whose checkpoint blocks or sums do not fit one workgroup."""
     both_passes(size, dtype, 1, ck, seed=20)
+
+
+@pytest.mark.parametrize("act_ckpt", ["none", "mx8"])
+@pytest.mark.parametrize("name", ["mobilenet_v2", "resnet50"])
+def test_every_layer_of_a_model(name, act_ckpt):
+    """A training step under autocast: each norm's and each checkpointed 1x1 convolution's output and gradients against
+    the oracle on the operands that it had there. (Whole models are no measure: one relu that falls to the other side
+    moves gradients by a hundredth, in torch's own fp32 norms too.)"""
+    from pgdist.models import build_model
+    torch.manual_seed(0)
+    m = build_model(name, 10, norm="group", act_ckpt=act_ckpt).cuda().eval()
+    seen = []
+
+    def look(mod, args, y):
+        io = dict(mod=mod, x=args[0].detach(), y=y.detach().clone())   # the program may write into y
+        args[0].register_hook(lambda g: io.setdefault("dx", g)) if args[0].requires_grad else None
+        y.register_hook(lambda g: io.setdefault("dy", g))
+        seen.append(io)
+
+    for mod in m.modules():
+        if isinstance(mod, (N.GroupNormAct, N.Conv1x1Ckpt8)):
+            mod.register_forward_hook(look)
+    x = randn(4, 3, 64, 64).contiguous(memory_format=torch.channels_last)
+    with torch.autocast("cuda", dtype=BF):
+        out = m(x)
+    F.cross_entropy(out.float(), torch.tensor([0, 1, 2, 3], device="cuda")).backward()
+    assert len(seen) == sum(isinstance(mod, (N.GroupNormAct, N.Conv1x1Ckpt8)) for mod in m.modules()) > 50
+    for io in seen:
+        mod, (B, C) = io["mod"], io["x"].shape[:2]
+        S = io["x"][0, 0].numel()
+        rows = lambda t: t.movedim(1, -1).contiguous()  # noqa: E731
+        if isinstance(mod, N.GroupNormAct):
+            G, act = mod.num_groups, N.ACTS[mod.act]
+            xr, w, b = rows(io["x"]).view(B, S, C), mod.weight.detach(), mod.bias.detach()
+            y, mean, rstd = torch.empty_like(xr), torch.empty(B, G, device="cuda"), torch.empty(B, G, device="cuda")
+            K.gn_fwd(xr, w, b, y, mean, rstd, B, S, C, G, eps=mod.eps, act=act, as_ckpt8=mod.ckpt8)
+            assert torch.equal(rows(io["y"]).view(B, S, C), y)
+            want, bound = O.fwd(xr, w, b, B, S, C, G, mod.eps, act)
+            O.within(y, want[0], bound[0])
+            v = O.unpack(*O.pack(xr.view(B * S, C))) if mod.ckpt8 else xr
+            want, bound = O.bwd(rows(io["dy"]).view(B, S, C), v, w, b, mean, rstd, B, S, C, G, act)
+            O.within(rows(io["dx"]).view(B, S, C), want[0], bound[0])
+            O.within(mod.weight.grad, want[1], bound[1])
+            O.within(mod.bias.grad, want[2], bound[2])
+        else:
+            assert mod.bias is None
+            xr = rows(io["x"].to(BF)[:, :, ::mod.stride[0], ::mod.stride[1]]).view(-1, C)
+            d, w, M = rows(io["dy"]).view(len(xr), -1).double(), mod.weight.detach().view(-1, C).to(BF).double(), len(xr)
+            y = rows(io["y"]).view(M, -1)
+            want, mag = xr.double() @ w.t(), xr.double().abs() @ w.abs().t()
+            O.within(y, want, O.half(BF) * want.abs() + (C + 1) * O.U * mag)
+            X = O.unpack(*O.pack(xr))
+            want, mag = d.t().contiguous() @ X, d.abs().t().contiguous() @ X.abs()
+            O.within(mod.weight.grad.view(-1, C), want, (M + 64) * O.U * mag)

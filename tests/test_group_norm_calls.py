@@ -1,8 +1,12 @@
 """Group norm and 8-bit checkpoints as programs call them, without a GPU: arguments, checkpoints of models, plans."""
+import os
+
 import pytest
 import torch
+import torch.distributed as dist
 import torch.nn.functional as F
 
+from mp_util import free_port, run_ranks
 from pgdist.ops import nn as N
 
 
@@ -102,3 +106,26 @@ def test_forms_of_group_norm():
     assert form(2, 7, 3249, 100, 10, False, False, 0) == form(0, 96, 784, 192, 24, True, True, 0) == 1
     assert form(0, 128, 3136, 144, 18, True, False, 0) == form(0, 128, 12544, 96, 12, False, True, 0) == 2
     assert form(0, 2, 9, 2049, 1, False, False, 0) == form(0, 2050, 2, 8200, 1, False, True, 0) == 3
+
+
+def _train_two_ranks(rank, world, port, tmp, bn_sync, q):
+    import pgdist  # noqa: F401
+    from pgdist.config import TrainConfig
+    from pgdist.engine.trainer import Trainer
+    from pgdist.parallel.bootstrap import DistInfo
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    info = DistInfo(rank=rank, world_size=world, local_rank=rank, local_world_size=world, master_port=port)
+    tr = Trainer(TrainConfig(data="synthetic", synthetic_train_size=32, synthetic_test_size=16, batch_size=8, epochs=1,
+                             img_size=32, device="cpu", backend="torch", precision="fp32", augment="none", norm="group",
+                             act_ckpt="mx8", save_path=os.path.join(tmp, "b.pth"), log_format="ddp", seed=42,
+                             bn_sync=bn_sync), info=info)
+    tr.fit()
+    q.put(("ok", rank, tr.replicas_ok, tr.history[-1]["train_images"]))
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("bn_sync", ["eval", "broadcast"])
+def test_two_ranks_train_without_batch_statistics(tmp_path, bn_sync):
+    """There are no buffers to broadcast or compare."""
+    for _, rank, ok, n in run_ranks(_train_two_ranks, 2, (2, free_port(), str(tmp_path), bn_sync), expect=2, timeout=300):
+        assert ok == (True, True) and n == 32

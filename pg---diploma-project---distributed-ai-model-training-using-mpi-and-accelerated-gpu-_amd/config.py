@@ -24,7 +24,8 @@ class TrainConfig:
     pretrained: Optional[str] = None          # path to a torchvision-format state_dict
     img_size: int = 224                       # IMG_SIZE (:28)
     norm: str = "batch"                       # batch | group (group norm; torch backend)
-    act_ckpt: str = "none"                    # none | mx8 (with group: activations kept for backward in 8 bits)
+    act_ckpt: str = "none"                    # none | mx8 (with group: activations kept for backward in 8 bits;
+    #                                           in fp32 those of norms only)
     # optimisation (reference :75-77)
     batch_size: int = 128                     # per process
     epochs: int = 20

@@ -9,19 +9,28 @@
 //   solo     a workgroup holds all S rows of a slab of whole groups in registers: one read
 //   held     the S rows are k tiles, and all tiles of the tensor are so few that their workgroups run
 //            together: each keeps its tile in registers, publishes its sums, waits for the k - 1
-//            others of its image and goes on.  One read.  (96 x 784 x 192 from a checkpoint, backward: 27
+//            others of its image and goes on.  One read.  (96 x 784 x 192 from a checkpoint, backward: 26
 //            us a call, 33 staged.  With more tiles than fit, a workgroup's chain load - sum - publish -
 //            wait - join - store is not hidden behind others': 128 x 12544 x 96 backward 1129 us.)
 //   staged   longer maps: the S rows are k tiles.  One launch holds a sums and a use workgroup for
 //            every tile; the use of an image's tiles is queued `lead` tiles behind its sums, so
 //            that it hardly ever waits for them and finds the tile in the memory-side cache
 //            (256 MB).  HBM sees every value once: 128 x 12544 x 96 backward reads 607 MB and
-//            writes 308 in 226 us, 4.1 TB/s; 128 x 3136 x 144 forward with checkpoint 289 MB in 75 us,
-//            3.8 TB/s.  What is left of a copy's 5.1 TB/s goes to a workgroup's latencies.
-//   wide     a group has more vectors than a workgroup has threads: plain kernels (groupnorm.hip),
-//            one workgroup per (image, group), then one value a thread.
+//            writes 308 in 230 us, 4.0 TB/s; 128 x 3136 x 144 forward with checkpoint 289 MB in 75 us,
+//            3.8 TB/s.  What is left of a copy's 5.1 TB/s goes to a workgroup's latencies and, as the
+//            checkpointed forward's counters have it, to the issue of its vector instructions (more
+//            than half of their units' time).  Not so for wide rows on long maps: a use workgroup reads all k pairs of
+//            each of its groups, and a tile has few rows there (8 x 9765 x 1280 in 160 groups, backward:
+//            k = 814, 1 MB of pairs for a tile of 61 KB; 2.0 ms, 117 us of it for the tensors' bytes).
+//   wide     what no workgroup holds: a slab (whole groups, vectors and, where one is written, checkpoint
+//            blocks) of more vectors than threads, or whose sums pass 64 KB of shared memory (backward, bf16
+//            and fp16: some 1900 to 2048 channels and other slabs of that width; 625 channels in 25 groups
+//            with a checkpoint).  Plain kernels (groupnorm.hip): a workgroup at a time per (image, group),
+//            then one value a thread.  32 x 784 x 2048 in 32 groups, backward: 705 us; 1880 channels, staged,
+//            398.
 // A thread owns one vector of V channels (16 bytes where C allows) and every R-th row of the tile.
-// Sums are taken in a fixed order, so results do not vary from run to run.
+// Sums are taken in a fixed order, so results do not vary from run to run, unless a wait for other workgroups'
+// sums is given up: those sums are then taken from the tensor, in another order (right, but other last bits).
 #pragma once
 #include "mx8.h"
 #include "vec.h"

@@ -14,8 +14,10 @@ namespace {
 constexpr long long kMostItems = 0xffffffffll;
 constexpr long long kMostWgs = 65536;   // of kernels that loop: more than are resident, many times over
 
-// ---- wide groups: not tuned, every access one value -----------------------------------------------
-// Plain loops over memory, with grids of kMostWgs workgroups at most: C / G of thousands of channels, or over a thousand of an odd number.
+// ---- wide: not tuned, every access one value ------------------------------------------------------
+// Plain loops over memory, with grids of kMostWgs workgroups at most, for slabs that no workgroup holds: C / G of
+// thousands of channels, or over a thousand of an odd number; sums past the shared memory; checkpoint blocks of odd
+// widths (groupnorm.h).
 PG_DEVICE float load_one(const void *x, int dt, long long i) {
   return dt == 0 ? bf2f(static_cast<const bf16_t *>(x)[i])
                  : dt == 1 ? (float)static_cast<const _Float16 *>(x)[i] : static_cast<const float *>(x)[i];

@@ -187,13 +187,13 @@ __global__ __launch_bounds__(kThreads) void mx8_unpack_run_kernel(const uint8_t 
 // scales change with the row, so they are decoded on their way into shared memory: to bf16 exactly
 // (4 significant bits), 2 an instruction.
 //   tile     W x W outputs, 4 waves of a quarter each; 64 rows a step, two buffers in shared memory and
-//            two steps in registers or on their way (25088 x 1024 x 1024: kernel 83 us; 100 with one, and
+//            two steps in registers or on their way (25088 x 1024 x 1024: kernel 85 us; 100 with one, and
 //            with four the registers' moves cost more than is gained; 91 with 256 x 256 and 8 waves)
 //   rows     of the tile in shared memory keep their 32-byte pieces in an order that depends on the
 //            row (wg_swz), so that transposed reads meet no bank twice
 //   split    the M rows are cut into `splits` so that every CU has two workgroups; each writes a
 //            partial [N * K + N] and a second kernel adds them in order
-// A call with its join: 25088 x 1024 x 1024 80 us, 655 TFLOP/s (a step's reads, decoding, products and barrier
+// A call with its join: 25088 x 1024 x 1024 81 us, 650 TFLOP/s (a step's reads, decoding, products and barrier
 // follow one another, and two workgroups a CU hide half of it); 401408 x 144 x 24 37 us, 3.4 TB/s; 128 x 1000 x
 // 2048 7 us, most of it the launch and the first loads' latency.
 // ---------------------------------------------------------------------------

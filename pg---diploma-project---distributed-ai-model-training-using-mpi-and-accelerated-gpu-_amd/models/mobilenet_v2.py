@@ -110,8 +110,8 @@ class MobileNetV2(nn.Module):
     def __init__(self, num_classes: int = 1000, width_mult: float = 1.0,
                  dropout: float = 0.2, round_nearest: int = 8, norm: str = "batch", act_ckpt: str = "none"):
         """``norm``: batch, or group (groups of 8 channels, nothing kept between batches or exchanged
-        between ranks).  ``act_ckpt="mx8"`` (with group): norms and 1x1 convolutions keep their
-        inputs for the backward pass in 8 bits."""
+        between ranks).  ``act_ckpt="mx8"`` (with group): norms and, in half precision or under
+        autocast, 1x1 convolutions keep their inputs for the backward pass in 8 bits."""
         super().__init__()
         check_variant(norm, act_ckpt)
         if norm == "group" and round_nearest % 8:

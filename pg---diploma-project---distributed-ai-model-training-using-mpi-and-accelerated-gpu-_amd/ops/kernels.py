@@ -1138,7 +1138,9 @@ def gn_fwd(x, gamma, beta, y, mean, rstd, B, S, C, G, eps=1e-5, act=GN_NONE, q=N
     None.  With q, qs the 8-bit checkpoint of x (:func:`mx8_pack` of [B*S, C]) is also written.
     ``as_ckpt8`` without them: sums in the order of a call with them, so that y, mean and rstd have its bits.
     ``ws``: :func:`gn_workspace` floats for this call alone; None takes them from the allocator.
-    No output may overlap another operand.  S = 0 gives mean 0, rstd 1/sqrt(eps)."""
+    No output may overlap another operand.  S = 0 gives mean 0, rstd 1/sqrt(eps).  Tensors of more
+    tiles than one grid holds (2^32 threads, of some 270 GB) and rows so wide that a tile passes 2^31
+    bytes (2^28 channels of bf16, longer for few rows) are refused with ValueError."""
     _gn_check("gn_fwd", x, B, S, C, G, act)
     if not 2.0 ** -126 <= eps < float("inf"):
         raise ValueError(f"gn_fwd: eps={eps} must be a positive normal fp32 number")
@@ -1167,7 +1169,8 @@ def gn_bwd(dy, x, gamma, beta, mean, rstd, dx, dgb, B, S, C, G, act=GN_NONE, q=N
     """Backward of :func:`gn_fwd` from dy and either x or (x None) its 8-bit checkpoint q, qs, whose
     decoded values then stand for x; mean / rstd as gn_fwd wrote them.  dx [B, S, C] in dy's type,
     dgb fp32 [2, C] = (dgamma, dbeta), overwritten, or None where neither is wanted.  Sums are in
-    fp32 in a fixed order.  On which side of relu's or relu6's borders a value lies is decided from
+    fp32 in a fixed order (the same bits, unless a workgroup gives up its wait for others' sums and
+    takes them from the tensor in another).  On which side of relu's or relu6's borders a value lies is decided from
     the operands in 64 bits where fp32 could tell it wrongly.  ``ws``: as gn_fwd (bwd=True)."""
     _gn_check("gn_bwd", dy, B, S, C, G, act)
     if (q is None) != (qs is None) or (x is None) == (q is None):
@@ -1205,7 +1208,7 @@ def mx8_pack(x, q, qs, M, C):
     uint8 [M, mx8_blocks(C)] the biased exponents (e + 127) of one power-of-two scale per 32
     channels of a row; x ~ code * 2^e.  e is the least exponent at which the block's largest finite
     magnitude is at most 448 * 2^e (within [-117, 120]), so nothing saturates; codes round to
-    nearest even; NaN and infinities become NaN."""
+    nearest even; NaN and infinities become NaN.  C is below 2^30."""
     _mx8_check("mx8_pack", x, M, C)
     n, ns = M * C, M * mx8_blocks(C)
     px, pq, ps = _operand(x, "x", x.dtype, n), _operand(q, "q", torch.uint8, n), _operand(qs, "qs", torch.uint8, ns)
@@ -1243,7 +1246,9 @@ def mx8_wgrad(dy, q, qs, grad, M, N, K, db=None, ws=None):
     the checkpoint q, qs of [M, K]: grad [N, K] (fp32, overwritten) = dy^T x~, and db [N] (fp32) =
     the column sums of dy.  dy [M, N] bf16 or fp16; x~ is decoded inside the product (exact in
     bf16; in fp16 as :func:`mx8_unpack`).  fp32 accumulation in a fixed order.  ``ws``:
-    :func:`mx8_wgrad_workspace` floats for this call alone; None takes them from the allocator."""
+    :func:`mx8_wgrad_workspace` floats for this call alone; None takes them from the allocator.
+    Where N or K is no multiple of 8, dy and q are read in aligned 4-byte words: up to 3 bytes behind
+    their ends, in the same word, are read too, and take no part."""
     if dy.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"mx8_wgrad: dy bf16 or fp16, got {dy.dtype}")
     _wgrad_sizes("mx8_wgrad", M, N, K)

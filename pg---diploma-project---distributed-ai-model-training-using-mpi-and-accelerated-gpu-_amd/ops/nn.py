@@ -2,7 +2,7 @@
 
 ``group_norm_act`` and ``conv1x1`` take tensors as a module has them (any strides, any device, channels
 first in shape) and hand channels-last operands to the kernels; a ``channels_last`` tensor is not
-copied.  On a CPU tensor they are the plain torch operations, with exact gradients.
+copied.  Outputs are channels last, and code may write into them.  On a CPU tensor they are the plain torch operations, with exact gradients.
 """
 import contextlib
 from typing import Tuple, Union
@@ -90,7 +90,8 @@ class _GroupNormAct(torch.autograd.Function):
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", ckpt8=False):
-    """act(group_norm(x)) of [B, C, ...] with its gradients.  act: none, relu, relu6 or silu.
+    """act(group_norm(x)) of [B, C, ...] with its gradients.  act: none, relu, relu6 or silu.  On the
+    GPU x is bf16, fp16 or fp32; weight and bias are [C] of any floating type.
     ``ckpt8``: the backward pass keeps x as its 8-bit checkpoint (kernels.mx8_pack) instead of as it
     is, and its gradients are those of the values that stands for.  Without gradients none is made, and
     the result has the same bits."""
@@ -177,8 +178,9 @@ class _Conv1x1(torch.autograd.Function):
 def conv1x1(x, weight, bias=None, stride=1):
     """1x1 convolution of [B, C, H, W] (weight [N, C, 1, 1]; stride one number or one a direction) whose
     backward pass keeps its input as the 8-bit checkpoint (kernels.mx8_pack): dW and db come from
-    kernels.mx8_wgrad.  On the GPU in bf16 or fp16 (the input's type, or autocast's); any other call is
-    the plain convolution."""
+    kernels.mx8_wgrad.  On the GPU in bf16 or fp16 (the input's type, or autocast's); any other call,
+    in fp32 above all, is the plain convolution, which keeps its input as it is.  Where no gradient is
+    wanted no checkpoint is made."""
     stride = tuple(stride) if isinstance(stride, (tuple, list)) else (stride,)
     stride = stride * 2 if len(stride) == 1 else stride
     if len(stride) != 2 or min(stride) < 1:

@@ -16,12 +16,11 @@ def randn(*shape, seed=0):
     return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
 
 
-@pytest.mark.parametrize("layout", ["channels_last", "contiguous", "rows"])
-@pytest.mark.parametrize("op", ["norm", "norm_ckpt8", "conv"])
+@pytest.mark.parametrize("op,layout", [(op, layout) for op in ("norm", "norm_ckpt8", "conv")
+                                       for layout in ("channels_last", "contiguous", "rows")
+                                       if (op, layout) != ("conv", "rows")])
 def test_in_place_code_behind_an_output(op, layout):
     """relu_ and += on an output give the bits and gradients that the same code gives out of place."""
-    if op == "conv" and layout == "rows":
-        pytest.skip("a 1x1 convolution takes images")
     shape = (3, 32, 50) if layout == "rows" else (3, 32, 9, 7)
     x = randn(*shape).to(BF)
     if layout == "channels_last":
